@@ -12,7 +12,9 @@ CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(CSRC, "libglenet_hip.so")
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 FLAGS = ["-O3", "--offload-arch=gfx950", "-fPIC", "-std=c++17", "-ffp-contract=off",
-         "-Wall", "-Wno-unused-function", "-Wno-unused-variable"]
+         "-Wall", "-Wno-unused-function", "-Wno-unused-variable",
+         # no packed fp32 arithmetic: some forms of v_pk_add / mul / fma_f32 have given wrong results on this part now and then
+         "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 FLAGS += os.environ.get("GLX_HIPCC_EXTRA", "").split()      # experiments: e.g. -DBN_THREADS=512
 
 
