@@ -46,7 +46,8 @@ def load():
                  "glx_deconv_packed_bytes", "glx_deconv_wgrad_workspace_bytes", "glx_pair_lists_bytes",
                  "glx_sconv_wgrad_pairs_workspace_bytes", "glx_pointmax_wsum_workspace_bytes", "glx_rows128_moments_workspace_bytes", "glx_rows_bwd_64_128_workspace_bytes",
                  "glx_head1x1_wgrad_workspace_bytes", "glx_topk_workspace_bytes", "glx_fc_tower_scratch_bytes",
-                 "glx_bn_cm_workspace_bytes", "glx_rows_linear_workspace_bytes", "glx_narrowfeat_workspace_bytes", "glx_point_layer1_workspace_bytes", "glx_flat_l2_workspace_bytes"):
+                 "glx_bn_cm_workspace_bytes", "glx_rows_linear_workspace_bytes", "glx_narrowfeat_workspace_bytes", "glx_point_layer1_workspace_bytes", "glx_flat_l2_workspace_bytes",
+                 "glx_layer_norm_workspace_bytes"):
         if hasattr(lib, name):
             getattr(lib, name).restype = c_size_t
     lib.glx_index_words.restype = c_int64
@@ -86,6 +87,34 @@ def call(name, *args):
     if rc != 0:
         raise GlxError("%s failed (%d): %s" % (name, rc, lib.glx_last_error().decode()))
     return rc
+
+
+def call_on(device, name, *args):
+    """call() on `device`'s current stream: tensors may live on another device than the current one."""
+    if device.index is None or device.index == torch.cuda.current_device():
+        return call(name, *args)
+    with torch.cuda.device(device):
+        return call(name, *args)
+
+
+DTYPE_CODES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}       # GLX_F32 / GLX_BF16 / GLX_F16
+
+
+def dtype_code(dtype):
+    return DTYPE_CODES[dtype]
+
+
+def check_device(who, *tensors):
+    """The tensors (None: not given) are device tensors of ONE device."""
+    first = None
+    for t in tensors:
+        if t is None:
+            continue
+        if not t.is_cuda:
+            raise GlxError("%s: expected device tensors (HIP), got %s; there is no CPU path" % (who, t.device))
+        if first is not None and t.device != first:
+            raise GlxError("%s: tensors on %s and %s" % (who, first, t.device))
+        first = t.device
 
 
 def call_nostream(name, *args):

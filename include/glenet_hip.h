@@ -38,6 +38,11 @@ extern "C" {
 #define GLX_EHIP (-2)       /* HIP runtime / launch failure */
 #define GLX_EWORKSPACE (-3) /* workspace too small */
 
+/* Element types of the entry points that take more than fp32 (their `dtype` arguments). */
+#define GLX_F32 0
+#define GLX_BF16 1
+#define GLX_F16 2
+
 /* Message of the last failing call on this host thread ("" if none). */
 const char* glx_last_error(void);
 /* Library ABI version (bumped on any signature change). */
@@ -1477,6 +1482,19 @@ int glx_fc_tower_backward(const glx_fc_tower* t, const glx_fc_tower_grads* g, vo
 int glx_gather_proposals(const float* cand, const float* top, const int64_t* lab, const int64_t* order,
                          const int64_t* keep, const int* num, int F, int A, int K, int keep_stride, int P, int C,
                          float* rois, float* scores, int64_t* labels, void* stream);
+
+/* ---- layer norm: y = (x - mean) / sqrt(var + eps) * weight + bias over the last dimension (glenet_amd/norm.py) ----
+ * x (rows, width) with `ldx` elements between rows, y (rows, width) dense, both of `dtype`; weight / bias (width) of `wdtype`
+ * (GLX_F32 or `dtype`; either may be NULL: 1 / 0).  Statistics in fp32 over the biased variance; mean / rstd (rows) fp32 are
+ * what the backward pass reads (both NULL: inference).  Any width >= 1, any address that is a multiple of the element. */
+int glx_layer_norm_forward(const void* x, int64_t ldx, int dtype, const void* weight, const void* bias, int wdtype,
+                           int64_t rows, int64_t width, float eps, void* y, float* mean, float* rstd, void* stream);
+/* dx (rows, width) dense, dweight / dbias (width) of `wdtype`; any of the three may be NULL.  gy (rows, width) with `ldg`
+ * elements between rows.  The two column sums are formed in fp32 in a fixed order (no atomics). */
+size_t glx_layer_norm_workspace_bytes(int64_t rows, int64_t width);
+int glx_layer_norm_backward(const void* gy, int64_t ldg, const void* x, int64_t ldx, int dtype, const void* weight, int wdtype,
+                            const float* mean, const float* rstd, int64_t rows, int64_t width, void* dx, void* dweight,
+                            void* dbias, void* workspace, size_t workspace_bytes, void* stream);
 
 /* Stage stamps: a one-thread launch on `stream` that stores the device's constant 100 MHz wall clock into
  * stamps[slot] (10 ns per tick).  Recorded into a captured training step at its stage boundaries
