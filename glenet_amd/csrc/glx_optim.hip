@@ -155,6 +155,104 @@ extern "C" int glx_adamw_clip_step_scaled(float* params, const float* grads, flo
   return GLX_OK;
 }
 
+// ------------------------------------------------------------------------------------------------ orthogonalised updates
+// Update of a flat buffer whose weight MATRICES take orthogonalised momentum steps and whose other tensors take AdamW's
+// (glenet_amd.optim.FlatMuon).  chunks[i] covers up to OPT_CHUNK elements of one tensor; scale > 0: of a matrix.
+//   k_muon_moments : clip; AdamW where scale = 0; else m += (1 - b1)(g - m), u = g + b1 (m - g) (the look-ahead form) or m
+//   (glx_orthogonalize on the matrices' u, in place)
+//   k_muon_apply   : p = p (1 - lr wd) - lr scale u
+// An m x n matrix of orthonormal rows has entries of RMS 1 / sqrt(max(m, n)); scale = 0.2 sqrt(max(m, n)) gives the step the
+// RMS that AdamW's has in practice, so one learning rate and one decay serve both kinds.  Both launches are bound by memory
+// (5 and 3 x 4 bytes per element of a matrix).
+#define OPT_CHUNK 4096
+__global__ __launch_bounds__(OPT_THREADS) void k_muon_moments(float* __restrict__ p, const float* __restrict__ g,
+                                                              float* __restrict__ m, float* __restrict__ v, float* __restrict__ u,
+                                                              const glx_opt_chunk* __restrict__ chunks,
+                                                              const float* __restrict__ hyper, float beta2, float eps, float wd,
+                                                              float max_norm, float grad_scale, int lookahead,
+                                                              const int* __restrict__ step, const double* __restrict__ partial,
+                                                              int nparts, float* __restrict__ norm_out) {
+  __shared__ float s_coef;
+  __shared__ double s_wave[OPT_THREADS / 64];
+  double mine = 0;
+  for (int i = threadIdx.x; i < nparts; i += OPT_THREADS) mine += partial[i];
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) mine += __shfl_xor(mine, o, 64);
+  if ((threadIdx.x & 63) == 0) s_wave[threadIdx.x >> 6] = mine;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    double s = 0;
+    for (int i = 0; i < OPT_THREADS / 64; ++i) s += s_wave[i];
+    const float total = (float)sqrt(s);
+    const float coef = max_norm > 0.f ? max_norm / (total + 1e-6f) : 1.f;
+    s_coef = coef > 1.f ? 1.f : coef;
+    if (blockIdx.x == 0 && norm_out) *norm_out = total;
+  }
+  __syncthreads();
+  const float coef = s_coef, lr = hyper[0], b1 = hyper[1];
+  const glx_opt_chunk c = chunks[blockIdx.x];
+  if (c.scale > 0.f) {
+    for (int i = threadIdx.x; i < c.len; i += OPT_THREADS) {
+      const long long e = c.start + i;
+      const float gi = (g[e] * grad_scale) * coef;
+      const float me = m[e] + (gi - m[e]) * (1.f - b1);
+      m[e] = me;
+      u[e] = lookahead ? gi + (me - gi) * b1 : me;
+    }
+    return;
+  }
+  const int t = *step;
+  const float bc1 = 1.f - powf(b1, (float)t), bc2 = 1.f - powf(beta2, (float)t);
+  const float step_size = lr / bc1, bc2_sqrt = sqrtf(bc2), decay = 1.f - lr * wd;
+  for (int i = threadIdx.x; i < c.len; i += OPT_THREADS) {
+    const long long e = c.start + i;
+    const float gi = (g[e] * grad_scale) * coef;
+    const float me = m[e] + (gi - m[e]) * (1.f - b1);
+    const float ve = v[e] * beta2 + (1.f - beta2) * gi * gi;
+    p[e] = p[e] * decay - step_size * (me / (sqrtf(ve) / bc2_sqrt + eps));
+    m[e] = me; v[e] = ve;
+  }
+}
+__global__ __launch_bounds__(OPT_THREADS) void k_muon_apply(float* __restrict__ p, const float* __restrict__ u,
+                                                            const glx_opt_chunk* __restrict__ chunks,
+                                                            const float* __restrict__ hyper, float wd) {
+  const glx_opt_chunk c = chunks[blockIdx.x];
+  if (!(c.scale > 0.f)) return;
+  const float lr = hyper[0], decay = 1.f - lr * wd, size = lr * c.scale;
+  for (int i = threadIdx.x; i < c.len; i += OPT_THREADS) p[c.start + i] = p[c.start + i] * decay - size * u[c.start + i];
+}
+
+extern "C" int glx_muon_moments(float* params, const float* grads, float* exp_avg, float* exp_avg_sq, float* update, int64_t n,
+                                const glx_opt_chunk* chunks, int nchunks, const float* hyper, float beta2, float eps,
+                                float weight_decay, float max_norm, float grad_scale, int lookahead, int32_t* step,
+                                float* norm_out, void* workspace, size_t workspace_bytes, void* stream) {
+  GLX_REQUIRE(n >= 0 && nchunks >= 0 && (nchunks == 0 || (params && grads && exp_avg && exp_avg_sq && update && chunks)) && hyper && step,
+              "glx_muon_moments: null pointer");
+  GLX_REQUIRE(((uintptr_t)grads & 15) == 0, "glx_muon_moments: the gradients must be 16-byte aligned");
+  if (!workspace || workspace_bytes < glx_adamw_workspace_bytes() - 256) {
+    glx_set_error("glx_muon_moments: workspace %zu < %zu bytes", workspace_bytes, glx_adamw_workspace_bytes() - 256);
+    return GLX_EWORKSPACE;
+  }
+  if (n == 0 || nchunks == 0) return GLX_OK;
+  hipStream_t st = (hipStream_t)stream;
+  const int blocks = opt_blocks(n);
+  hipLaunchKernelGGL(k_gradnorm_partial, dim3(blocks), dim3(OPT_THREADS), 0, st, grads, (long long)n, grad_scale,
+                     (double*)workspace, step);
+  hipLaunchKernelGGL(k_muon_moments, dim3(nchunks), dim3(OPT_THREADS), 0, st, params, grads, exp_avg, exp_avg_sq, update, chunks,
+                     hyper, beta2, eps, weight_decay, max_norm, grad_scale, lookahead, (const int*)step, (const double*)workspace,
+                     blocks, norm_out);
+  GLX_LAUNCH_CHECK();
+  return GLX_OK;
+}
+extern "C" int glx_muon_apply(float* params, const float* update, const glx_opt_chunk* chunks, int nchunks, const float* hyper,
+                              float weight_decay, void* stream) {
+  GLX_REQUIRE(nchunks >= 0 && (nchunks == 0 || (params && update && chunks)) && hyper, "glx_muon_apply: null pointer");
+  if (nchunks == 0) return GLX_OK;
+  hipLaunchKernelGGL(k_muon_apply, dim3(nchunks), dim3(OPT_THREADS), 0, (hipStream_t)stream, params, update, chunks, hyper, weight_decay);
+  GLX_LAUNCH_CHECK();
+  return GLX_OK;
+}
+
 // ------------------------------------------------------------------------------------------------ sum of the tensors' 2-norms
 // The regulariser of cvae_uncertainty/model.py:20-28 (`l2_regularisation`: the SUM over a module's parameter tensors of their 2-norms)
 // on a flat parameter buffer whose tensors are the segments segs[i] = (start, length): one block per tensor for the norms (fixed

@@ -1,0 +1,687 @@
+// Orthogonalised updates (glenet_amd/optim.py): Newton-Schulz steps on a list of matrices of any shapes, few launches for all.
+//
+//   X = G / (|G|_F + eps), transposed where G has more rows than columns (X: m x n, m <= n);  per step
+//   A = X X^T,  X <- a X + (b A + c A^2) X  =  P X,  P = a I + b A + c A^2
+//
+// The next step's Gram matrix is P A P, and every P is a polynomial of the first A: a SEGMENT of s steps runs on m x m matrices
+// alone (P = aI + bA + cA^2;  H = P A;  A <- H P;  Q <- P Q) and touches X twice, A = X X^T before and X <- Q X behind.  With
+// symmetric products formed once per pair of tiles a segment costs 3 m^2 n + (4 s - 3) m^3 multiply-adds instead of
+// s (3 m^2 n + m^3): the same for square matrices, s times less work on X for wide ones.  What limits s is rounding: a
+// perturbation of A in directions of small singular values grows by a^2 = 11.9 per step until the next look at X.  Measured
+// against 64 bits on gradients with decaying spectra, Frobenius: one step per segment 1e-5, 3 + 2 steps 1e-5, 5 steps 1e-4 to
+// 4e-4.  So fp32 and fp16 matrices take segments of three, bf16 ones (half a step is 4e-3) of five, nearly square ones of one.
+//
+// Products: every operand is held as two fp16 planes of value * 2^k (hi + lo: 22 bits down to 2^-25 of the scale), and a
+// product is three MFMAs hi hi + hi lo + lo hi into fp32.  The scales 2^k come from bounds of the spectral norms that follow
+// from the coefficients (the eigenvalues start in [0, 1]) and from |X_0| = |G| / (|G| + eps), so nothing overflows and a
+// gradient far below eps keeps its precision.
+// Zero padding to whole tiles is exact: it stays zero in A and X.
+#include "glx_elem.h"
+
+#include <math.h>
+#include <vector>
+
+#define NS_K 32                // k elements of a staged tile
+#define NS_OPS 32              // products of one launch (kernel arguments: 120 bytes each)
+#define NS_MATS 36             // matrices of one prologue launch
+#define NS_SMALL 128           // up to here a segment's steps run in one block
+#define NS_STEPS 64            // at most
+#define NS_PARTS 256           // partial sums of squares per matrix, at most
+
+typedef _Float16 nh8 __attribute__((ext_vector_type(8)));
+typedef _Float16 nh4 __attribute__((ext_vector_type(4)));
+typedef float nf16 __attribute__((ext_vector_type(16)));
+typedef float nf4 __attribute__((ext_vector_type(4)));
+
+enum { NS_PLANES, NS_PARTIAL, NS_XPLANES, NS_FINAL };
+
+// out = epilogue(alpha A B^T): A (mp, K), B (np, K) planes, lo plane behind the hi plane
+struct NsOp {
+  const _Float16* a; const _Float16* b;
+  const _Float16* d;           // NS_PLANES: + beta D, D (mp, mp) planes, or NULL
+  void* out; void* out2;       // NS_PLANES: planes (mp, mp); NS_PARTIAL: fp32 [splits][mp][mp]; NS_XPLANES: planes (mp, np) and
+                               // their transpose (np, mp); NS_FINAL: the caller's matrix
+  const float* xin; const float* xout;      // device scales of the X planes that are read (`xpow` of the operands) / written
+  float alpha, beta, diag, scale;
+  int mp, np, K, kper;         // kper: k elements of a split
+  int m, n;
+  long long ldd;               // NS_FINAL: elements between the caller's rows
+  int block0;
+  short splits;
+  unsigned char kind, sym, tall, dtype, xpow;
+};
+struct NsOps { NsOp op[NS_OPS]; int count; };
+
+struct NsMat {
+  const void* src; long long ld;       // the caller's matrix, `rows` x `cols`
+  _Float16* x; _Float16* xt;           // planes (mp, np) and (np, mp)
+  double* parts; float* xscale;        // sums of squares; the scale of X's planes in front of every step
+  int rows, cols, mp, np, tall, nparts;
+  int block0, tblock0;                 // first block of the norm launch / of the plane launch
+};
+// xb[s], qb[s]: bounds of |X| in front of step s, and of |X| / |X_0|
+struct NsMats { NsMat mat[NS_MATS]; int count, dtype, steps; double eps; float xb[NS_STEPS], qb[NS_STEPS]; };
+static_assert(sizeof(NsMats) <= 4000 && sizeof(NsOps) <= 4000, "kernel arguments");
+
+__device__ __forceinline__ void ns_split(float v, _Float16& hi, _Float16& lo) {
+  hi = (_Float16)v;
+  lo = (_Float16)(v - (float)hi);
+}
+__device__ __forceinline__ float ns_elem(const void* p, long long i, int dtype) {
+  return dtype == GLX_F32 ? ((const float*)p)[i] : dtype == GLX_BF16 ? (float)((const __bf16*)p)[i] : (float)((const _Float16*)p)[i];
+}
+
+// ------------------------------------------------------------------------------------------------ |G|_F and the planes of X
+__global__ __launch_bounds__(256) void k_ns_norm(NsMats s) {
+  int k = 0;
+  while (k + 1 < s.count && (int)blockIdx.x >= s.mat[k + 1].block0) ++k;
+  const NsMat& t = s.mat[k];
+  const int part = blockIdx.x - t.block0;
+  const long long total = (long long)t.rows * t.cols;
+  double sum = 0.0;
+  for (long long e = (long long)part * 256 + threadIdx.x; e < total; e += (long long)t.nparts * 256) {
+    const long long r = e / t.cols;
+    const double v = (double)ns_elem(t.src, r * t.ld + (e - r * t.cols), s.dtype);
+    sum += v * v;
+  }
+  __shared__ double red[256];
+  red[threadIdx.x] = sum;
+  __syncthreads();
+  for (int o = 128; o > 0; o >>= 1) {
+    if ((int)threadIdx.x < o) red[threadIdx.x] += red[threadIdx.x + o];
+    __syncthreads();
+  }
+  if (threadIdx.x == 0) t.parts[part] = red[0];
+}
+
+// a 64 x 64 tile of X: read along the caller's rows, written as planes of X and of its transpose
+__global__ __launch_bounds__(256) void k_ns_planes(NsMats s) {
+  __shared__ float tile[64][65];
+  __shared__ double red[256];
+  int k = 0;
+  while (k + 1 < s.count && (int)blockIdx.x >= s.mat[k + 1].tblock0) ++k;
+  const NsMat& t = s.mat[k];
+  red[threadIdx.x] = (int)threadIdx.x < t.nparts ? t.parts[threadIdx.x] : 0.0;
+  __syncthreads();
+  for (int o = 128; o > 0; o >>= 1) {
+    if ((int)threadIdx.x < o) red[threadIdx.x] += red[threadIdx.x + o];
+    __syncthreads();
+  }
+  const int b = blockIdx.x - t.tblock0, tiles_n = t.np / 64;
+  const double norm = sqrt(red[0]), rho = norm / (norm + s.eps);
+  auto scale = [&](int st) {                                   // brings min(xb, qb rho) into [2^14, 2^15)
+    const float bound = fminf(s.xb[st], (float)(s.qb[st] * rho));
+    int e = bound > 0.f ? 14 - ilogbf(bound) : 60;
+    return ldexpf(1.f, e > 60 ? 60 : e);
+  };
+  const float inv = (float)((double)scale(0) / (norm + s.eps));
+  if (b == 0 && (int)threadIdx.x < s.steps) t.xscale[threadIdx.x] = scale(threadIdx.x);
+  const int i0 = b / tiles_n * 64, j0 = b % tiles_n * 64;      // of X
+  const int c = threadIdx.x & 63;
+#pragma unroll 4
+  for (int r = threadIdx.x >> 6; r < 64; r += 4) {
+    const int row = t.tall ? j0 + r : i0 + r, col = t.tall ? i0 + c : j0 + c;       // of the caller's matrix
+    const float v = row < t.rows && col < t.cols ? ns_elem(t.src, row * t.ld + col, s.dtype) * inv : 0.f;
+    if (t.tall) tile[c][r] = v; else tile[r][c] = v;
+  }
+  __syncthreads();
+  const long long plane = (long long)t.mp * t.np;
+#pragma unroll
+  for (int it = 0; it < 2; ++it) {
+    const int q = threadIdx.x + it * 256, r = q >> 3, c8 = (q & 7) * 8;
+    nh8 h, l, th, tl;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      _Float16 u, v;
+      ns_split(tile[r][c8 + e], u, v);
+      h[e] = u; l[e] = v;
+      ns_split(tile[c8 + e][r], u, v);
+      th[e] = u; tl[e] = v;
+    }
+    const long long o = (long long)(i0 + r) * t.np + j0 + c8, ot = (long long)(j0 + r) * t.mp + i0 + c8;
+    *reinterpret_cast<nh8*>(t.x + o) = h;
+    *reinterpret_cast<nh8*>(t.x + plane + o) = l;
+    *reinterpret_cast<nh8*>(t.xt + ot) = th;
+    *reinterpret_cast<nh8*>(t.xt + plane + ot) = tl;
+  }
+}
+
+// ------------------------------------------------------------------------------------------------ the products
+// A block forms a TILE x TILE tile with four waves of (TILE / 2)^2, k in steps of NS_K through two LDS stages; a staged row is
+// NS_K fp16 = four 16-byte chunks whose order is rotated by the row so that the 32 rows an operand read touches spread over the banks.
+template <int TILE>
+__global__ __launch_bounds__(256) void k_ns_gemm(NsOps s) {
+  constexpr int W = TILE / 2, F = W / 32, CH = TILE * 4 / 256;       // a wave's tile, its 32-wide parts, chunks per thread and plane
+  __shared__ __attribute__((aligned(16))) char smem[2][2][2][TILE * NS_K * 2];       // stage, operand, plane
+  int k = 0;
+  while (k + 1 < s.count && (int)blockIdx.x >= s.op[k + 1].block0) ++k;
+  const NsOp& t = s.op[k];
+  int b = blockIdx.x - t.block0;
+  const int tm = t.mp / TILE, tn = t.np / TILE;
+  const int per = t.sym ? tm * (tm + 1) / 2 : tm * tn, split = b / per;
+  b -= split * per;
+  int ti, tj;
+  if (t.sym) {                                                       // row ti holds the tiles tj <= ti
+    ti = (int)((sqrtf(8.f * b + 1.f) - 1.f) * 0.5f);
+    while ((ti + 1) * (ti + 2) / 2 <= b) ++ti;
+    while (ti * (ti + 1) / 2 > b) --ti;
+    tj = b - ti * (ti + 1) / 2;
+  } else {
+    ti = b / tn; tj = b - ti * tn;
+  }
+  const float xin = t.xin ? t.xin[0] : 1.f, alpha = t.alpha / (t.xpow == 2 ? xin * xin : xin), scale = t.xout ? t.xout[0] : t.scale;
+  const int k0 = split * t.kper, k1 = k0 + t.kper < t.K ? k0 + t.kper : t.K;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wi = wave >> 1, wj = wave & 1, half = lane >> 5, l32 = lane & 31;
+  const _Float16* src[2] = {t.a + (long long)ti * TILE * t.K, t.b + (long long)tj * TILE * t.K};
+  const long long plane[2] = {(long long)t.mp * t.K, (long long)t.np * t.K};
+  nh8 stage[2][2][CH];
+  auto fetch = [&](int kk) {
+#pragma unroll
+    for (int o = 0; o < 2; ++o)
+#pragma unroll
+      for (int p = 0; p < 2; ++p)
+#pragma unroll
+        for (int c = 0; c < CH; ++c) {
+          const int q = threadIdx.x + c * 256, r = q >> 2, ch = q & 3;
+          stage[o][p][c] = *reinterpret_cast<const nh8*>(src[o] + p * plane[o] + (long long)r * t.K + kk + ch * 8);
+        }
+  };
+  auto put = [&](int buf) {
+#pragma unroll
+    for (int o = 0; o < 2; ++o)
+#pragma unroll
+      for (int p = 0; p < 2; ++p)
+#pragma unroll
+        for (int c = 0; c < CH; ++c) {
+          const int q = threadIdx.x + c * 256, r = q >> 2, ch = q & 3;
+          *reinterpret_cast<nh8*>(&smem[buf][o][p][r * 64 + ((ch ^ (r >> 1)) & 3) * 16]) = stage[o][p][c];
+        }
+  };
+  nf16 acc[F][F];
+#pragma unroll
+  for (int i = 0; i < F; ++i)
+#pragma unroll
+    for (int j = 0; j < F; ++j) acc[i][j] = (nf16)(0.f);
+  if (k0 < k1) { fetch(k0); put(0); }
+  __syncthreads();
+  int buf = 0;
+  for (int kk = k0; kk < k1; kk += NS_K) {
+    const bool more = kk + NS_K < k1;
+    if (more) fetch(kk + NS_K);
+#pragma unroll
+    for (int ks = 0; ks < NS_K / 16; ++ks) {
+      nh8 fa[2][F], fb[2][F];
+#pragma unroll
+      for (int p = 0; p < 2; ++p)
+#pragma unroll
+        for (int f = 0; f < F; ++f) {
+          const int ra = wi * W + f * 32 + l32, rb = wj * W + f * 32 + l32, ch = ks * 2 + half;
+          fa[p][f] = *reinterpret_cast<const nh8*>(&smem[buf][0][p][ra * 64 + ((ch ^ (ra >> 1)) & 3) * 16]);
+          fb[p][f] = *reinterpret_cast<const nh8*>(&smem[buf][1][p][rb * 64 + ((ch ^ (rb >> 1)) & 3) * 16]);
+        }
+#pragma unroll
+      for (int i = 0; i < F; ++i)
+#pragma unroll
+        for (int j = 0; j < F; ++j) {
+          acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fa[1][i], fb[0][j], acc[i][j], 0, 0, 0);
+          acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fa[0][i], fb[1][j], acc[i][j], 0, 0, 0);
+          acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fa[0][i], fb[0][j], acc[i][j], 0, 0, 0);
+        }
+    }
+    if (more) put(buf ^ 1);
+    __syncthreads();
+    buf ^= 1;
+  }
+  // a lane's accumulators: column l32, rows 8 g + 4 half + 0..3 of the 32 x 32 part
+#pragma unroll
+  for (int i = 0; i < F; ++i)
+#pragma unroll
+    for (int j = 0; j < F; ++j)
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const int row = ti * TILE + wi * W + i * 32 + g * 8 + half * 4, col = tj * TILE + wj * W + j * 32 + l32;
+        nf4 v;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = acc[i][j][g * 4 + e] * alpha;
+        if (t.kind == NS_PARTIAL) {
+          float* o = (float*)t.out + (long long)split * t.mp * t.mp;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) o[(long long)(row + e) * t.mp + col] = v[e];
+        } else if (t.kind == NS_FINAL) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            if (row + e >= t.m || col >= t.n) continue;
+            const long long at = t.tall ? (long long)col * t.ldd + row + e : (long long)(row + e) * t.ldd + col;
+            if (t.dtype == GLX_F32) ((float*)t.out)[at] = v[e];
+            else if (t.dtype == GLX_BF16) ((__bf16*)t.out)[at] = (__bf16)v[e];
+            else ((_Float16*)t.out)[at] = (_Float16)v[e];
+          }
+        } else {
+          const int ldo = t.kind == NS_PLANES ? t.mp : t.np;
+          const long long po = (long long)t.mp * ldo;
+          if (t.d) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const _Float16* d = t.d + (long long)(row + e) * t.mp + col;
+              v[e] += t.beta * ((float)d[0] + (float)d[(long long)t.mp * t.mp]);
+              if (row + e == col) v[e] += t.diag;
+            }
+          }
+          nh4 h, l;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            _Float16 u, w;
+            ns_split(v[e] * scale, u, w);
+            h[e] = u; l[e] = w;
+            _Float16* o = (_Float16*)t.out + (long long)(row + e) * ldo + col;
+            o[0] = u; o[po] = w;
+          }
+          // the transpose: X's other planes, or the mirrored tile of a symmetric product
+          if (t.kind == NS_XPLANES || ti != tj) {
+            _Float16* o = (_Float16*)(t.kind == NS_XPLANES ? t.out2 : t.out) + (long long)col * t.mp + row;
+            *reinterpret_cast<nh4*>(o) = h;
+            *reinterpret_cast<nh4*>(o + po) = l;
+          }
+        }
+      }
+}
+
+// the splits' sum of a Gram matrix (tiles on and below the diagonal were formed) as planes of the whole matrix
+__global__ __launch_bounds__(256) void k_ns_join(NsOps s, int tile) {
+  int k = 0;
+  while (k + 1 < s.count && (int)blockIdx.x >= s.op[k + 1].block0) ++k;
+  const NsOp& t = s.op[k];
+  const long long e = (long long)(blockIdx.x - t.block0) * 256 + threadIdx.x, plane = (long long)t.mp * t.mp;
+  if (e >= plane) return;
+  int r = (int)(e / t.mp), c = (int)(e - (long long)r * t.mp);
+  if (c / tile > r / tile) { const int x = r; r = c; c = x; }
+  const float* p = (const float*)t.a + (long long)r * t.mp + c;
+  float v = 0.f;
+#pragma unroll 8
+  for (int q = 0; q < t.splits; ++q) v += p[q * plane];
+  _Float16 u, w;
+  ns_split(v * t.scale, u, w);
+  ((_Float16*)t.out)[e] = u;
+  ((_Float16*)t.out)[plane + e] = w;
+}
+
+// ------------------------------------------------------------------------------------------------ a segment of a small matrix
+// One block per matrix of up to 32 MT rows: wave w owns the columns 32 w .. 32 w + 31 of A, H and Q in registers, in the layout
+// the MFMA leaves them in, which is also a B operand whose k order is permuted (the A operand is read in that order from LDS).
+// Every product is [matrix in LDS] x [own columns]: A A, A P, P (A P), P Q -- only A and P ever pass through LDS.  (P (A P), not
+// P (P A): errors between directions of small and large singular values grow by p_small p_large a step, not by p_small^2.)
+struct NsSmall { const _Float16* g; _Float16* q; int mp; };
+struct NsSmalls { NsSmall m[NS_MATS]; int count, steps; float a, b, c; float gs[8], ps[8], hs[8], qs[8]; };     // scales by step
+
+template <int MT>
+__device__ __forceinline__ void ns_panel(const char* lds, const nf16 (&own)[MT], float scale, float alpha, nf16 (&out)[MT]) {
+  constexpr int LD = MT * 64 + 16, PL = MT * 32 * LD;
+  const int lane = threadIdx.x & 63, half = lane >> 5, l32 = lane & 31;
+#pragma unroll
+  for (int i = 0; i < MT; ++i) out[i] = (nf16)(0.f);
+#pragma unroll
+  for (int kt = 0; kt < MT; ++kt)
+#pragma unroll
+    for (int ks = 0; ks < 2; ++ks) {
+      nh8 bh, bl;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        _Float16 u, w;
+        ns_split(own[kt][ks * 8 + e] * scale, u, w);
+        bh[e] = u; bl[e] = w;
+      }
+#pragma unroll
+      for (int i = 0; i < MT; ++i) {
+        const char* p = lds + (i * 32 + l32) * LD + (kt * 32 + ks * 16 + half * 4) * 2;
+        const nh4 h0 = *reinterpret_cast<const nh4*>(p), h1 = *reinterpret_cast<const nh4*>(p + 16);
+        const nh4 l0 = *reinterpret_cast<const nh4*>(p + PL), l1 = *reinterpret_cast<const nh4*>(p + PL + 16);
+        const nh8 ah = {h0[0], h0[1], h0[2], h0[3], h1[0], h1[1], h1[2], h1[3]};
+        const nh8 al = {l0[0], l0[1], l0[2], l0[3], l1[0], l1[1], l1[2], l1[3]};
+        out[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(al, bh, out[i], 0, 0, 0);
+        out[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ah, bl, out[i], 0, 0, 0);
+        out[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ah, bh, out[i], 0, 0, 0);
+      }
+    }
+#pragma unroll
+  for (int i = 0; i < MT; ++i)
+#pragma unroll
+    for (int e = 0; e < 16; ++e) out[i][e] *= alpha;
+}
+// own columns -> the planes in LDS (or global memory), row = own column (the matrices are symmetric)
+template <int MT>
+__device__ __forceinline__ void ns_panel_put(char* dst, int ld, long long plane, const nf16 (&own)[MT], float scale) {
+  const int lane = threadIdx.x & 63, half = lane >> 5, col = (threadIdx.x >> 6) * 32 + (lane & 31);
+#pragma unroll
+  for (int i = 0; i < MT; ++i)
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      nh4 h, l;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        _Float16 u, w;
+        ns_split(own[i][g * 4 + e] * scale, u, w);
+        h[e] = u; l[e] = w;
+      }
+      char* p = dst + (long long)col * ld + (i * 32 + g * 8 + half * 4) * 2;
+      *reinterpret_cast<nh4*>(p) = h;
+      *reinterpret_cast<nh4*>(p + plane) = l;
+    }
+}
+
+template <int MT>
+__global__ __launch_bounds__(MT * 64) void k_ns_small(NsSmalls s) {
+  constexpr int LD = MT * 64 + 16, PL = MT * 32 * LD, MP = MT * 32;
+  __shared__ __attribute__((aligned(16))) char lds[2 * PL];
+  const NsSmall& t = s.m[blockIdx.x];
+  const int lane = threadIdx.x & 63, half = lane >> 5, col = (threadIdx.x >> 6) * 32 + (lane & 31);
+  nf16 G[MT], P[MT], Q[MT], H[MT];
+  const float unscale = 1.f / s.gs[0];
+#pragma unroll
+  for (int i = 0; i < MT; ++i)
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const _Float16* p = t.g + (long long)col * MP + i * 32 + g * 8 + half * 4;
+      const nh4 h = *reinterpret_cast<const nh4*>(p), l = *reinterpret_cast<const nh4*>(p + MP * MP);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) G[i][g * 4 + e] = ((float)h[e] + (float)l[e]) * unscale;
+    }
+  for (int st = 0; st < s.steps; ++st) {
+    const float gs = s.gs[st], ps = s.ps[st];
+    ns_panel_put<MT>(lds, LD, PL, G, gs);
+    __syncthreads();
+    ns_panel<MT>(lds, G, gs, 1.f / (gs * gs), P);
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        P[i][e] = s.b * G[i][e] + s.c * P[i][e];
+        if (i * 32 + (e >> 2) * 8 + half * 4 + (e & 3) == col) P[i][e] += s.a;
+      }
+    if (st + 1 < s.steps) ns_panel<MT>(lds, P, ps, 1.f / (gs * ps), H);
+    __syncthreads();
+    ns_panel_put<MT>(lds, LD, PL, P, ps);
+    __syncthreads();
+    if (st == 0) {
+#pragma unroll
+      for (int i = 0; i < MT; ++i) Q[i] = P[i];
+    } else {
+      ns_panel<MT>(lds, Q, s.qs[st - 1], 1.f / (s.qs[st - 1] * ps), P);
+#pragma unroll
+      for (int i = 0; i < MT; ++i) Q[i] = P[i];
+    }
+    if (st + 1 < s.steps) {
+      ns_panel<MT>(lds, H, s.hs[st], 1.f / (s.hs[st] * ps), G);
+      __syncthreads();
+    }
+  }
+  ns_panel_put<MT>((char*)t.q, MP * 2, (long long)MP * MP * 2, Q, s.qs[s.steps - 1]);
+}
+
+// ------------------------------------------------------------------------------------------------ host: programs
+struct NsPlan {                // one matrix
+  int rows, cols, m, n, mp, np, tile, tall, seg, splits, kper, nparts;
+  bool small;
+  size_t x, xt, x2, xt2, g, h, p[2], q[2], part, parts, xscale;        // byte offsets in the workspace
+};
+struct NsBounds { double g, p, h, q; };       // of one step of a segment: spectral norms of A, P, H = P A and Q behind the step
+
+static float ns_scale(double bound) { return (float)exp2(floor(log2(32768.0 / bound))); }
+
+// the largest eigenvalues that the coefficients allow, step by step: lambda <- lambda p(lambda)^2 from [0, 1]
+static bool ns_bounds(int steps, const float* c, std::vector<double>& lam, std::vector<double>& pmax, std::vector<double>& hmax) {
+  if (!isfinite(c[0]) || !isfinite(c[1]) || !isfinite(c[2])) return false;
+  double top = 1.01;           // (A's eigenvalues are at most 1 up to its own rounding)
+  lam.push_back(top);
+  for (int s = 0; s < steps; ++s) {
+    double pm = 0, hm = 0, next = 0;
+    for (int i = 0; i <= 2048; ++i) {
+      const double l = top * i / 2048, p = c[0] + c[1] * l + c[2] * l * l;
+      pm = fmax(pm, fabs(p)); hm = fmax(hm, fabs(l * p)); next = fmax(next, l * p * p);
+    }
+    // (between the samples: a polynomial of degree 5 moves by far less than 1 % of its maximum)
+    pmax.push_back(pm * 1.01 + 1e-6); hmax.push_back(hm * 1.01 + 1e-6);
+    top = next * 1.02 + 1e-6;
+    if (!(top < 64.0) || !(pm < 64.0)) return false;
+    lam.push_back(top);
+  }
+  return true;
+}
+
+static int ns_padded(int v, int tile) { return (v + tile - 1) / tile * tile; }
+
+static NsPlan ns_plan(int rows, int cols, int dtype, int steps, size_t& at) {
+  NsPlan p = {};
+  p.rows = rows; p.cols = cols; p.tall = rows > cols;
+  p.m = p.tall ? cols : rows; p.n = p.tall ? rows : cols;
+  p.small = p.m <= NS_SMALL;
+  // 128-wide tiles once the symmetric products fill the card with them
+  p.tile = p.m > 2048 ? 128 : 64;
+  p.mp = ns_padded(p.m, p.tile); p.np = ns_padded(p.n, p.tile);
+  p.seg = dtype == GLX_BF16 ? 5 : 3;
+  if (!p.small && 4ll * p.n <= 5ll * p.m) p.seg = 1;
+  if (p.seg > steps) p.seg = steps;
+  const int t = p.mp / p.tile;
+  const long long tiles = (long long)t * (t + 1) / 2, ksteps = p.np / NS_K;
+  long long splits = 512 / tiles;                       // two blocks per compute unit
+  if (splits > ksteps / 4) splits = ksteps / 4;         // 128 k elements a split, at least
+  if (splits < 1) splits = 1;
+  p.kper = (int)((ksteps + splits - 1) / splits) * NS_K;
+  p.splits = (int)((p.np + p.kper - 1) / p.kper);
+  const long long total = (long long)p.m * p.n;
+  p.nparts = (int)((total + 16383) / 16384);
+  if (p.nparts > NS_PARTS) p.nparts = NS_PARTS;
+  const size_t X = glx_align((size_t)p.mp * p.np * 4), S = glx_align((size_t)p.mp * p.mp * 4);
+  auto take = [&](size_t bytes) { const size_t o = at; at += glx_align(bytes); return o; };
+  p.x = take(X); p.xt = take(X); p.x2 = take(X); p.xt2 = take(X);
+  p.g = take(S); p.h = take(S); p.p[0] = take(S); p.p[1] = take(S); p.q[0] = take(S); p.q[1] = take(S);
+  p.part = take(p.splits > 1 ? S * p.splits : 256);
+  p.parts = take(NS_PARTS * sizeof(double));
+  p.xscale = take(NS_STEPS * sizeof(float));
+  return p;
+}
+
+static int ns_check(const char* who, const glx_matrix* mats, int count, int dtype, int steps) {
+  GLX_REQUIRE(count >= 0 && (count == 0 || mats), "%s: null list", who);
+  GLX_REQUIRE(glx_elem_ok(dtype), "%s: dtype %d", who, dtype);
+  GLX_REQUIRE(steps >= 1 && steps <= NS_STEPS, "%s: %d steps", who, steps);
+  for (int i = 0; i < count; ++i)
+    GLX_REQUIRE(mats[i].rows >= 1 && mats[i].cols >= 1 && mats[i].rows <= (1 << 20) && mats[i].cols <= (1 << 20)
+                && (mats[i].rows < mats[i].cols ? mats[i].rows : mats[i].cols) <= (1 << 15),
+                "%s: matrix %d is %d x %d", who, i, mats[i].rows, mats[i].cols);
+  return GLX_OK;
+}
+
+extern "C" size_t glx_orthogonalize_workspace_bytes(const glx_matrix* mats, int count, int dtype, int steps) {
+  if (ns_check("glx_orthogonalize_workspace_bytes", mats, count, dtype, steps) != GLX_OK) return 0;
+  size_t at = 0;
+  for (int i = 0; i < count; ++i) ns_plan(mats[i].rows, mats[i].cols, dtype, steps, at);
+  return at + 256;
+}
+
+struct NsStage {               // what one launch round does, over all matrices
+  std::vector<NsOp> gemm[2], join[2];
+  std::vector<NsSmall> small[2];
+  int steps = 0, first = 0;    // of the small ones
+};
+
+static void ns_launch_ops(std::vector<NsOp>& ops, int tile, bool join, hipStream_t st) {
+  for (size_t i = 0; i < ops.size(); i += NS_OPS) {
+    NsOps s;
+    memset(&s, 0, sizeof(s));
+    int blocks = 0;
+    for (size_t j = i; j < ops.size() && j < i + NS_OPS; ++j) {
+      NsOp& o = s.op[s.count++] = ops[j];
+      o.block0 = blocks;
+      const int tm = o.mp / tile, tn = o.np / tile;
+      blocks += join ? glx_divup((long long)o.mp * o.mp, 256) : (o.sym ? tm * (tm + 1) / 2 : tm * tn) * o.splits;
+    }
+    if (join) hipLaunchKernelGGL(k_ns_join, dim3(blocks), dim3(256), 0, st, s, tile);
+    else if (tile == 128) hipLaunchKernelGGL((k_ns_gemm<128>), dim3(blocks), dim3(256), 0, st, s);
+    else hipLaunchKernelGGL((k_ns_gemm<64>), dim3(blocks), dim3(256), 0, st, s);
+  }
+}
+
+extern "C" int glx_orthogonalize(const glx_matrix* mats, int count, int dtype, int steps, const float* coefficients, double eps,
+                                 void* workspace, size_t workspace_bytes, void* stream) try {
+  if (int rc = ns_check("glx_orthogonalize", mats, count, dtype, steps)) return rc;
+  GLX_REQUIRE(coefficients && eps >= 0.0, "glx_orthogonalize: bad coefficients or eps");
+  if (count == 0) return GLX_OK;
+  for (int i = 0; i < count; ++i)
+    GLX_REQUIRE(mats[i].src && mats[i].dst && mats[i].ld_src >= mats[i].cols && mats[i].ld_dst >= mats[i].cols,
+                "glx_orthogonalize: matrix %d: null pointer or rows that overlap", i);
+  std::vector<double> lam, pmax, hmax;
+  GLX_REQUIRE(ns_bounds(steps, coefficients, lam, pmax, hmax),
+              "glx_orthogonalize: these coefficients let singular values grow beyond the arithmetic's range");
+  std::vector<NsPlan> plans;
+  size_t need = 0;
+  for (int i = 0; i < count; ++i) plans.push_back(ns_plan(mats[i].rows, mats[i].cols, dtype, steps, need));
+  if (!workspace || workspace_bytes < need) {
+    glx_set_error("glx_orthogonalize: workspace %zu < %zu bytes", workspace_bytes, need);
+    return GLX_EWORKSPACE;
+  }
+  GLX_REQUIRE(((uintptr_t)workspace & 15) == 0, "glx_orthogonalize: the workspace must be 16-byte aligned");
+  hipStream_t st = (hipStream_t)stream;
+  char* ws = (char*)workspace;
+  const float a = coefficients[0], b = coefficients[1], c = coefficients[2];
+  auto qbound = [&](int s0, int s) { double v = 1; for (int i = s0; i <= s; ++i) v *= pmax[i]; return v; };
+
+  for (int i = 0; i < count; i += NS_MATS) {           // |G|_F, then the planes
+    NsMats s;
+    memset(&s, 0, sizeof(s));
+    s.dtype = dtype; s.eps = eps; s.steps = steps;
+    double growth = 1.0;
+    for (int k = 0; k < steps; ++k) {
+      s.xb[k] = (float)sqrt(lam[k]); s.qb[k] = (float)fmin(growth, 1e30);
+      growth *= pmax[k];
+    }
+    int nb = 0, tb = 0;
+    for (int j = i; j < count && j < i + NS_MATS; ++j) {
+      const NsPlan& p = plans[j];
+      NsMat& t = s.mat[s.count++];
+      t.src = mats[j].src; t.ld = mats[j].ld_src;
+      t.x = (_Float16*)(ws + p.x); t.xt = (_Float16*)(ws + p.xt); t.parts = (double*)(ws + p.parts); t.xscale = (float*)(ws + p.xscale);
+      t.rows = p.rows; t.cols = p.cols; t.mp = p.mp; t.np = p.np; t.tall = p.tall; t.nparts = p.nparts;
+      t.block0 = nb; t.tblock0 = tb;
+      nb += p.nparts; tb += p.mp / 64 * (p.np / 64);
+    }
+    hipLaunchKernelGGL(k_ns_norm, dim3(nb), dim3(256), 0, st, s);
+    hipLaunchKernelGGL(k_ns_planes, dim3(tb), dim3(256), 0, st, s);
+  }
+
+  // every matrix's program as a list of stages; stage k of all matrices runs together
+  std::vector<NsStage> stages;
+  for (int i = 0; i < count; ++i) {
+    const NsPlan& p = plans[i];
+    const int kind = p.tile == 128;
+    size_t k = 0;
+    auto stage = [&]() -> NsStage& {
+      if (k == stages.size()) stages.emplace_back();
+      return stages[k++];
+    };
+    auto planes = [&](size_t o) { return (_Float16*)(ws + o); };
+    auto square = [&](size_t A, float as, size_t B, float bs, size_t out, float scale) {       // out = A B, symmetric
+      NsOp o = {};
+      o.a = planes(A); o.b = planes(B); o.out = planes(out);
+      o.alpha = 1.f / (as * bs); o.scale = scale;
+      o.mp = p.mp; o.np = p.mp; o.K = p.mp; o.kper = p.mp; o.splits = 1; o.kind = NS_PLANES; o.sym = 1;
+      return o;
+    };
+    size_t x = p.x, xt = p.xt, x2 = p.x2, xt2 = p.xt2;
+    for (int s0 = 0; s0 < steps; s0 += p.seg) {
+      const int s1 = s0 + p.seg < steps ? s0 + p.seg : steps;
+      const float* xs = (const float*)(ws + p.xscale) + s0;
+      float gs = ns_scale(lam[s0]);
+      {                                                // A = X X^T
+        NsOp o = {};
+        o.a = o.b = planes(x);
+        o.alpha = 1.f; o.scale = gs; o.xin = xs; o.xpow = 2;
+        o.mp = o.np = p.mp; o.K = p.np; o.kper = p.kper; o.splits = (short)p.splits; o.sym = 1;
+        if (p.splits > 1) {
+          o.kind = NS_PARTIAL; o.out = ws + p.part;
+          stage().gemm[kind].push_back(o);
+          NsOp j = {};
+          j.a = planes(p.part); j.out = planes(p.g); j.scale = gs; j.mp = j.np = p.mp; j.splits = (short)p.splits;
+          stage().join[kind].push_back(j);
+        } else {
+          o.kind = NS_PLANES; o.out = planes(p.g);
+          stage().gemm[kind].push_back(o);
+          stage();                                     // (every matrix keeps a place for the join: small ones meet in one launch)
+        }
+      }
+      size_t q = p.q[0];
+      float qs = 0.f;
+      if (p.small) {
+        NsStage& g = stage();
+        NsSmall m = {planes(p.g), planes(q), p.mp};
+        g.small[p.mp == 128].push_back(m);
+        g.steps = s1 - s0; g.first = s0;
+        qs = ns_scale(qbound(s0, s1 - 1));
+      } else {
+        for (int s = s0; s < s1; ++s) {
+          const float ps = ns_scale(pmax[s]), hs = ns_scale(hmax[s]);
+          const size_t P = p.p[(s - s0) & 1];
+          NsOp o = square(p.g, gs, p.g, gs, P, ps);    // P = a I + b A + c A A
+          o.alpha *= c; o.d = planes(p.g); o.beta = b / gs; o.diag = a;
+          stage().gemm[kind].push_back(o);
+          if (s == s0) {
+            q = P; qs = ps;
+          } else {                                     // (beside H where a step follows)
+            const float nqs = ns_scale(qbound(s0, s));
+            const size_t nq = p.q[(s - s0) & 1];
+            NsOp oq = square(P, ps, q, qs, nq, nqs);
+            NsStage& g = stage();
+            g.gemm[kind].push_back(oq);
+            q = nq; qs = nqs;
+            --k;
+          }
+          if (s + 1 < s1) {
+            stage().gemm[kind].push_back(square(P, ps, p.g, gs, p.h, hs));
+            const float ngs = ns_scale(lam[s + 1]);
+            stage().gemm[kind].push_back(square(p.h, hs, P, ps, p.g, ngs));
+            gs = ngs;
+          } else if (s > s0) {
+            ++k;
+          }
+        }
+      }
+      {                                                // X <- Q X
+        NsOp o = {};
+        o.a = planes(q); o.b = planes(xt);
+        o.alpha = 1.f / qs; o.xin = xs; o.xpow = 1;
+        o.mp = p.mp; o.np = p.np; o.K = p.mp; o.kper = p.mp; o.splits = 1;
+        if (s1 == steps) {
+          o.kind = NS_FINAL; o.out = mats[i].dst; o.ldd = mats[i].ld_dst;
+          o.m = p.m; o.n = p.n; o.tall = (unsigned char)p.tall; o.dtype = (unsigned char)dtype;
+        } else {
+          o.kind = NS_XPLANES; o.out = planes(x2); o.out2 = planes(xt2); o.xout = (const float*)(ws + p.xscale) + s1;
+        }
+        stage().gemm[kind].push_back(o);
+        size_t y = x; x = x2; x2 = y;
+        y = xt; xt = xt2; xt2 = y;
+      }
+    }
+  }
+  for (auto& g : stages) {
+    for (int t = 0; t < 2; ++t) {
+      ns_launch_ops(g.gemm[t], t ? 128 : 64, false, st);
+      ns_launch_ops(g.join[t], t ? 128 : 64, true, st);
+      for (size_t i = 0; i < g.small[t].size(); i += NS_MATS) {
+        NsSmalls s;
+        memset(&s, 0, sizeof(s));
+        for (size_t j = i; j < g.small[t].size() && j < i + NS_MATS; ++j) s.m[s.count++] = g.small[t][j];
+        s.steps = g.steps; s.a = a; s.b = b; s.c = c;
+        for (int k = 0; k < g.steps; ++k) {
+          s.gs[k] = ns_scale(lam[g.first + k]); s.ps[k] = ns_scale(pmax[g.first + k]); s.hs[k] = ns_scale(hmax[g.first + k]);
+          s.qs[k] = ns_scale(qbound(g.first, g.first + k));
+        }
+        if (t) hipLaunchKernelGGL((k_ns_small<4>), dim3(s.count), dim3(256), 0, st, s);
+        else hipLaunchKernelGGL((k_ns_small<2>), dim3(s.count), dim3(128), 0, st, s);
+      }
+    }
+  }
+  GLX_LAUNCH_CHECK();
+  return GLX_OK;
+} catch (const std::exception& e) {
+  glx_set_error("glx_orthogonalize: %s", e.what());
+  return GLX_EINVAL;
+}

@@ -17,10 +17,87 @@ from weights (packed sparse-conv images, folded BatchNorms, recorded inference g
 Python -- advances; in training mode the sparse convs re-pack inside the step anyway
 (spconv.core.SparseConvolution._packed_weight)."""
 import ctypes
+import math
 
 import torch
 
 from . import _lib
+
+MUON_COEFFICIENTS = (3.4445, -4.7750, 2.0315)
+
+
+class _Matrix(ctypes.Structure):           # glx_matrix
+    _fields_ = [("src", ctypes.c_void_p), ("dst", ctypes.c_void_p), ("ld_src", ctypes.c_int64), ("ld_dst", ctypes.c_int64),
+                ("rows", ctypes.c_int32), ("cols", ctypes.c_int32)]
+
+
+def _check_steps(who, steps, coefficients, eps):
+    if int(steps) != steps or not 1 <= steps <= 64:
+        raise ValueError("%s: steps must be a whole number from 1 to 64, got %r" % (who, steps))
+    coefficients = tuple(float(c) for c in coefficients)
+    if len(coefficients) != 3 or not all(math.isfinite(c) for c in coefficients):
+        raise ValueError("%s: coefficients must be three finite numbers, got %r" % (who, coefficients))
+    if not float(eps) >= 0.0:
+        raise ValueError("%s: eps must not be negative, got %r" % (who, eps))
+    return int(steps), (ctypes.c_float * 3)(*coefficients), float(eps)
+
+
+def orthogonalize(mats, steps=5, coefficients=MUON_COEFFICIENTS, eps=1e-7):
+    """The nearest matrices with orthonormal rows (or columns), roughly: `steps` Newton-Schulz steps of
+    X <- a X + (b A + c A^2) X, A = X X^T, from X = G / (|G|_F + eps), transposed where G has more rows than columns.
+    The default coefficients bring singular values from ~1e-3 .. 1 into 0.7 .. 1.2 in five steps.
+
+    mats: a device tensor (..., rows, cols), or a list / tuple of 2-D tensors of ANY shapes but one type (float32, bfloat16 or
+    float16) and one device: a list costs as many launches as one matrix (csrc/glx_orthogonal.hip).
+    -> new tensors of the same shapes and type (a list for a list), outside autograd."""
+    who = "orthogonalize"
+    steps, coeffs, eps = _check_steps(who, steps, coefficients, eps)
+    if isinstance(mats, torch.Tensor):
+        if mats.dim() < 2:
+            raise ValueError("%s: expected (..., rows, cols), got shape %s" % (who, tuple(mats.shape)))
+        if mats.dtype not in _lib.DTYPE_CODES:
+            raise ValueError("%s: float32, bfloat16 or float16 matrices, got %s" % (who, mats.dtype))
+        if mats.dim() == 2:
+            return _orthogonalize([mats], steps, coeffs, eps)[0]
+        _lib.check_device(who, mats)
+        out = torch.empty(mats.shape, dtype=mats.dtype, device=mats.device)
+        if mats.numel() or 0 in mats.shape[-2:]:
+            flat = mats.detach().reshape(-1, *mats.shape[-2:])
+            _orthogonalize(list(flat.unbind(0)), steps, coeffs, eps, list(out.view(-1, *mats.shape[-2:]).unbind(0)))
+        return out
+    mats = list(mats)
+    for m in mats:
+        if not isinstance(m, torch.Tensor) or m.dim() != 2:
+            raise ValueError("%s: a list holds 2-D tensors, got %s" % (who, tuple(m.shape) if isinstance(m, torch.Tensor) else type(m)))
+        if m.dtype not in _lib.DTYPE_CODES or m.dtype != mats[0].dtype:
+            raise ValueError("%s: float32, bfloat16 or float16 matrices of one type, got %s beside %s" % (who, m.dtype, mats[0].dtype))
+    return _orthogonalize(mats, steps, coeffs, eps) if mats else []
+
+
+def _orthogonalize(mats, steps, coeffs, eps, outs=None):
+    who = "orthogonalize"
+    for m in mats:
+        r, c = m.shape
+        if r < 1 or c < 1 or max(r, c) > 1 << 20 or min(r, c) > 1 << 15:
+            raise ValueError("%s: a matrix of %d x %d (1 .. 2^20 each, the smaller one up to 2^15)" % (who, r, c))
+    _lib.check_device(who, *mats)
+    if outs is None:
+        outs = [torch.empty(m.shape, dtype=m.dtype, device=m.device) for m in mats]
+    srcs = []
+    for m in mats:
+        m = m.detach()
+        if m.stride(1) != 1 and m.shape[1] > 1 or m.stride(0) < m.shape[1] and m.shape[0] > 1:
+            m = m.contiguous()
+        srcs.append(m)
+    table = (_Matrix * len(mats))()
+    for t, s, o in zip(table, srcs, outs):
+        t.src, t.dst, t.rows, t.cols = s.data_ptr(), o.data_ptr(), s.shape[0], s.shape[1]
+        t.ld_src, t.ld_dst = max(s.stride(0), s.shape[1]), o.shape[1]
+    dev, code = mats[0].device, _lib.dtype_code(mats[0].dtype)
+    ws = torch.empty(_lib.query("glx_orthogonalize_workspace_bytes", table, len(mats), code, steps), dtype=torch.uint8, device=dev)
+    _lib.call_on(dev, "glx_orthogonalize", table, len(mats), code, steps, coeffs, ctypes.c_double(eps), ws,
+                 _lib.size_arg(ws.numel()))
+    return outs
 
 
 class FlatGrads:
@@ -266,3 +343,83 @@ class FlatAdamW:
         self.exp_avg_sq.copy_(sd["exp_avg_sq"])
         self.step_count.copy_(sd["step"])
         self.hyper.copy_(sd["hyper"])
+
+
+class FlatMuon(FlatAdamW):
+    """Flat buffers as FlatAdamW's, with orthogonalised momentum steps for the weight matrices and AdamW for everything else:
+
+        m = beta1 m + (1 - beta1) g;   u = beta1 m + (1 - beta1) g (lookahead) or m;   O = orthogonalize(u)
+        p = p (1 - lr weight_decay) - lr 0.2 sqrt(max(rows, cols)) O
+
+    The factor gives a matrix' step the size that AdamW's has, so one learning rate, decay and beta1 (device scalars, set_lr)
+    serve both.  A parameter's matrix is its MEMORY as (rows, cols): shape[0] rows for 2-D to 4-D weights (Linear, Conv1d,
+    Conv2d, channels-last ones too: the columns' order does not matter), the last dimension as columns for the 5-D filters of
+    the sparse convolutions (kd, kh, kw, Cin, Cout).  shapes: {parameter: (rows, cols) or None} overrides that; None, vectors
+    and matrices of one row or column take AdamW.  The whole update is recorded into a HIP graph like FlatAdamW's, gradient
+    exchange, state dictionary and buckets included; it is what StaticTrainStep(optimizer=FlatMuon(model.parameters())) steps."""
+
+    def __init__(self, params, lr=1e-2, betas=(0.95, 0.99), eps=1e-8, weight_decay=1e-2, max_norm=None, lookahead=True, steps=5,
+                 coefficients=MUON_COEFFICIENTS, ns_eps=1e-7, shapes=None):
+        self._ns = _check_steps("FlatMuon", steps, coefficients, ns_eps)
+        super().__init__(params, lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, max_norm=max_norm)
+        shapes = dict(shapes) if shapes else {}
+        self.lookahead = bool(lookahead)
+        self.matrix_shapes = []
+        for p in self.params:
+            rc = shapes[p] if p in shapes else self.matrix_shape(p)
+            if rc is not None:
+                rc = (int(rc[0]), int(rc[1]))
+                if rc[0] * rc[1] != p.numel() or min(rc) < 1:
+                    raise ValueError("FlatMuon: a parameter of %d elements as a %d x %d matrix" % ((p.numel(),) + rc))
+                if max(rc) > 1 << 20 or min(rc) > 1 << 15:
+                    rc = None
+            self.matrix_shapes.append(rc if rc is not None and min(rc) > 1 else None)
+        dev = self.flat_param.device
+        self.update = torch.zeros(self.n, dtype=torch.float32, device=dev)
+        chunks, self._table = [], (_Matrix * max(1, sum(s is not None for s in self.matrix_shapes)))()
+        self._mats = 0
+        for p, o, rc in zip(self.params, self.offsets, self.matrix_shapes):
+            scale = 0.2 * math.sqrt(max(rc)) if rc else 0.0
+            chunks += [(o + i, min(4096, p.numel() - i), scale) for i in range(0, p.numel(), 4096)]
+            if rc:
+                t = self._table[self._mats]
+                t.src = t.dst = self.update.data_ptr() + 4 * o
+                t.rows, t.cols = rc
+                t.ld_src = t.ld_dst = rc[1]
+                self._mats += 1
+        raw = torch.empty(len(chunks), 2, dtype=torch.int64)
+        raw[:, 0] = torch.tensor([c[0] for c in chunks])
+        tail = raw.view(torch.int32).view(len(chunks), 4)
+        tail[:, 2] = torch.tensor([c[1] for c in chunks], dtype=torch.int32)
+        tail[:, 3] = torch.tensor([c[2] for c in chunks], dtype=torch.float32).view(torch.int32)
+        self._chunks = raw.to(dev)
+        self._ns_ws = None
+        if self._mats:
+            self._ns_ws = torch.empty(_lib.query("glx_orthogonalize_workspace_bytes", self._table, self._mats, 0, self._ns[0]),
+                                      dtype=torch.uint8, device=dev)
+
+    @staticmethod
+    def matrix_shape(p):
+        """(rows, cols) of a parameter's memory, None where it is no matrix."""
+        if p.dim() < 2 or p.numel() == 0:
+            return None
+        return (p.numel() // p.shape[-1], p.shape[-1]) if p.dim() == 5 else (p.shape[0], p.numel() // p.shape[0])
+
+    def step(self, packed=False):
+        """clip, AdamW, momentum, orthogonalisation, update.  packed=True: flat_grad already holds this step's gradients."""
+        if not packed:
+            self.pack_grads()
+            for fn in self.after_pack:
+                fn()
+        dev, nchunks = self.flat_param.device, int(self._chunks.shape[0])
+        _lib.call_on(dev, "glx_muon_moments", self.flat_param, self.flat_grad, self.exp_avg, self.exp_avg_sq, self.update,
+                     ctypes.c_int64(self.n), self._chunks, nchunks, self.hyper, ctypes.c_float(self.beta2), ctypes.c_float(self.eps),
+                     ctypes.c_float(self.weight_decay), ctypes.c_float(self.max_norm), ctypes.c_float(self.grad_scale),
+                     1 if self.lookahead else 0, self.step_count, self.grad_norm, self._ws, _lib.size_arg(self._ws.numel()))
+        if self._mats:
+            steps, coeffs, eps = self._ns
+            _lib.call_on(dev, "glx_orthogonalize", self._table, self._mats, 0, steps, coeffs, ctypes.c_double(eps), self._ns_ws,
+                         _lib.size_arg(self._ns_ws.numel()))
+            _lib.call_on(dev, "glx_muon_apply", self.flat_param, self.update, self._chunks, nchunks, self.hyper,
+                         ctypes.c_float(self.weight_decay))
+        _lib.bump_weights_epoch(self.params)

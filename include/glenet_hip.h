@@ -1496,6 +1496,36 @@ int glx_layer_norm_backward(const void* gy, int64_t ldg, const void* x, int64_t 
                             const float* mean, const float* rstd, int64_t rows, int64_t width, void* dx, void* dweight,
                             void* dbias, void* workspace, size_t workspace_bytes, void* stream);
 
+/* ---- orthogonalised updates: Newton-Schulz steps on a list of matrices (glenet_amd/optim.py) ----
+ * Per matrix: X = src / (|src|_F + eps), transposed where rows > cols; `steps` times  A = X X^T,
+ * X = a X + (b A + c A A) X  with coefficients = {a, b, c}; dst = X (transposed back).  src and dst are row-major of `dtype`
+ * with ld_src / ld_dst elements between rows; dst may be src.  coefficients and the list are host memory, read during the
+ * call.  Coefficients under which singular values leave the arithmetic's range are refused. */
+typedef struct glx_matrix {
+  const void* src; void* dst;
+  int64_t ld_src, ld_dst;
+  int32_t rows, cols;
+} glx_matrix;
+size_t glx_orthogonalize_workspace_bytes(const glx_matrix* mats, int count, int dtype, int steps);    /* 0: bad arguments */
+int glx_orthogonalize(const glx_matrix* mats, int count, int dtype, int steps, const float* coefficients, double eps,
+                      void* workspace, size_t workspace_bytes, void* stream);
+
+/* The flat update whose matrices take orthogonalised steps (glenet_amd.optim.FlatMuon).  A chunk is a run of at most 4096
+ * elements of one tensor of the flat buffer; scale > 0: of a matrix.  glx_muon_moments: gradient clipping, AdamW of the other
+ * tensors (as glx_adamw_clip_step_scaled, step count included), the matrices' momentum and the matrix to orthogonalise in
+ * `update`; glx_muon_apply: params = params (1 - lr weight_decay) - lr scale update on the matrices. */
+typedef struct glx_opt_chunk {
+  int64_t start;
+  int32_t len;
+  float scale;
+} glx_opt_chunk;
+int glx_muon_moments(float* params, const float* grads, float* exp_avg, float* exp_avg_sq, float* update, int64_t n,
+                     const glx_opt_chunk* chunks, int nchunks, const float* hyper, float beta2, float eps, float weight_decay,
+                     float max_norm, float grad_scale, int lookahead, int32_t* step, float* norm_out, void* workspace,
+                     size_t workspace_bytes, void* stream);
+int glx_muon_apply(float* params, const float* update, const glx_opt_chunk* chunks, int nchunks, const float* hyper,
+                   float weight_decay, void* stream);
+
 /* Stage stamps: a one-thread launch on `stream` that stores the device's constant 100 MHz wall clock into
  * stamps[slot] (10 ns per tick).  Recorded into a captured training step at its stage boundaries
  * (StaticTrainPipeline.mark) it times the stages inside graph replays; the reference has no counterpart (it times

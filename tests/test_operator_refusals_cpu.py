@@ -23,3 +23,48 @@ def test_layer_norm_refuses():
         layer_norm(torch.zeros(()))
     with pytest.raises(ValueError, match="eps"):
         layer_norm(x, eps=-1.0)
+
+
+def test_orthogonalize_refuses():
+    from glenet_amd import _lib
+    from glenet_amd.optim import orthogonalize
+    m = torch.zeros(4, 6)
+    with pytest.raises(_lib.GlxError, match="no CPU path"):
+        orthogonalize(m)
+    with pytest.raises(_lib.GlxError, match="no CPU path"):
+        orthogonalize([m, m])
+    assert orthogonalize([]) == []
+    for bad in (torch.zeros(5), m.double(), [m, m.half()], [torch.zeros(2, 3, 4)], [3.0], torch.zeros(0, 3), [torch.zeros(2, 0)]):
+        with pytest.raises(ValueError):
+            orthogonalize(bad)
+    for kw in (dict(steps=0), dict(steps=65), dict(steps=2.5), dict(coefficients=(1.0, 2.0)),
+               dict(coefficients=(float("nan"), 0.0, 0.0)), dict(eps=-1.0)):
+        with pytest.raises(ValueError):
+            orthogonalize(m, **kw)
+
+
+def test_orthogonalize_c_entry_refuses():
+    """The C entry's own checks, on the host: shapes, steps, coefficients that diverge, workspaces that are too small."""
+    import ctypes
+
+    from glenet_amd import _lib
+    from glenet_amd.optim import _Matrix
+    lib = _lib.load()
+
+    def call(rows=4, cols=6, ld=6, dtype=0, steps=5, coeffs=(3.4445, -4.775, 2.0315), eps=1e-7, ws=16, nbytes=0, src=64):
+        t = (_Matrix * 1)(_Matrix(src, 64, ld, 6, rows, cols))
+        rc = lib.glx_orthogonalize(t, 1, dtype, steps, (ctypes.c_float * 3)(*coeffs), ctypes.c_double(eps), ctypes.c_void_p(ws),
+                                   ctypes.c_size_t(nbytes), ctypes.c_void_p(0))
+        return rc, lib.glx_last_error().decode()
+
+    assert call()[0] == -3 and "workspace" in call()[1]                       # every other check passed
+    for kw in (dict(rows=0), dict(cols=1 << 21, ld=1 << 21), dict(rows=40000, cols=40000, ld=40000), dict(dtype=3), dict(steps=0),
+               dict(steps=65), dict(eps=-1.0), dict(ld=5), dict(src=0)):
+        assert call(**kw)[0] == -1, kw
+    for coeffs in ((50.0, 0.0, 0.0), (3.4445, -4.775, 9.0), (float("nan"), 0.0, 0.0), (float("inf"), 0.0, 0.0)):
+        rc, msg = call(coeffs=coeffs)
+        assert rc == -1 and "range" in msg, (coeffs, rc, msg)
+    assert call(coeffs=(1.875, -1.25, 0.375), steps=64)[0] == -3
+    assert call(steps=64)[0] == -3
+    t = (_Matrix * 1)(_Matrix(64, 64, 6, 6, 4, 6))
+    assert lib.glx_orthogonalize_workspace_bytes(t, 1, 0, 5) > 0 and lib.glx_orthogonalize_workspace_bytes(t, 1, 7, 5) == 0
