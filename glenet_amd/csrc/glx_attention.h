@@ -1,0 +1,210 @@
+// Cross attention of stacked frames: what the forward and backward kernels share (glx_attention.hip, glx_attention_bwd.hip).
+//
+// Queries (Nq, H, D) and encoder states (Nk, Hkv, D) of B frames lie behind each other; a frame's counts come from device
+// memory or are the same for all frames.  The G = H / Hkv query heads that share a key head are ROWS beside each other: row
+// r of a frame and key head is query r / G, head hk G + r % G.  So a single query with shared heads still fills a tile, and the
+// gradients of shared keys are sums over rows like any other.
+//
+// All products run on 32 x 32 MFMA tiles in one register layout.  A product C = A B leaves lane (l32, half) with column l32 and
+// rows 8 (i / 4) + 4 half + i % 4 (i = 0..15) of C.  Eight consecutive i are a B operand of the next product whose k index runs
+// in that order, so scores turn into probabilities and into the next operand without leaving the lane; the other operand is
+// read from LDS in the same k order (16-bit: the transposing read; 32-bit: plain reads).
+#pragma once
+#include "glx_elem.h"
+
+#define XA_KEYS 64            // keys of a staged tile
+
+typedef float xf16 __attribute__((ext_vector_type(16)));
+typedef float xf4 __attribute__((ext_vector_type(4)));
+typedef short xs4 __attribute__((ext_vector_type(4)));
+typedef short xs8 __attribute__((ext_vector_type(8)));
+
+struct XaArgs {
+  const void *q, *k, *v, *o, *go;
+  void *out, *dq, *dk, *dv;
+  float *lse, *delta;               // (Nq, H); lse in base 2, +inf where no key is left
+  float *part;                      // splits' partial results
+  const unsigned char* mask;        // (Nk) or NULL
+  const int *qcnt, *kcnt;           // (B) or NULL: Lq, Lk
+  long long sq, hq, sk, hk, sv, hv, sg, hg;      // elements between rows and between heads of q, k, v, go
+  long long nq, nk;
+  int frames, lq, lk, heads, kvheads, group, dim, splits;
+  float scale, scale2;              // scale2 = scale log2(e)
+};
+
+// ------------------------------------------------------------------------------------------------ operands
+template <typename T> struct XaFrag { typedef T vec __attribute__((ext_vector_type(8))); };
+
+__device__ __forceinline__ void xa_mma(xf16& c, const XaFrag<__bf16>::vec& a, const XaFrag<__bf16>::vec& b) {
+  c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+}
+__device__ __forceinline__ void xa_mma(xf16& c, const XaFrag<_Float16>::vec& a, const XaFrag<_Float16>::vec& b) {
+  c = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+}
+__device__ __forceinline__ void xa_mma(xf16& c, const XaFrag<float>::vec& a, const XaFrag<float>::vec& b) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a[i], b[i], c, 0, 0, 0);
+}
+
+// A staged tile: rows of DP values, 16 bytes of padding (the 32 rows of an operand read spread over the banks)
+template <typename T, int DP> struct XaTile {
+  static constexpr int LD = DP * (int)sizeof(T) + 16, E = 16 / (int)sizeof(T), CPR = DP / E;
+};
+
+// eight values along a row: the operand whose k index is d; row = l32, k = 16 ks + 8 half + 0..7
+template <typename T, int DP>
+__device__ __forceinline__ typename XaFrag<T>::vec xa_along(const char* tile, int row, int ks, int half) {
+  const char* p = tile + row * XaTile<T, DP>::LD + (ks * 16 + half * 8) * (int)sizeof(T);
+  if constexpr (sizeof(T) == 2) {
+    return *reinterpret_cast<const typename XaFrag<T>::vec*>(p);
+  } else {
+    const xf4 a = *reinterpret_cast<const xf4*>(p), b = *reinterpret_cast<const xf4*>(p + 16);
+    return {a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
+  }
+}
+// eight values down the rows row0 + 4 half + {0..3, 8..11}, column d0 + l32: the operand whose k index is the row
+template <typename T, int DP>
+__device__ __forceinline__ typename XaFrag<T>::vec xa_down(const char* tile, int row0, int d0, int lane) {
+  constexpr int LD = XaTile<T, DP>::LD;
+  const int half = lane >> 5;
+  if constexpr (sizeof(T) == 2) {
+    // a 16-lane group reads 4 rows x 16 columns and every lane gets a column's four values
+    typedef xs4 __attribute__((address_space(3))) * lds_p;
+    const char* p = tile + (row0 + half * 4 + ((lane >> 2) & 3)) * LD + (d0 + (lane & 16) + (lane & 3) * 4) * 2;
+    const xs4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_p)(p));
+    const xs4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_p)(p + 8 * LD));
+    const xs8 v = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+    return __builtin_bit_cast(typename XaFrag<T>::vec, v);
+  } else {
+    const char* p = tile + (row0 + half * 4) * LD + (d0 + (lane & 31)) * 4;
+    typename XaFrag<T>::vec v;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = *reinterpret_cast<const float*>(p + ((i >> 2) * 8 + (i & 3)) * LD);
+    return v;
+  }
+}
+// accumulators 8 c .. 8 c + 7 as an operand
+template <typename T>
+__device__ __forceinline__ typename XaFrag<T>::vec xa_pack(const xf16& s, int c) {
+  typename XaFrag<T>::vec v;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) v[i] = (T)s[c * 8 + i];
+  return v;
+}
+// eight values of a row in global memory, d = 16 ks + 8 half .., zeros beyond D
+template <typename T>
+__device__ __forceinline__ typename XaFrag<T>::vec xa_row(const T* p, int d, int D) {
+  if (d + 8 <= D) return GlxVec<T, 8>::load(p + d);
+  typename XaFrag<T>::vec v;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) v[i] = d + i < D ? p[d + i] : (T)0.f;
+  return v;
+}
+
+// ------------------------------------------------------------------------------------------------ staging
+// ROWS rows through registers into LDS.  row(r) gives a row's address or NULL (zeros: a masked or absent row is never read).
+template <typename T, int DP, int ROWS, int THREADS>
+struct XaStage {
+  static constexpr int E = XaTile<T, DP>::E, CPR = XaTile<T, DP>::CPR, LD = XaTile<T, DP>::LD;
+  static constexpr int N = (ROWS * CPR + THREADS - 1) / THREADS;
+  typedef typename GlxVec<T, E>::vec vec;
+  vec r[N];
+  template <typename F>
+  __device__ __forceinline__ void fetch(F row, int D) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int c = threadIdx.x + i * THREADS, rr = c / CPR, d = (c - rr * CPR) * E;
+#pragma unroll
+      for (int e = 0; e < E; ++e) r[i][e] = (T)0.f;
+      if (ROWS * CPR % THREADS && rr >= ROWS) continue;
+      const T* p = row(rr);
+      if (!p) continue;
+      if (d + E <= D) {
+        r[i] = GlxVec<T, E>::load(p + d);
+      } else {
+#pragma unroll
+        for (int e = 0; e < E; ++e)
+          if (d + e < D) r[i][e] = p[d + e];
+      }
+    }
+  }
+  __device__ __forceinline__ void put(char* tile) const {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int c = threadIdx.x + i * THREADS, rr = c / CPR;
+      if (ROWS * CPR % THREADS && rr >= ROWS) continue;
+      *reinterpret_cast<vec*>(tile + rr * LD + (c - rr * CPR) * 16) = r[i];
+    }
+  }
+};
+
+// ------------------------------------------------------------------------------------------------ frames
+struct XaPlace { long long q0, k0; int nq, nk, tile; };      // tile: index within the frame, -1: nothing there
+
+// which frame holds the tile `t` when every frame has ceil(size / unit) tiles, size = its rows (queries x G) or its keys; the
+// rows behind the last frame count as a frame whose other side is empty.  Counts are clamped into the tensors.
+__device__ __forceinline__ XaPlace xa_place(const XaArgs& a, long long t, int unit, bool keys) {
+  XaPlace p = {0, 0, 0, 0, -1};
+  if (!a.qcnt) {
+    const long long size = keys ? a.lk : (long long)a.lq * a.group, per = (size + unit - 1) / unit;
+    if (per == 0) return p;
+    const long long b = t / per;
+    if (b >= a.frames) return p;
+    p.q0 = b * a.lq; p.k0 = b * a.lk; p.nq = a.lq; p.nk = a.lk; p.tile = (int)(t - b * per);
+    return p;
+  }
+  const int lane = threadIdx.x & 63;
+  long long tiles0 = 0, q0 = 0, k0 = 0;
+  for (int f0 = 0; f0 < a.frames; f0 += 64) {
+    const int f = f0 + lane;
+    long long cq = f < a.frames ? a.qcnt[f] : 0, ck = f < a.frames ? a.kcnt[f] : 0;
+    cq = cq < 0 ? 0 : (cq > a.nq ? a.nq : cq);
+    ck = ck < 0 ? 0 : (ck > a.nk ? a.nk : ck);
+    long long sq = cq, sk = ck;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const long long x = __shfl_up(sq, o, 64), y = __shfl_up(sk, o, 64);
+      if (lane >= o) { sq += x; sk += y; }
+    }
+    // (exclusive prefix, clamped to what is left of the tensors)
+    long long eq = q0 + sq - cq, ek = k0 + sk - ck;
+    eq = eq > a.nq ? a.nq : eq; ek = ek > a.nk ? a.nk : ek;
+    cq = cq > a.nq - eq ? a.nq - eq : cq;
+    ck = ck > a.nk - ek ? a.nk - ek : ck;
+    const long long size = keys ? ck : cq * a.group, n = (size + unit - 1) / unit;
+    long long sn = n;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const long long x = __shfl_up(sn, o, 64);
+      if (lane >= o) sn += x;
+    }
+    const bool here = t >= tiles0 + sn - n && t < tiles0 + sn;
+    const unsigned long long hit = __ballot(here);
+    if (hit) {
+      const int l = __ffsll((long long)hit) - 1;
+      p.q0 = __shfl(eq, l, 64); p.k0 = __shfl(ek, l, 64);
+      p.nq = (int)__shfl(cq, l, 64); p.nk = (int)__shfl(ck, l, 64);
+      p.tile = (int)(t - __shfl(tiles0 + sn - n, l, 64));
+      return p;
+    }
+    tiles0 += __shfl(sn, 63, 64);
+    q0 = __shfl(eq + cq, 63, 64);
+    k0 = __shfl(ek + ck, 63, 64);
+  }
+  const long long left = keys ? a.nk - k0 : a.nq - q0, size = keys ? left : left * a.group, n = (size + unit - 1) / unit;
+  if (t >= tiles0 + n) return p;
+  p.q0 = q0; p.k0 = k0; p.tile = (int)(t - tiles0);
+  (keys ? p.nk : p.nq) = (int)left;
+  return p;
+}
+
+// bit j: key k0 + j exists (j < n) and is not masked; the same in every lane
+__device__ __forceinline__ unsigned long long xa_valid(const unsigned char* mask, long long k0, int n) {
+  const int lane = threadIdx.x & 63;
+  return __ballot(lane < n && (!mask || mask[k0 + lane] != 0));
+}
+
+// host: upper bound of the tiles that xa_place hands out
+static inline long long xa_tiles(long long n, int frames, int per_frame, bool counts, int unit) {
+  return counts ? n / unit + frames + 1 : (long long)frames * ((per_frame + (long long)unit - 1) / unit);
+}

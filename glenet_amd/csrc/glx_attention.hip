@@ -1,0 +1,299 @@
+// Cross attention of stacked frames, forward (glenet_amd/attention.py; the layouts: glx_attention.h).
+//
+//   O = softmax(scale Q K^T) V over a frame's unmasked keys, one pass over the keys with a running maximum and sum per row:
+//   S^T = K Q^T (a lane owns a row's scores), p = 2^(s - m), O^T <- O^T 2^(m_old - m) + V^T p.  A row without keys gives 0.
+//
+// A block is four waves: four tiles of 32 rows that share the staged keys, or, where a frame has few rows, ONE tile whose
+// waves take the staged keys in turn and are joined at the end.  Few tiles are split over the keys as well; the splits' results
+// (O unnormalised, m, l) are joined by a second launch.  Scores, m, l and O are fp32; for 16-bit inputs p is rounded to their
+// type in front of the second product (each to half a step, unbiased: below the rounding of O itself).
+#include "glx_attention.h"
+
+template <typename T, int DP, int RW>
+__global__ __launch_bounds__(256) void k_xa_forward(XaArgs a) {
+  constexpr int KW = 4 / RW, BN = XA_KEYS * (KW == 4 && sizeof(T) == 2 ? 2 : 1), SUB = BN / 32 / KW > 0 ? BN / 32 / KW : 1;
+  constexpr int KU = BN / 32 < KW ? BN / 32 : KW;          // waves of a row tile that have keys of a staged tile
+  constexpr int KS = DP / 16, DT = DP / 32;
+  typedef XaTile<T, DP> Tile;
+  constexpr int TB = BN * Tile::LD;
+  constexpr int JB = KW > 1 ? 4 * 32 * (DP + 1) * 4 : 0;
+  constexpr int STAGES = 4 * TB <= 140 * 1024 ? 2 : 1;
+  constexpr int BYTES = STAGES * 2 * TB > JB ? STAGES * 2 * TB : JB;
+  __shared__ __attribute__((aligned(16))) char smem[BYTES];
+  __shared__ float sm[4][32], sl[4][32];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5, l32 = lane & 31;
+  const int rw = wave / KW, kw = wave % KW;
+  const int hk = blockIdx.y;
+  const int split = blockIdx.x % a.splits;
+  const XaPlace f = xa_place(a, blockIdx.x / a.splits, RW * 32, false);
+  if (f.tile < 0) return;
+  const int rows = f.nq * a.group, row = f.tile * RW * 32 + rw * 32 + l32;
+  const int tiles = (f.nk + BN - 1) / BN;
+  const int t0 = (int)((long long)tiles * split / a.splits), t1 = (int)((long long)tiles * (split + 1) / a.splits);
+  const bool live = row < rows;
+  const int qi = live ? row / a.group : 0, head = hk * a.group + (live ? row - qi * a.group : 0);
+  const T* kbase = (const T*)a.k + f.k0 * a.sk + hk * a.hk;
+  const T* vbase = (const T*)a.v + f.k0 * a.sv + hk * a.hv;
+  typename XaFrag<T>::vec Q[KS];
+  {
+    const T* p = (const T*)a.q + (f.q0 + qi) * a.sq + head * a.hq;
+#pragma unroll
+    for (int s = 0; s < KS; ++s) {
+      if (live) Q[s] = xa_row<T>(p, s * 16 + half * 8, a.dim);
+      else Q[s] = typename XaFrag<T>::vec{};
+    }
+  }
+  xf16 O[DT];
+#pragma unroll
+  for (int i = 0; i < DT; ++i) O[i] = (xf16)(0.f);
+  float m = -INFINITY, l = 0.f;
+  XaStage<T, DP, BN, 256> ks, vs;
+  unsigned long long ok[2], nok[2];
+  auto fetch = [&](int t) {
+    const int k0 = t * BN;
+#pragma unroll
+    for (int h = 0; h < BN / 64; ++h) nok[h] = xa_valid(a.mask, f.k0 + k0 + h * 64, f.nk - k0 - h * 64);
+    auto on = [&](int r) { return (nok[BN == 64 ? 0 : r >> 6] >> (r & 63)) & 1; };
+    ks.fetch([&](int r) { return on(r) ? kbase + (long long)(k0 + r) * a.sk : (const T*)nullptr; }, a.dim);
+    vs.fetch([&](int r) { return on(r) ? vbase + (long long)(k0 + r) * a.sv : (const T*)nullptr; }, a.dim);
+  };
+  if (t0 < t1) {
+    fetch(t0);
+    ks.put(smem); vs.put(smem + TB);
+  }
+  ok[0] = nok[0]; ok[1] = nok[1];
+  __syncthreads();
+  int buf = 0;
+  for (int t = t0; t < t1; ++t) {
+    const bool more = t + 1 < t1;
+    if (more) fetch(t + 1);
+    const char* tk = smem + (STAGES == 2 ? buf * 2 * TB : 0);
+    const char* tv = tk + TB;
+    if (KU == KW || kw < KU) {
+#pragma unroll
+      for (int u = 0; u < SUB; ++u) {
+        const int c0 = (u * KU + kw) * 32;                    // first of this wave's 32 keys in the tile
+        const unsigned valid = (unsigned)(ok[BN == 64 ? 0 : c0 >> 6] >> (c0 & 63));
+        if (!valid) continue;
+        xf16 s = (xf16)(0.f);
+#pragma unroll
+        for (int k = 0; k < KS; ++k) xa_mma(s, xa_along<T, DP>(tk, c0 + l32, k, half), Q[k]);
+        float top = -INFINITY;
+        if (valid == 0xffffffffu) {
+#pragma unroll
+          for (int i = 0; i < 16; ++i) { s[i] *= a.scale2; top = fmaxf(top, s[i]); }
+        } else {
+          const unsigned mine = valid >> (half * 4);
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            s[i] = (mine >> ((i >> 2) * 8 + (i & 3))) & 1 ? s[i] * a.scale2 : -INFINITY;
+            top = fmaxf(top, s[i]);
+          }
+        }
+        top = fmaxf(top, __shfl_xor(top, 32, 64));
+        const float now = fmaxf(m, top), at = now == -INFINITY ? 0.f : now;
+        const float shrink = exp2f(m - at);
+        m = now;
+        float sum = 0.f;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) { s[i] = exp2f(s[i] - at); sum += s[i]; }
+        l = l * shrink + sum;
+#pragma unroll
+        for (int i = 0; i < DT; ++i)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) O[i][e] *= shrink;
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          const typename XaFrag<T>::vec p = xa_pack<T>(s, c);
+#pragma unroll
+          for (int i = 0; i < DT; ++i) xa_mma(O[i], xa_down<T, DP>(tv, c0 + c * 16, i * 32, lane), p);
+        }
+      }
+    }
+    if (STAGES == 1) __syncthreads();
+    if (more) {
+      char* n = smem + (STAGES == 2 ? (buf ^ 1) * 2 * TB : 0);
+      ks.put(n); vs.put(n + TB);
+    }
+    ok[0] = nok[0]; ok[1] = nok[1];
+    __syncthreads();
+    buf ^= 1;
+  }
+  l += __shfl_xor(l, 32, 64);
+  if (KW > 1) {                                               // the waves of a row tile, joined in order
+    if (half == 0) { sm[wave][l32] = m; sl[wave][l32] = l; }
+    __syncthreads();
+    float top = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < KW; ++i) top = fmaxf(top, sm[rw * KW + i][l32]);
+    const float at = top == -INFINITY ? 0.f : top;
+    float* x = (float*)smem + wave * 32 * (DP + 1);
+    const float w = exp2f(m - at);
+    float all = 0.f;
+#pragma unroll
+    for (int i = 0; i < KW; ++i) all += sl[rw * KW + i][l32] * exp2f(sm[rw * KW + i][l32] - at);
+#pragma unroll
+    for (int i = 0; i < DT; ++i)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) x[l32 * (DP + 1) + i * 32 + (e >> 2) * 8 + half * 4 + (e & 3)] = O[i][e] * w;
+    __syncthreads();
+    m = top; l = all;
+    if (kw == 0) {
+#pragma unroll
+      for (int i = 0; i < DT; ++i)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          float v = 0.f;
+#pragma unroll
+          for (int j = 0; j < KW; ++j)
+            v += x[j * 32 * (DP + 1) + l32 * (DP + 1) + i * 32 + (e >> 2) * 8 + half * 4 + (e & 3)];
+          O[i][e] = v;
+        }
+    }
+  }
+  if (!live || kw != 0) return;
+  const long long at = (f.q0 + qi) * a.heads + head;
+  if (a.splits > 1) {
+    float* part = a.part + ((long long)split * a.nq * a.heads + at) * (a.dim + 2);
+#pragma unroll
+    for (int i = 0; i < DT; ++i)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        const int d = i * 32 + (e >> 2) * 8 + half * 4 + (e & 3);
+        if (d < a.dim) part[2 + d] = O[i][e];
+      }
+    if (half == 0) { part[0] = m; part[1] = l; }
+    return;
+  }
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  T* out = (T*)a.out + at * a.dim;
+#pragma unroll
+  for (int i = 0; i < DT; ++i)
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const int d = i * 32 + g * 8 + half * 4;
+      typename GlxVec<T, 4>::vec v;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] = (T)(O[i][g * 4 + e] * inv);
+      if (d + 4 <= a.dim) GlxVec<T, 4>::store(out + d, v);
+      else
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (d + e < a.dim) out[d + e] = v[e];
+    }
+  if (a.lse && half == 0) a.lse[at] = l == 0.f ? INFINITY : m + log2f(l);
+}
+
+// the splits of a row: one wave per row
+template <typename T>
+__global__ __launch_bounds__(256) void k_xa_join(XaArgs a) {
+  const long long at = (long long)blockIdx.x * 4 + (threadIdx.x >> 6), rows = a.nq * a.heads;
+  const int lane = threadIdx.x & 63;
+  if (at >= rows) return;
+  const long long step = rows * (a.dim + 2);
+  const float* part = a.part + at * (a.dim + 2);
+  float top = -INFINITY;
+  for (int s = lane; s < a.splits; s += 64) top = fmaxf(top, part[s * step]);
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o, 64));
+  const float base = top == -INFINITY ? 0.f : top;
+  float l = 0.f;
+  for (int s = lane; s < a.splits; s += 64) l += part[s * step + 1] * exp2f(part[s * step] - base);
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) l += __shfl_xor(l, o, 64);
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  for (int d = lane; d < a.dim; d += 64) {
+    float v = 0.f;
+#pragma unroll 4
+    for (int s = 0; s < a.splits; ++s) v += part[s * step + 2 + d] * exp2f(part[s * step] - base);
+    ((T*)a.out)[at * a.dim + d] = (T)(v * inv);
+  }
+  if (a.lse && lane == 0) a.lse[at] = l == 0.f ? INFINITY : top + log2f(l);
+}
+
+// ------------------------------------------------------------------------------------------------ host
+int xa_splits(long long blocks, long long keys_per_frame) {
+  if (blocks < 1) blocks = 1;
+  long long s = 1024 / blocks, most = keys_per_frame / 256;        // 256 keys a split, at least
+  s = s < most ? s : most;
+  return (int)(s < 1 ? 1 : (s > 256 ? 256 : s));
+}
+struct XaForward { int rw, splits; long long tiles; };
+static XaForward xa_forward_plan(const glx_attention* t) {
+  XaForward p;
+  const int group = t->heads / t->kv_heads;
+  const bool counts = t->q_cnt != nullptr;
+  const long long rows = counts ? t->q_rows * group / (t->frames > 0 ? t->frames : 1) : (long long)t->q_len * group;
+  p.rw = rows <= 64 ? 1 : 4;
+  p.tiles = xa_tiles(t->q_rows * group, t->frames, (int)(t->q_len * group), counts, p.rw * 32);
+  const long long blocks = (counts ? t->q_rows * group / (p.rw * 32) + 1 : p.tiles) * t->kv_heads;
+  p.splits = xa_splits(blocks, t->frames > 0 ? t->k_rows / t->frames : 0);
+  return p;
+}
+
+int xa_check(const char* who, const glx_attention* t) {
+  GLX_REQUIRE(t, "%s: null descriptor", who);
+  GLX_REQUIRE(glx_elem_ok(t->dtype), "%s: dtype %d", who, t->dtype);
+  GLX_REQUIRE(t->frames >= 0 && t->q_rows >= 0 && t->k_rows >= 0 && t->heads >= 1 && t->kv_heads >= 1, "%s: negative sizes", who);
+  GLX_REQUIRE(t->heads % t->kv_heads == 0, "%s: %d heads over %d key heads", who, t->heads, t->kv_heads);
+  GLX_REQUIRE(t->dim >= 1 && t->dim <= 128, "%s: head dimension %d (1 .. 128)", who, t->dim);
+  GLX_REQUIRE(t->kv_heads <= 65535 && t->q_rows * t->heads < (1ll << 31) && t->k_rows * t->kv_heads < (1ll << 31), "%s: too many rows", who);
+  GLX_REQUIRE(!t->q_cnt == !t->k_cnt, "%s: counts of one side only", who);
+  GLX_REQUIRE(t->q_cnt || (t->q_len >= 0 && t->k_len >= 0 && t->q_len * t->frames == t->q_rows && t->k_len * t->frames == t->k_rows),
+              "%s: %d frames of %lld queries and %lld keys do not fill the tensors", who, t->frames, (long long)t->q_len, (long long)t->k_len);
+  GLX_REQUIRE(t->q_rows == 0 || (t->q && t->out), "%s: null queries or output", who);
+  GLX_REQUIRE(t->k_rows == 0 || (t->k && t->v), "%s: null keys or values", who);
+  return GLX_OK;
+}
+XaArgs xa_args(const glx_attention* t) {
+  XaArgs a = {};
+  a.q = t->q; a.k = t->k; a.v = t->v; a.out = t->out; a.o = t->out; a.lse = t->lse; a.mask = t->key_mask;
+  a.qcnt = t->q_cnt; a.kcnt = t->k_cnt;
+  a.sq = t->q_stride; a.hq = t->q_head_stride; a.sk = t->k_stride; a.hk = t->k_head_stride; a.sv = t->v_stride; a.hv = t->v_head_stride;
+  a.nq = t->q_rows; a.nk = t->k_rows;
+  a.frames = t->frames; a.lq = (int)t->q_len; a.lk = (int)t->k_len; a.heads = t->heads; a.kvheads = t->kv_heads;
+  a.group = t->heads / t->kv_heads; a.dim = t->dim; a.splits = 1;
+  a.scale = t->scale; a.scale2 = t->scale * 1.4426950408889634f;
+  return a;
+}
+
+extern "C" size_t glx_attention_workspace_bytes(const glx_attention* t) {
+  if (xa_check("glx_attention_workspace_bytes", t) != GLX_OK) return 0;
+  const XaForward p = xa_forward_plan(t);
+  return glx_align(p.splits > 1 ? (size_t)p.splits * t->q_rows * t->heads * (t->dim + 2) * sizeof(float) : 0) + 256;
+}
+
+template <typename T, int DP>
+static void xa_launch_forward(const XaForward& p, const XaArgs& a, hipStream_t st) {
+  const dim3 grid((unsigned)(p.tiles * p.splits), a.kvheads);
+  if (p.rw == 1) hipLaunchKernelGGL((k_xa_forward<T, DP, 1>), grid, dim3(256), 0, st, a);
+  else hipLaunchKernelGGL((k_xa_forward<T, DP, 4>), grid, dim3(256), 0, st, a);
+}
+template <typename T>
+static void xa_forward_of(const XaForward& p, const XaArgs& a, hipStream_t st) {
+  if (a.dim <= 32) xa_launch_forward<T, 32>(p, a, st);
+  else if (a.dim <= 64) xa_launch_forward<T, 64>(p, a, st);
+  else if (a.dim <= 96) xa_launch_forward<T, 96>(p, a, st);
+  else xa_launch_forward<T, 128>(p, a, st);
+  if (p.splits > 1) hipLaunchKernelGGL((k_xa_join<T>), dim3((unsigned)((a.nq * a.heads + 3) / 4)), dim3(256), 0, st, a);
+}
+
+extern "C" int glx_attention_forward(const glx_attention* t, void* workspace, size_t workspace_bytes, void* stream) {
+  if (int rc = xa_check("glx_attention_forward", t)) return rc;
+  if (t->q_rows == 0) return GLX_OK;
+  const XaForward p = xa_forward_plan(t);
+  XaArgs a = xa_args(t);
+  a.splits = p.splits;
+  a.part = (float*)workspace;
+  if (p.splits > 1 && (!workspace || workspace_bytes < glx_attention_workspace_bytes(t) - 256)) {
+    glx_set_error("glx_attention_forward: workspace %zu < %zu bytes", workspace_bytes, glx_attention_workspace_bytes(t));
+    return GLX_EWORKSPACE;
+  }
+  GLX_REQUIRE(p.tiles * p.splits < (1ll << 31), "glx_attention_forward: too many rows");
+  hipStream_t st = (hipStream_t)stream;
+  if (t->dtype == GLX_F32) xa_forward_of<float>(p, a, st);
+  else if (t->dtype == GLX_BF16) xa_forward_of<__bf16>(p, a, st);
+  else xa_forward_of<_Float16>(p, a, st);
+  GLX_LAUNCH_CHECK();
+  return GLX_OK;
+}

@@ -1,0 +1,414 @@
+// Cross attention of stacked frames, backward (glenet_amd/attention.py; the layouts: glx_attention.h).
+//
+//   P = 2^(scale2 Q K^T - lse),  dP = dO V^T,  delta = rowsum(dO O),  dS = P (dP - delta)
+//   dQ = scale dS K,   dK = scale dS^T Q,   dV = P^T dO
+//
+// Nothing of the size of the scores is stored: P is formed again from Q, K and the row's lse in each of two launches, one that
+// owns rows (dQ, and delta for the other one) and one that owns keys (dK, dV; the rows of all query heads that share a key head
+// are its sum).  Seven tile products instead of the five of a single pass that would need atomics or a second dQ buffer; the
+// results are the same bits every time.  Few tiles are split over the other side and added by a last launch.
+//
+// P and dS are rounded to the inputs' type in front of their products.  fp16 would lose both to its range -- over a thousand
+// keys P sits where fp16 has few bits left, and dS inherits the loss' scale -- so P is multiplied by 2^12 and dS by a power of
+// two that keeps a wave's largest value between 2^8 and 2^15 (taken from the first tile, lowered with the accumulators when a
+// later tile would pass it).
+#include "glx_attention.h"
+
+#define XA_PSCALE 4096.f      // fp16: of P
+
+int xa_splits(long long blocks, long long keys_per_frame);
+int xa_check(const char* who, const glx_attention* t);
+XaArgs xa_args(const glx_attention* t);
+
+// fp16: 2^e for the values of one 32 x 32 tile; N accumulators of earlier tiles follow a change
+template <typename T, int N>
+__device__ __forceinline__ void xa_range(xf16& s, xf16 (&acc)[N], int& e) {
+  if constexpr (__is_same(T, _Float16)) {
+    float top = 0.f;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) top = fmaxf(top, fabsf(s[i]));
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o, 64));
+    if (top > 0.f && top < 3e38f) {
+      const int want = 8 - ilogbf(top);
+      if (e > 200) {
+        e = want > 120 ? 120 : want;
+      } else if (ldexpf(top, e) >= 32768.f) {
+        const float f = ldexpf(1.f, want - e);
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+#pragma unroll
+          for (int k = 0; k < 16; ++k) acc[i][k] *= f;
+        e = want;
+      }
+    }
+    const float f = ldexpf(1.f, e > 200 ? 0 : e);
+#pragma unroll
+    for (int i = 0; i < 16; ++i) s[i] *= f;
+  }
+}
+template <typename T>
+__device__ __forceinline__ float xa_unrange(int e) {
+  return __is_same(T, _Float16) && e <= 200 ? ldexpf(1.f, -e) : 1.f;
+}
+
+// ------------------------------------------------------------------------------------------------ dQ, delta
+template <typename T, int DP, int RW>
+__global__ __launch_bounds__(256) void k_xa_dq(XaArgs a) {
+  constexpr int KW = 4 / RW, BN = XA_KEYS, KU = BN / 32 < KW ? BN / 32 : KW, SUB = BN / 32 / KU;
+  constexpr int KS = DP / 16, DT = DP / 32;
+  typedef XaTile<T, DP> Tile;
+  constexpr int TB = BN * Tile::LD;
+  constexpr int JB = KW > 1 ? 4 * 32 * (DP + 1) * 4 : 0;
+  constexpr int STAGES = 4 * TB <= 140 * 1024 ? 2 : 1;
+  constexpr int BYTES = STAGES * 2 * TB > JB ? STAGES * 2 * TB : JB;
+  __shared__ __attribute__((aligned(16))) char smem[BYTES];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5, l32 = lane & 31;
+  const int rw = wave / KW, kw = wave % KW;
+  const int hk = blockIdx.y;
+  const int split = blockIdx.x % a.splits;
+  const XaPlace f = xa_place(a, blockIdx.x / a.splits, RW * 32, false);
+  if (f.tile < 0) return;
+  const int rows = f.nq * a.group, row = f.tile * RW * 32 + rw * 32 + l32;
+  const int tiles = a.dq ? (f.nk + BN - 1) / BN : 0;
+  const int t0 = (int)((long long)tiles * split / a.splits), t1 = (int)((long long)tiles * (split + 1) / a.splits);
+  const bool live = row < rows;
+  const int qi = live ? row / a.group : 0, head = hk * a.group + (live ? row - qi * a.group : 0);
+  const long long at = (f.q0 + qi) * a.heads + head;
+  const T* kbase = (const T*)a.k + f.k0 * a.sk + hk * a.hk;
+  const T* vbase = (const T*)a.v + f.k0 * a.sv + hk * a.hv;
+  typename XaFrag<T>::vec Q[KS], G[KS];
+  float delta = 0.f;
+  {
+    const T* p = (const T*)a.q + (f.q0 + qi) * a.sq + head * a.hq;
+    const T* g = (const T*)a.go + (f.q0 + qi) * a.sg + head * a.hg;
+    const T* o = (const T*)a.o + at * a.dim;
+#pragma unroll
+    for (int s = 0; s < KS; ++s) {
+      Q[s] = G[s] = typename XaFrag<T>::vec{};
+      if (!live) continue;
+      Q[s] = xa_row<T>(p, s * 16 + half * 8, a.dim);
+      G[s] = xa_row<T>(g, s * 16 + half * 8, a.dim);
+      const typename XaFrag<T>::vec x = xa_row<T>(o, s * 16 + half * 8, a.dim);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) delta += (float)G[s][i] * (float)x[i];
+    }
+    delta += __shfl_xor(delta, 32, 64);
+  }
+  const float lse = live ? a.lse[at] : INFINITY;
+  if (lse == INFINITY) delta = 0.f;                           // a row without keys: no gradient, whatever dO holds
+  if (live && kw == 0 && half == 0 && split == 0) a.delta[at] = delta;
+  if (!a.dq) return;
+  xf16 D[DT];
+#pragma unroll
+  for (int i = 0; i < DT; ++i) D[i] = (xf16)(0.f);
+  int e = 999;
+  XaStage<T, DP, BN, 256> ks, vs;
+  unsigned long long ok = 0, nok = 0;
+  auto fetch = [&](int t) {
+    const int k0 = t * BN;
+    nok = xa_valid(a.mask, f.k0 + k0, f.nk - k0);
+    ks.fetch([&](int r) { return (nok >> r) & 1 ? kbase + (long long)(k0 + r) * a.sk : (const T*)nullptr; }, a.dim);
+    vs.fetch([&](int r) { return (nok >> r) & 1 ? vbase + (long long)(k0 + r) * a.sv : (const T*)nullptr; }, a.dim);
+  };
+  if (t0 < t1) {
+    fetch(t0);
+    ks.put(smem); vs.put(smem + TB);
+  }
+  ok = nok;
+  __syncthreads();
+  int buf = 0;
+  for (int t = t0; t < t1; ++t) {
+    const bool more = t + 1 < t1;
+    if (more) fetch(t + 1);
+    const char* tk = smem + (STAGES == 2 ? buf * 2 * TB : 0);
+    const char* tv = tk + TB;
+    if (kw < KU) {
+#pragma unroll
+      for (int u = 0; u < SUB; ++u) {
+        const int c0 = (u * KU + kw) * 32;
+        const unsigned valid = (unsigned)(ok >> c0);
+        if (!valid) continue;
+        xf16 s = (xf16)(0.f), d = (xf16)(0.f);
+#pragma unroll
+        for (int k = 0; k < KS; ++k) {
+          xa_mma(s, xa_along<T, DP>(tk, c0 + l32, k, half), Q[k]);
+          xa_mma(d, xa_along<T, DP>(tv, c0 + l32, k, half), G[k]);
+        }
+        const unsigned mine = valid >> (half * 4);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const float p = exp2f(s[i] * a.scale2 - lse) * (d[i] - delta);
+          s[i] = (mine >> ((i >> 2) * 8 + (i & 3))) & 1 ? p : 0.f;
+        }
+        xa_range<T, DT>(s, D, e);
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          const typename XaFrag<T>::vec p = xa_pack<T>(s, c);
+#pragma unroll
+          for (int i = 0; i < DT; ++i) xa_mma(D[i], xa_down<T, DP>(tk, c0 + c * 16, i * 32, lane), p);
+        }
+      }
+    }
+    if (STAGES == 1) __syncthreads();
+    if (more) {
+      char* n = smem + (STAGES == 2 ? (buf ^ 1) * 2 * TB : 0);
+      ks.put(n); vs.put(n + TB);
+    }
+    ok = nok;
+    __syncthreads();
+    buf ^= 1;
+  }
+  const float size = a.scale * xa_unrange<T>(e);
+#pragma unroll
+  for (int i = 0; i < DT; ++i)
+#pragma unroll
+    for (int k = 0; k < 16; ++k) D[i][k] *= size;
+  if (KW > 1) {
+    float* x = (float*)smem + wave * 32 * (DP + 1);
+#pragma unroll
+    for (int i = 0; i < DT; ++i)
+#pragma unroll
+      for (int k = 0; k < 16; ++k) x[l32 * (DP + 1) + i * 32 + (k >> 2) * 8 + half * 4 + (k & 3)] = D[i][k];
+    __syncthreads();
+    if (kw == 0) {
+#pragma unroll
+      for (int i = 0; i < DT; ++i)
+#pragma unroll
+        for (int k = 0; k < 16; ++k) {
+          float v = 0.f;
+#pragma unroll
+          for (int j = 0; j < KU; ++j) v += x[j * 32 * (DP + 1) + l32 * (DP + 1) + i * 32 + (k >> 2) * 8 + half * 4 + (k & 3)];
+          D[i][k] = v;
+        }
+    }
+  }
+  if (!live || kw != 0) return;
+  float* part = a.part + ((long long)split * a.nq * a.heads + at) * a.dim;
+  T* out = (T*)a.dq + at * a.dim;
+#pragma unroll
+  for (int i = 0; i < DT; ++i)
+#pragma unroll
+    for (int g = 0; g < 4; ++g)
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const int d = i * 32 + g * 8 + half * 4 + k;
+        if (d >= a.dim) continue;
+        if (a.splits > 1) part[d] = D[i][g * 4 + k];
+        else out[d] = (T)D[i][g * 4 + k];
+      }
+}
+
+// ------------------------------------------------------------------------------------------------ dK, dV
+template <typename T, int DP>
+__global__ __launch_bounds__(256) void k_xa_dkv(XaArgs a) {
+  constexpr int BM = sizeof(T) == 2 ? 64 : 32;
+  constexpr int KS = DP / 16, DT = DP / 32;
+  typedef XaTile<T, DP> Tile;
+  constexpr int TB = BM * Tile::LD;
+  __shared__ __attribute__((aligned(16))) char smem[2 * 2 * TB];
+  __shared__ __attribute__((aligned(16))) float srow[2][2][BM];         // stage; lse, delta
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5, l32 = lane & 31;
+  const int hk = blockIdx.y;
+  const int split = blockIdx.x % a.splits;
+  const XaPlace f = xa_place(a, blockIdx.x / a.splits, 128, true);
+  if (f.tile < 0) return;
+  const int rows = f.nq * a.group, key = f.tile * 128 + wave * 32 + l32;
+  const int tiles = (rows + BM - 1) / BM;
+  const int t0 = (int)((long long)tiles * split / a.splits), t1 = (int)((long long)tiles * (split + 1) / a.splits);
+  const bool there = key < f.nk, valid = there && (!a.mask || a.mask[f.k0 + key] != 0);
+  typename XaFrag<T>::vec K[KS], V[KS];
+  {
+    const T* k = (const T*)a.k + (f.k0 + key) * a.sk + hk * a.hk;
+    const T* v = (const T*)a.v + (f.k0 + key) * a.sv + hk * a.hv;
+#pragma unroll
+    for (int s = 0; s < KS; ++s) {
+      K[s] = V[s] = typename XaFrag<T>::vec{};
+      if (!valid) continue;
+      K[s] = xa_row<T>(k, s * 16 + half * 8, a.dim);
+      V[s] = xa_row<T>(v, s * 16 + half * 8, a.dim);
+    }
+  }
+  xf16 dK[DT], dV[DT];
+#pragma unroll
+  for (int i = 0; i < DT; ++i) dK[i] = dV[i] = (xf16)(0.f);
+  int e = 999;
+  XaStage<T, DP, BM, 256> qs, gs;
+  float lse = INFINITY, delta = 0.f;
+  auto fetch = [&](int t) {
+    const int r0 = t * BM;
+    auto place = [&](const void* base, long long s, long long h, int r) -> const T* {
+      if (r0 + r >= rows) return nullptr;
+      const int qi = (int)((unsigned)(r0 + r) / (unsigned)a.group);
+      return (const T*)base + (f.q0 + qi) * s + (hk * a.group + (r0 + r - qi * a.group)) * h;
+    };
+    qs.fetch([&](int r) { return place(a.q, a.sq, a.hq, r); }, a.dim);
+    gs.fetch([&](int r) { return place(a.go, a.sg, a.hg, r); }, a.dim);
+    lse = INFINITY; delta = 0.f;
+    if ((int)threadIdx.x < BM && r0 + (int)threadIdx.x < rows) {
+      const int r = r0 + threadIdx.x, qi = (int)((unsigned)r / (unsigned)a.group);
+      const long long at = (f.q0 + qi) * a.heads + hk * a.group + (r - qi * a.group);
+      lse = a.lse[at]; delta = a.delta[at];
+    }
+  };
+  auto put = [&](int buf) {
+    qs.put(smem + buf * 2 * TB);
+    gs.put(smem + buf * 2 * TB + TB);
+    if ((int)threadIdx.x < BM) { srow[buf][0][threadIdx.x] = lse; srow[buf][1][threadIdx.x] = delta; }
+  };
+  if (t0 < t1) { fetch(t0); put(0); }
+  __syncthreads();
+  int buf = 0;
+  for (int t = t0; t < t1; ++t) {
+    const bool more = t + 1 < t1;
+    if (more) fetch(t + 1);
+    const char* tq = smem + buf * 2 * TB;
+    const char* tg = tq + TB;
+#pragma unroll
+    for (int u = 0; u < BM / 32; ++u) {
+      xf16 s = (xf16)(0.f), d = (xf16)(0.f);
+#pragma unroll
+      for (int k = 0; k < KS; ++k) {
+        xa_mma(s, xa_along<T, DP>(tq, u * 32 + l32, k, half), K[k]);
+        xa_mma(d, xa_along<T, DP>(tg, u * 32 + l32, k, half), V[k]);
+      }
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const xf4 ls = *reinterpret_cast<const xf4*>(&srow[buf][0][u * 32 + g * 8 + half * 4]);
+        const xf4 de = *reinterpret_cast<const xf4*>(&srow[buf][1][u * 32 + g * 8 + half * 4]);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float p = exp2f(s[g * 4 + i] * a.scale2 - ls[i]);
+          s[g * 4 + i] = valid ? p : 0.f;
+          d[g * 4 + i] = valid ? p * (d[g * 4 + i] - de[i]) : 0.f;
+        }
+      }
+      if constexpr (__is_same(T, _Float16)) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) s[i] *= XA_PSCALE;
+      }
+      xa_range<T, DT>(d, dK, e);
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        const typename XaFrag<T>::vec p = xa_pack<T>(s, c), q = xa_pack<T>(d, c);
+#pragma unroll
+        for (int i = 0; i < DT; ++i) {
+          xa_mma(dV[i], xa_down<T, DP>(tg, u * 32 + c * 16, i * 32, lane), p);
+          xa_mma(dK[i], xa_down<T, DP>(tq, u * 32 + c * 16, i * 32, lane), q);
+        }
+      }
+    }
+    if (more) put(buf ^ 1);
+    __syncthreads();
+    buf ^= 1;
+  }
+  if (!there) return;
+  const float ksize = a.scale * xa_unrange<T>(e), vsize = __is_same(T, _Float16) ? 1.f / XA_PSCALE : 1.f;
+  const long long at = (f.k0 + key) * a.kvheads + hk, n = a.nk * a.kvheads * a.dim;
+  float* pk = a.part + (long long)split * 2 * n + at * a.dim;
+#pragma unroll
+  for (int i = 0; i < DT; ++i)
+#pragma unroll
+    for (int g = 0; g < 4; ++g)
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const int d = i * 32 + g * 8 + half * 4 + k;
+        if (d >= a.dim) continue;
+        const float x = dK[i][g * 4 + k] * ksize, y = dV[i][g * 4 + k] * vsize;
+        if (a.splits > 1) {
+          pk[d] = x; pk[n + d] = y;
+        } else {
+          if (a.dk) ((T*)a.dk)[at * a.dim + d] = (T)x;
+          if (a.dv) ((T*)a.dv)[at * a.dim + d] = (T)y;
+        }
+      }
+}
+
+// out = the splits' sum, in order
+template <typename T>
+__global__ __launch_bounds__(256) void k_xa_sum(const float* __restrict__ part, long long n, long long step, int splits, T* __restrict__ out) {
+  for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < n; i += (long long)gridDim.x * 256) {
+    float v = 0.f;
+#pragma unroll 4
+    for (int s = 0; s < splits; ++s) v += part[s * step + i];
+    out[i] = (T)v;
+  }
+}
+
+// ------------------------------------------------------------------------------------------------ host
+struct XaBackward { int rw, qsplits, ksplits; long long qtiles, ktiles; size_t delta, qpart, kpart, bytes; };
+static XaBackward xa_backward_plan(const glx_attention* t) {
+  XaBackward p;
+  const int group = t->heads / t->kv_heads, fr = t->frames > 0 ? t->frames : 1;
+  const bool counts = t->q_cnt != nullptr;
+  const long long rows = t->q_rows * group / fr, keys = t->k_rows / fr;
+  p.rw = rows <= 128 ? 1 : 4;
+  p.qtiles = xa_tiles(t->q_rows * group, t->frames, (int)(t->q_len * group), counts, p.rw * 32);
+  p.ktiles = xa_tiles(t->k_rows, t->frames, (int)t->k_len, counts, 128);
+  p.qsplits = xa_splits((counts ? t->q_rows * group / (p.rw * 32) + 1 : p.qtiles) * t->kv_heads, keys);
+  p.ksplits = xa_splits((counts ? t->k_rows / 128 + 1 : p.ktiles) * t->kv_heads, rows);
+  p.delta = 0;
+  p.qpart = glx_align((size_t)t->q_rows * t->heads * sizeof(float));
+  p.kpart = p.qpart + (p.qsplits > 1 ? glx_align((size_t)p.qsplits * t->q_rows * t->heads * t->dim * sizeof(float)) : 0);
+  p.bytes = p.kpart + (p.ksplits > 1 ? glx_align((size_t)p.ksplits * 2 * t->k_rows * t->kv_heads * t->dim * sizeof(float)) : 0);
+  return p;
+}
+extern "C" size_t glx_attention_backward_workspace_bytes(const glx_attention* t) {
+  if (xa_check("glx_attention_backward_workspace_bytes", t) != GLX_OK) return 0;
+  return xa_backward_plan(t).bytes + 256;
+}
+
+template <typename T, int DP>
+static void xa_launch_backward(const XaBackward& p, XaArgs& a, char* ws, hipStream_t st) {
+  if (p.qtiles) {
+    const dim3 grid((unsigned)(p.qtiles * p.qsplits), a.kvheads);
+    a.splits = p.qsplits;
+    a.part = (float*)(ws + p.qpart);
+    if (p.rw == 1) hipLaunchKernelGGL((k_xa_dq<T, DP, 1>), grid, dim3(256), 0, st, a);
+    else hipLaunchKernelGGL((k_xa_dq<T, DP, 4>), grid, dim3(256), 0, st, a);
+    if (a.dq && p.qsplits > 1) {
+      const long long n = a.nq * a.heads * a.dim, blocks = (n + 1023) / 1024;
+      hipLaunchKernelGGL((k_xa_sum<T>), dim3((unsigned)(blocks < 4096 ? blocks : 4096)), dim3(256), 0, st, a.part, n, n, p.qsplits, (T*)a.dq);
+    }
+  }
+  if (p.ktiles && (a.dk || a.dv)) {
+    a.splits = p.ksplits;
+    a.part = (float*)(ws + p.kpart);
+    hipLaunchKernelGGL((k_xa_dkv<T, DP>), dim3((unsigned)(p.ktiles * p.ksplits), a.kvheads), dim3(256), 0, st, a);
+    if (p.ksplits > 1) {
+      const long long n = a.nk * a.kvheads * a.dim, blocks = (n + 1023) / 1024;
+      const dim3 grid((unsigned)(blocks < 4096 ? blocks : 4096));
+      if (a.dk) hipLaunchKernelGGL((k_xa_sum<T>), grid, dim3(256), 0, st, a.part, n, 2 * n, p.ksplits, (T*)a.dk);
+      if (a.dv) hipLaunchKernelGGL((k_xa_sum<T>), grid, dim3(256), 0, st, a.part + n, n, 2 * n, p.ksplits, (T*)a.dv);
+    }
+  }
+}
+template <typename T>
+static void xa_backward_of(const XaBackward& p, XaArgs& a, char* ws, hipStream_t st) {
+  if (a.dim <= 32) xa_launch_backward<T, 32>(p, a, ws, st);
+  else if (a.dim <= 64) xa_launch_backward<T, 64>(p, a, ws, st);
+  else if (a.dim <= 96) xa_launch_backward<T, 96>(p, a, ws, st);
+  else xa_launch_backward<T, 128>(p, a, ws, st);
+}
+
+extern "C" int glx_attention_backward(const glx_attention* t, const void* grad_out, int64_t g_stride, int64_t g_head_stride,
+                                      void* dq, void* dk, void* dv, void* workspace, size_t workspace_bytes, void* stream) {
+  if (int rc = xa_check("glx_attention_backward", t)) return rc;
+  GLX_REQUIRE(t->q_rows == 0 || (grad_out && t->lse), "glx_attention_backward: null gradient or lse");
+  const XaBackward p = xa_backward_plan(t);
+  if (!workspace || workspace_bytes < p.bytes) {
+    glx_set_error("glx_attention_backward: workspace %zu < %zu bytes", workspace_bytes, p.bytes);
+    return GLX_EWORKSPACE;
+  }
+  GLX_REQUIRE(p.qtiles * p.qsplits < (1ll << 31) && p.ktiles * p.ksplits < (1ll << 31), "glx_attention_backward: too many rows");
+  XaArgs a = xa_args(t);
+  a.go = grad_out; a.sg = g_stride; a.hg = g_head_stride;
+  a.dq = dq; a.dk = dk; a.dv = dv;
+  a.delta = (float*)workspace;
+  hipStream_t st = (hipStream_t)stream;
+  if (t->dtype == GLX_F32) xa_backward_of<float>(p, a, (char*)workspace, st);
+  else if (t->dtype == GLX_BF16) xa_backward_of<__bf16>(p, a, (char*)workspace, st);
+  else xa_backward_of<_Float16>(p, a, (char*)workspace, st);
+  GLX_LAUNCH_CHECK();
+  return GLX_OK;
+}

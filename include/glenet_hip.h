@@ -1526,6 +1526,31 @@ int glx_muon_moments(float* params, const float* grads, float* exp_avg, float* e
 int glx_muon_apply(float* params, const float* update, const glx_opt_chunk* chunks, int nchunks, const float* hyper,
                    float weight_decay, void* stream);
 
+/* ---- cross attention of stacked frames (glenet_amd/attention.py) ----
+ * out (q_rows, heads, dim) = softmax(scale q k^T) v, every query over the unmasked keys of its own frame.  q (q_rows, heads,
+ * dim), k / v (k_rows, kv_heads, dim) of `dtype` with unit stride inside a head and the given strides (elements) between rows
+ * and heads; heads / kv_heads query heads share a key head.  Frames lie behind each other: q_cnt / k_cnt (frames) int32 DEVICE
+ * counts (clamped into the tensors; rows behind the last frame give zeros), or both NULL and q_len / k_len rows per frame.
+ * key_mask (k_rows) bytes, 0 = not attended and never read; NULL: none.  A row without keys gives 0.  lse (q_rows, heads) fp32:
+ * the rows' base-2 log-sum-exp for the backward pass (+inf without keys), NULL: inference.  dim 1 .. 128. */
+typedef struct glx_attention {
+  const void* q; const void* k; const void* v;
+  void* out; float* lse;
+  const uint8_t* key_mask;
+  const int32_t* q_cnt; const int32_t* k_cnt;
+  int64_t q_rows, k_rows, q_len, k_len;
+  int64_t q_stride, q_head_stride, k_stride, k_head_stride, v_stride, v_head_stride;
+  int32_t frames, heads, kv_heads, dim, dtype;
+  float scale;
+} glx_attention;
+size_t glx_attention_workspace_bytes(const glx_attention* t);       /* 0: bad arguments */
+int glx_attention_forward(const glx_attention* t, void* workspace, size_t workspace_bytes, void* stream);
+/* The gradients from grad_out (q_rows, heads, dim; its own strides), with `t` as the forward call left it (out, lse): dq as q's
+ * shape, dk / dv as k's, dense.  Fixed summation orders (no atomics). */
+size_t glx_attention_backward_workspace_bytes(const glx_attention* t);
+int glx_attention_backward(const glx_attention* t, const void* grad_out, int64_t g_stride, int64_t g_head_stride, void* dq,
+                           void* dk, void* dv, void* workspace, size_t workspace_bytes, void* stream);
+
 /* Stage stamps: a one-thread launch on `stream` that stores the device's constant 100 MHz wall clock into
  * stamps[slot] (10 ns per tick).  Recorded into a captured training step at its stage boundaries
  * (StaticTrainPipeline.mark) it times the stages inside graph replays; the reference has no counterpart (it times

@@ -1,0 +1,387 @@
+"""glenet_amd.attention.cross_attention (csrc/glx_attention.hip, glx_attention_bwd.hip) against the formulas in 64 bits.
+
+Tolerances, computed per output element from the inputs (u = 2^-24, h = half a step of the inputs' type, 2^-24 for fp32):
+  a product over D terms is off by (D + 8) u sum |terms|; a score s in base 2 by es = that + 4 u |s|, a probability by a relative
+  ep = 2 es + 16 u + the row's own sum (depth N: N u).
+  O:  (2 ep + N u + h) sum p |v| + h |O|            (h: p rounded in front of its product; the second one: the result)
+  dP, delta: (D + 8) u sum |terms|, delta also h sum |dO O| (from the rounded O);  dS: eds = p (edp + edelta) + (ep + h) |dS|
+  dQ: scale (sum eds |k| + N u sum |dS k|) + h |dQ|, dK alike over the M rows, dV: sum (ep + h + M u) p |dO| + h |dV|
+  fp16: p below 2^-14 of its scale loses up to 2^-25: + 2^-25 sum |v| / l forward; backward P carries 2^12, dS 2^8 over a tile's
+  largest value: + 2^-24 max |dS| sum |k|.  Nothing below half a subnormal step of the result's type is asked for."""
+import math
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+U = 2.0 ** -24
+HALF = {torch.float32: 2.0 ** -24, torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11}
+SUB = {torch.float32: 2.0 ** -149, torch.bfloat16: 2.0 ** -134, torch.float16: 2.0 ** -25}
+
+# q lengths, k lengths, heads, key heads, dim, mask, padded
+CASES = [
+    ([1], [1], 1, 1, 8, False, True),
+    ([1, 1], [7, 7], 4, 2, 16, True, True),
+    ([1, 1, 1], [2000, 2000, 2000], 8, 2, 64, False, True),
+    ([33, 33], [65, 65], 3, 3, 40, True, True),
+    ([130], [300], 2, 1, 128, False, True),
+    ([5, 0, 200, 17], [64, 90, 0, 1301], 4, 4, 32, False, False),
+    ([64, 1, 129], [63, 257, 128], 6, 2, 72, True, False),
+    ([31, 100], [1, 2], 7, 1, 20, False, False),
+    ([300], [500], 2, 2, 100, True, False),
+    ([4, 4], [3000, 900], 2, 1, 96, True, False),
+    ([700, 650], [40, 33], 4, 2, 64, False, False),
+    ([9, 3], [50, 70], 3, 1, 1, False, False),
+]
+
+
+def _frames(ql, kl):
+    q0 = k0 = 0
+    for a, b in zip(ql, kl):
+        yield q0, a, k0, b
+        q0, k0 = q0 + a, k0 + b
+
+
+def _inputs(case, dtype, seed, dev, tail=0):
+    ql, kl, h, hk, d, masked, padded = case
+    g = torch.Generator().manual_seed(seed)
+
+    def normal(*s):
+        return torch.randn(*s, generator=g).to(dtype).to(dev)
+
+    q, k, v, go = normal(sum(ql) + tail, h, d), normal(sum(kl) + tail, hk, d), normal(sum(kl) + tail, hk, d), normal(sum(ql) + tail, h, d)
+    mask = None
+    if masked:
+        mask = (torch.rand(sum(kl) + tail, generator=g) < 0.7).to(dev)
+        mask[:kl[0]] = False                                  # a frame without a state
+        if len(kl) > 1 and kl[1] > 2:
+            mask[kl[0]:kl[0] + kl[1]] = False
+            mask[kl[0] + kl[1] - 1] = True                    # one state, the last
+    cnts = None
+    if padded:
+        b = len(ql)
+        q, go = q.view(b, -1, h, d), go.view(b, -1, h, d)
+        k, v = k.view(b, -1, hk, d), v.view(b, -1, hk, d)
+        mask = mask.view(b, -1) if mask is not None else None
+    else:
+        cnts = tuple(torch.tensor(x, dtype=torch.int32, device=dev) for x in (ql, kl))
+    return q, k, v, go, mask, cnts
+
+
+def _reference(q, k, v, go, mask, case, dtype, scale=None):
+    """{name: (value, limit)} in 64 bits, on stacked rows."""
+    ql, kl, h, hk, d, _, _ = case
+    q, go = (t.detach().reshape(-1, h, d).double() for t in (q, go))
+    k, v = (t.detach().reshape(-1, hk, d).double() for t in (k, v))
+    mask = mask.reshape(-1) if mask is not None else torch.ones(k.shape[0], dtype=torch.bool, device=q.device)
+    scale = 1 / math.sqrt(d) if scale is None else scale
+    h_ = HALF[dtype]
+    fp16 = dtype == torch.float16
+    out = {n: [torch.zeros_like(t), torch.zeros_like(t)] for n, t in (("o", q), ("dq", q), ("dk", k), ("dv", v))}
+    for q0, lq, k0, lk in _frames(ql, kl):
+        live = torch.arange(k0, k0 + lk, device=q.device)[mask[k0:k0 + lk]]
+        if lq == 0 or live.numel() == 0:
+            continue
+        n = live.numel()
+        for j in range(h):
+            jk = j // (h // hk)
+            qq, gg, kk, vv = q[q0:q0 + lq, j], go[q0:q0 + lq, j], k[live, jk], v[live, jk]
+            s = qq @ kk.t() * scale
+            p = torch.softmax(s, 1)
+            o = p @ vv
+            dp = gg @ vv.t()
+            de = (gg * o).sum(1, keepdim=True)
+            ds = p * (dp - de)
+            es = ((d + 8) * U * (qq.abs() @ kk.abs().t()) * abs(scale) + 4 * U * s.abs()).amax(1, keepdim=True) * 1.5
+            ep = 2 * es + (16 + n) * U
+            tiny = 2.0 ** -25 * vv.abs().sum(0) if fp16 else 0.0
+            eo = (2 * ep + n * U + h_) * (p @ vv.abs()) + tiny
+            edp = (d + 8) * U * (gg.abs() @ vv.abs().t())
+            ede = (gg.abs() * ((d + 8) * U * o.abs() + eo + h_ * o.abs())).sum(1, keepdim=True)
+            eds = p * (edp + ede) + (ep + h_) * ds.abs()
+            if fp16:
+                eds = eds + 2.0 ** -24 * ds.abs().max()
+            out["o"][0][q0:q0 + lq, j] = o
+            out["o"][1][q0:q0 + lq, j] = eo
+            out["dq"][0][q0:q0 + lq, j] = scale * ds @ kk
+            out["dq"][1][q0:q0 + lq, j] = abs(scale) * (eds @ kk.abs() + n * U * (ds.abs() @ kk.abs()))
+            out["dk"][0][live, jk] += scale * ds.t() @ qq
+            out["dk"][1][live, jk] += abs(scale) * (eds.t() @ qq.abs() + h * lq * U * (ds.abs().t() @ qq.abs()))
+            out["dv"][0][live, jk] += p.t() @ gg
+            out["dv"][1][live, jk] += ((ep + h_ + h * lq * U) * p).t() @ gg.abs() + (2.0 ** -37 * gg.abs().sum(0) if fp16 else 0.0)
+    return out
+
+
+def _check(got, ref, name, dtype):
+    want, lim = ref[name]
+    got = got.detach().reshape(want.shape).double()
+    lim = lim + HALF[dtype] * want.abs() + SUB[dtype]
+    off = (got - want).abs()
+    assert bool((off <= lim).all()), "%s: %d of %d off, worst %.3g of its limit, nan %d" % (
+        name, int((~(off <= lim)).sum()), off.numel(), float((off / lim).nan_to_num(0).max()), int(torch.isnan(got).sum()))
+
+
+def _run(q, k, v, go, mask, cnts, **kw):
+    from glenet_amd.attention import cross_attention
+    leaves = [t.detach().requires_grad_(True) for t in (q, k, v)]
+    a = cnts if cnts is not None else (None, None)
+    o = cross_attention(*leaves, *a, key_mask=mask, **kw)
+    return [o] + list(torch.autograd.grad(o, leaves, go))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("index", range(len(CASES)))
+def test_cross_attention_and_its_gradients(dev, index, dtype):
+    from glenet_amd.attention import cross_attention
+    case = CASES[index]
+    q, k, v, go, mask, cnts = _inputs(case, dtype, index, dev)
+    outs = _run(q, k, v, go, mask, cnts)
+    ref = _reference(q, k, v, go, mask, case, dtype)
+    for t, n, like in zip(outs, ("o", "dq", "dk", "dv"), (q, q, k, v)):
+        assert t.shape == like.shape and t.dtype == dtype
+        _check(t, ref, n, dtype)
+    a = cnts if cnts is not None else (None, None)
+    assert torch.equal(cross_attention(q, k, v, *a, key_mask=mask), outs[0])            # the inference call
+    for x, y in zip(_run(q, k, v, go, mask, cnts), outs):
+        assert torch.equal(x, y)                                                       # fixed summation orders
+
+
+def test_cross_attention_gradients_equal_differences(dev):
+    """Central differences of the 64-bit formula; truncation h^2 of a third derivative of order 10, the kernel ~1e-5."""
+    case = ([3], [5], 2, 1, 4, False, False)
+    q, k, v, go, mask, cnts = _inputs(case, torch.float32, 1, dev)
+    grads = _run(q, k, v, go, mask, cnts)[1:]
+
+    def value(q, k, v):
+        s = torch.einsum("mhd,nd->hmn", q, k[:, 0]) / 2.0
+        return float((torch.einsum("hmn,nd->mhd", torch.softmax(s, 2), v[:, 0]) * go.double()).sum())
+
+    base = [t.double() for t in (q, k, v)]
+    h = 1e-5
+    for i, g in enumerate(grads):
+        for e in range(0, base[i].numel(), 3):
+            up, down = [t.clone() for t in base], [t.clone() for t in base]
+            up[i].view(-1)[e] += h
+            down[i].view(-1)[e] -= h
+            assert abs(float(g.reshape(-1)[e]) - (value(*up) - value(*down)) / (2 * h)) < 2e-5
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+def test_what_masked_and_trailing_states_hold_does_not_matter(dev, dtype):
+    """NaN, infinities and the type's lowest value in masked states and behind the last frame; trailing queries give zeros."""
+    case = ([40, 21], [90, 133], 4, 2, 48, True, False)
+    q, k, v, go, mask, cnts = _inputs(case, dtype, 3, dev, tail=9)
+    want = _run(q, k, v, go, mask, cnts)
+    k2, v2, q2, go2 = k.clone(), v.clone(), q.clone(), go.clone()
+    dead = torch.nonzero(~mask).flatten()
+    for i, bad in enumerate((float("nan"), float("inf"), -float("inf"), torch.finfo(dtype).min)):
+        k2[dead[i::4]] = bad
+        v2[dead[i::4]] = bad
+    k2[-9:], v2[-9:], q2[-9:] = float("nan"), float("inf"), float("nan")
+    go2[-9:] = float("nan")
+    got = _run(q2, k2, v2, go2, mask, cnts)
+    for w, g in zip(want, got):
+        assert torch.equal(w, g)
+    o, dq, dk, dv = got
+    for t in (o[-9:], dq[-9:], dk[-9:], dv[-9:], dk[dead], dv[dead], o[:40], dq[:40]):
+        assert not bool(t.any())
+    # an unmasked broken state breaks its own frame alone
+    k3 = k.clone()
+    k3[90 + 132, 0] = float("nan")
+    assert bool(mask[90 + 132])
+    o3 = _run(q, k3, v, go, mask, cnts)[0]
+    assert torch.equal(o3[:40], want[0][:40]) and bool(torch.isnan(o3[40:61, :2]).all()) and torch.equal(o3[:, 2:], want[0][:, 2:])
+
+
+def test_large_scores_and_equal_scores(dev):
+    """Scores of +-1e4: the maximum is taken out before the exponential; equal scores give the mean."""
+    from glenet_amd.attention import cross_attention
+    q = torch.zeros(1, 2, 1, 8, device=dev)
+    q[0, 0] = 100.0
+    k = torch.randn(1, 700, 1, 8, device=dev) * 30
+    v = torch.randn(1, 700, 1, 8, device=dev)
+    o = cross_attention(q, k, v, scale=1.0)
+    best = int((k[0, :, 0].double().sum(1)).argmax())
+    assert torch.equal(o[0, 0, 0], v[0, best, 0])
+    assert float((o[0, 1, 0].double() - v[0, :, 0].double().mean(0)).abs().max()) < 700 * U
+    o = cross_attention(q, k, v, scale=0.0)
+    assert float((o[0, 0, 0].double() - v[0, :, 0].double().mean(0)).abs().max()) < 700 * U
+
+
+@pytest.mark.parametrize("size", [1e-6, 1e4])
+def test_fp16_gradients_keep_their_range(dev, size):
+    """fp16 with a loss scale that puts dS far below or at the edge of fp16's range: both inner products carry their own scale."""
+    case = ([70], [900], 2, 1, 64, False, False)
+    q, k, v, go, mask, cnts = _inputs(case, torch.float16, 8, dev)
+    go = (go.double() * size).clamp(-6e4, 6e4).half()
+    outs = _run(q, k, v, go, mask, cnts)
+    ref = _reference(q, k, v, go, mask, case, torch.float16)
+    for t, n in zip(outs, ("o", "dq", "dk", "dv")):
+        _check(t, ref, n, torch.float16)
+
+
+def test_strides(dev):
+    """Views of packed projections, transposed head / row orders, expanded gradients."""
+    g = torch.Generator().manual_seed(5)
+    kv = torch.randn(2, 50, 2, 3, 32, generator=g).to(dev)                # frames, states, k | v, heads, dim
+    qt = torch.randn(2, 6, 20, 32, generator=g).to(dev).transpose(1, 2)   # heads in front of rows
+    k, v = kv[:, :, 0], kv[:, :, 1]
+    go = torch.randn(2, 20, 6, 32, generator=g).to(dev)
+    want = _run(qt.contiguous(), k.contiguous(), v.contiguous(), go, None, None)
+    for w, t in zip(want, _run(qt, k, v, go, None, None)):
+        assert torch.equal(w, t)
+    odd = torch.randn(2, 20, 6, 33, generator=g).to(dev)
+    for w, t in zip(_run(odd[..., 1:].contiguous(), k.contiguous(), v.contiguous(), go, None, None), _run(odd[..., 1:], k, v, go, None, None)):
+        assert torch.equal(w, t)
+    every = qt.permute(0, 1, 3, 2).contiguous().permute(0, 1, 3, 2)      # the head dimension strided
+    assert torch.equal(_run(every, k, v, go, None, None)[0], want[0])
+    one = torch.ones((), device=dev).expand(2, 20, 6, 32)
+    for w, t in zip(_run(qt, k, v, one.contiguous(), None, None), _run(qt, k, v, one, None, None)):
+        assert torch.equal(w, t)
+    cnt = torch.tensor([20, 20], device=dev), torch.tensor([50, 50], device=dev)      # int64 counts, the same frames stacked
+    st = _run(qt.reshape(40, 6, 32), k.reshape(100, 3, 32), v.reshape(100, 3, 32), go.reshape(40, 6, 32), None, cnt)
+    for w, t in zip(want, st):
+        assert torch.equal(w.reshape(t.shape), t)
+
+
+def test_one_side_needs_a_gradient(dev):
+    from glenet_amd.attention import cross_attention
+    case = ([40, 30], [60, 80], 4, 2, 32, False, False)
+    q, k, v, go, mask, cnts = _inputs(case, torch.float32, 3, dev)
+    full = _run(q, k, v, go, mask, cnts)[1:]
+    for i in range(3):
+        ts = [t.detach().clone().requires_grad_(j == i) for j, t in enumerate((q, k, v))]
+        g, = torch.autograd.grad(cross_attention(*ts, *cnts), ts[i], go)
+        assert torch.equal(g, full[i])
+
+
+def test_counts_that_do_not_fit_are_cut(dev):
+    from glenet_amd.attention import cross_attention
+    case = ([10, 20], [30, 40], 2, 1, 16, False, False)
+    q, k, v, go, _, cnts = _inputs(case, torch.float32, 3, dev)
+    want = _run(q, k, v, go, None, cnts)
+    wild = torch.tensor([10, 2 ** 31 - 1], dtype=torch.int32, device=dev), torch.tensor([30, 2 ** 31 - 1], dtype=torch.int32, device=dev)
+    for w, t in zip(want, _run(q, k, v, go, None, wild)):
+        assert torch.equal(w, t)
+    neg = torch.tensor([-5, 10, 20, -1], dtype=torch.int32, device=dev), torch.tensor([-3, 30, 40, 7], dtype=torch.int32, device=dev)
+    for w, t in zip(want, _run(q, k, v, go, None, neg)):
+        assert torch.equal(w, t)
+    none = torch.zeros(0, dtype=torch.int32, device=dev)
+    for t in _run(q, k, v, go, None, (none, none)):
+        assert not bool(t.any())
+    many = torch.ones(200, dtype=torch.int32, device=dev)                # more frames than a wave has lanes
+    q, k, v = torch.randn(200, 2, 16, device=dev), torch.randn(200, 1, 16, device=dev), torch.randn(200, 1, 16, device=dev)
+    o = cross_attention(q, k, v, many, many)
+    assert torch.equal(o, v.expand(200, 2, 16))
+
+
+def test_nothing_on_one_side(dev):
+    for ql, kl in ((0, 5), (5, 0), (0, 0)):
+        q = torch.randn(2, ql, 4, 16, device=dev)
+        k, v = torch.randn(2, kl, 2, 16, device=dev), torch.randn(2, kl, 2, 16, device=dev)
+        for t, like in zip(_run(q, k, v, torch.ones_like(q), None, None), (q, q, k, v)):
+            assert t.shape == like.shape and not bool(t.any())
+    k = torch.randn(0, 3, 2, 16, device=dev)
+    assert _run(torch.randn(0, 3, 4, 16, device=dev), k, k, torch.randn(0, 3, 4, 16, device=dev), None, None)[0].shape == (0, 3, 4, 16)
+
+
+def test_captured_graphs_and_another_stream(dev):
+    """Forward + backward of two sizes in two graphs, replayed in turn with other inputs and counts, beside eager calls."""
+    from glenet_amd import _lib
+    from glenet_amd.attention import cross_attention
+    sets = []
+    for seed, case in enumerate([([20, 60], [700, 900], 4, 2, 64, True, False), ([2, 1], [3000, 2000], 8, 2, 32, False, False)]):
+        q, k, v, go, mask, cnts = _inputs(case, torch.bfloat16, seed, dev)
+        leaves = [t.requires_grad_(True) for t in (q, k, v)]
+
+        def step(leaves=leaves, go=go, mask=mask, cnts=cnts):
+            o = cross_attention(*leaves, *cnts, key_mask=mask)
+            return [o.detach()] + list(torch.autograd.grad(o, leaves, go))
+
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            other = step()
+        torch.cuda.current_stream().wait_stream(side)
+        for x, y in zip(step(), other):
+            assert torch.equal(x, y)
+        graph = _lib.new_graph()
+        with torch.cuda.graph(graph):
+            outs = step()
+        sets.append((graph, step, outs, leaves, go, cnts))
+    for it in range(4):
+        for _, _, _, leaves, go, cnts in sets:
+            with torch.no_grad():
+                for t in leaves + [go]:
+                    t.copy_(torch.randn(t.shape, device=dev))
+                cnts[1][0] -= 13
+        for graph, *_ in sets:
+            graph.replay()
+        torch.cuda.synchronize()
+        for _, step, outs, *_ in sets:
+            for x, y in zip(outs, step()):
+                assert torch.equal(x, y)
+
+
+def test_a_long_sequence_with_offsets_beyond_32_bits(dev):
+    """States whose last rows lie more than 2^31 elements into their buffer: 70 frames' worth of one wide packed tensor."""
+    rows, width = 40000, 56000                                           # 2.24e9 elements of bf16, 4.5 GB
+    big = torch.empty(rows, width, dtype=torch.bfloat16, device=dev)
+    k, v = big[:, :64].view(rows, 1, 64), big[:, 64:128].view(rows, 1, 64)
+    k.copy_(torch.randn(rows, 1, 64, device=dev))
+    v.copy_(torch.randn(rows, 1, 64, device=dev))
+    q = torch.randn(2, 1, 64, dtype=torch.bfloat16, device=dev)
+    go = torch.randn(2, 1, 64, dtype=torch.bfloat16, device=dev)
+    cnts = torch.tensor([1, 1], dtype=torch.int32, device=dev), torch.tensor([39000, 1000], dtype=torch.int32, device=dev)
+    for x, y in zip(_run(q, k, v, go, None, cnts), _run(q, k.contiguous(), v.contiguous(), go, None, cnts)):
+        assert torch.equal(x, y)
+
+
+def test_an_attention_block_trained_with_muon(dev):
+    """The operators as they are used together: tokens normalised, proposals attending to their frame's points, the block's
+    matrices updated with orthogonalised steps.  Every parameter gets the gradient that 64-bit autograd gives."""
+    from glenet_amd.attention import cross_attention
+    from glenet_amd.norm import LayerNorm
+    from glenet_amd.optim import FlatMuon
+    torch.manual_seed(0)
+
+    class Block(torch.nn.Module):
+        def __init__(self, c, heads):
+            super().__init__()
+            self.norm, self.heads = LayerNorm(c), heads
+            self.wq, self.wkv, self.wo = (torch.nn.Linear(c, n * c, bias=False) for n in (1, 2, 1))
+
+        def forward(self, x, states, x_cnt, s_cnt):
+            c = x.shape[1]
+            q = self.wq(self.norm(x)).view(-1, self.heads, c // self.heads)
+            kv = self.wkv(states).view(states.shape[0], 2, self.heads, c // self.heads)
+            return x + self.wo(cross_attention(q, kv[:, 0], kv[:, 1], x_cnt, s_cnt).reshape(-1, c))
+
+    net = Block(64, 4).to(dev)
+    opt = FlatMuon(net.parameters(), lr=1e-3)
+    x, states = torch.randn(24, 64, device=dev), torch.randn(300, 64, device=dev)
+    x_cnt, s_cnt = (torch.tensor(c, dtype=torch.int32, device=dev) for c in ([10, 14], [180, 120]))
+    go = torch.randn(24, 64, device=dev)
+    y = net(x, states, x_cnt, s_cnt)
+    y.backward(go)
+    got = {n: p.grad.clone() for n, p in net.named_parameters()}
+    ref = {n: p.detach().double().requires_grad_(True) for n, p in net.named_parameters()}
+    xd, sd = x.double(), states.double()
+    xn = (xd - xd.mean(1, keepdim=True)) / (xd.var(1, correction=0, keepdim=True) + 1e-5).sqrt() * ref["norm.weight"] + ref["norm.bias"]
+    outs = []
+    for q0, lq, k0, lk in _frames([10, 14], [180, 120]):
+        kv = (sd[k0:k0 + lk] @ ref["wkv.weight"].t()).view(lk, 2, 4, 16)
+        q = (xn[q0:q0 + lq] @ ref["wq.weight"].t()).view(lq, 4, 16)
+        o = [torch.softmax(q[:, j] @ kv[:, 0, j].t() / 4, 1) @ kv[:, 1, j] for j in range(4)]
+        outs.append(torch.cat(o, 1))
+    want = xd + torch.cat(outs) @ ref["wo.weight"].t()
+    # products over 64 and 300 terms behind each other: a few hundred roundings of values of order 1 .. 10
+    assert float((y.double() - want).abs().max()) < 500 * U * 10
+    grads = torch.autograd.grad(want, list(ref.values()), go.double())
+    for (n, g), w in zip(got.items(), grads):
+        assert float((g.double() - w).norm()) < 500 * U * 10 * float(w.norm()), n
+    before = {n: p.detach().clone() for n, p in net.named_parameters()}
+    opt.step()
+    for n, p in net.named_parameters():
+        assert bool(torch.isfinite(p).all()) and not torch.equal(p, before[n])

@@ -68,3 +68,56 @@ def test_orthogonalize_c_entry_refuses():
     assert call(steps=64)[0] == -3
     t = (_Matrix * 1)(_Matrix(64, 64, 6, 6, 4, 6))
     assert lib.glx_orthogonalize_workspace_bytes(t, 1, 0, 5) > 0 and lib.glx_orthogonalize_workspace_bytes(t, 1, 7, 5) == 0
+
+
+def test_cross_attention_refuses():
+    from glenet_amd import _lib
+    from glenet_amd.attention import cross_attention
+    q, k = torch.zeros(2, 5, 4, 16), torch.zeros(2, 7, 2, 16)
+    c = torch.tensor([5, 5], dtype=torch.int32)
+    with pytest.raises(_lib.GlxError, match="no CPU path"):
+        cross_attention(q, k, k)
+    with pytest.raises(_lib.GlxError, match="no CPU path"):
+        cross_attention(q.view(10, 4, 16), k.view(14, 2, 16), k.view(14, 2, 16), c, c)
+    bad = [(q.double(), k.double(), k.double()), (q, k.half(), k), (q, k, k.half()), (q[0], k[0], k[0]), (q, k, k[:, :6]),
+           (q, k[..., :8], k[..., :8]), (q[:1], k, k), (q[:, :, :3], k, k), (torch.zeros(1, 2, 1, 129),) + (torch.zeros(1, 3, 1, 129),) * 2,
+           (torch.zeros(1, 2, 1, 0),) + (torch.zeros(1, 3, 1, 0),) * 2, (q, k[:, :, :0], k[:, :, :0])]
+    for args in bad:
+        with pytest.raises(ValueError):
+            cross_attention(*args)
+    for kw in (dict(key_mask=torch.ones(2, 7)), dict(key_mask=torch.ones(2, 5, dtype=torch.bool)), dict(scale=float("nan")),
+               dict(q_batch_cnt=c), dict(q_batch_cnt=c, k_batch_cnt=c)):
+        with pytest.raises(ValueError):
+            cross_attention(q, k, k, **kw)
+    q3, k3 = q.view(10, 4, 16), k.view(14, 2, 16)
+    for a, b in ((c, None), (None, c), (c, c[:1]), (c.float(), c), (c, c.view(2, 1))):
+        with pytest.raises(ValueError):
+            cross_attention(q3, k3, k3, a, b)
+
+
+def test_attention_c_entry_refuses():
+    import ctypes
+
+    from glenet_amd import _lib
+    from glenet_amd.attention import _Attention
+    lib = _lib.load()
+
+    def call(backward=False, **kw):
+        d = _Attention(q=64, k=64, v=64, out=64, lse=64, q_rows=2000, k_rows=8000, q_len=1000, k_len=4000, q_stride=64, q_head_stride=16,
+                       k_stride=32, k_head_stride=16, v_stride=32, v_head_stride=16, frames=2, heads=4, kv_heads=2, dim=16, dtype=1,
+                       scale=0.25)
+        for n, x in kw.items():
+            setattr(d, n, x)
+        size0, null = ctypes.c_size_t(0), ctypes.c_void_p(0)
+        if backward:
+            p = ctypes.c_void_p(64)
+            return lib.glx_attention_backward(ctypes.byref(d), p, ctypes.c_int64(64), ctypes.c_int64(16), p, p, p, null, size0, null)
+        return lib.glx_attention_forward(ctypes.byref(d), null, size0, null)
+
+    for kw in (dict(dtype=9), dict(dim=129), dict(dim=0), dict(heads=3), dict(kv_heads=0), dict(frames=-1), dict(q_len=999), dict(k_rows=1),
+               dict(q=0), dict(out=0), dict(v=0), dict(q_cnt=64), dict(k_cnt=64), dict(q_rows=1 << 40)):
+        assert call(**kw) == -1 and call(True, **kw) == -1, kw
+    assert call(True, lse=0) == -1
+    assert call(True) == -3                                          # every other check passed
+    assert call(q_rows=2, q_len=1) == -3                             # few rows: split over the keys, a workspace
+    assert lib.glx_attention_forward(None, None, ctypes.c_size_t(0), None) == -1
