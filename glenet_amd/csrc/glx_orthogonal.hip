@@ -21,12 +21,11 @@
 #include <math.h>
 #include <vector>
 
-#define NS_K 32                // k elements of a staged tile
+#define NS_K 64                // the k range of a split comes in multiples of this
 #define NS_OPS 32              // products of one launch (kernel arguments: 120 bytes each)
 #define NS_MATS 36             // matrices of one prologue launch
-#define NS_SMALL 128           // up to here a segment's steps run in one block
 #define NS_STEPS 64            // at most
-#define NS_PARTS 256           // partial sums of squares per matrix, at most
+#define NS_PARTS 1024          // partial sums of squares per matrix, at most
 
 typedef _Float16 nh8 __attribute__((ext_vector_type(8)));
 typedef _Float16 nh4 __attribute__((ext_vector_type(4)));
@@ -77,13 +76,29 @@ __global__ __launch_bounds__(256) void k_ns_norm(NsMats s) {
   while (k + 1 < s.count && (int)blockIdx.x >= s.mat[k + 1].block0) ++k;
   const NsMat& t = s.mat[k];
   const int part = blockIdx.x - t.block0;
-  const long long total = (long long)t.rows * t.cols;
   double sum = 0.0;
-  for (long long e = (long long)part * 256 + threadIdx.x; e < total; e += (long long)t.nparts * 256) {
-    const long long r = e / t.cols;
-    const double v = (double)ns_elem(t.src, r * t.ld + (e - r * t.cols), s.dtype);
-    sum += v * v;
-  }
+  auto add = [&](auto* src) {
+    typedef GlxVec<__remove_cvref(decltype(*src)), 4> V;
+    const bool dense = t.ld == t.cols;
+    const long long runs = dense ? 1 : t.rows, len = dense ? (long long)t.rows * t.cols : t.cols;
+    // one run: the parts stride over it; else over the rows
+    for (long long r = dense ? 0 : part; r < runs; r += dense ? 1 : t.nparts) {
+      const long long first = ((dense ? (long long)part * 256 : 0) + threadIdx.x) * 4, step = (dense ? (long long)t.nparts : 1) * 1024;
+#pragma unroll 4
+      for (long long e = first; e < len; e += step) {
+        if (e + 4 <= len) {
+          const auto v = V::load(src + r * t.ld + e);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) sum += (double)(float)v[i] * (double)(float)v[i];
+        } else {
+          for (long long i = e; i < len; ++i) sum += (double)(float)src[r * t.ld + i] * (double)(float)src[r * t.ld + i];
+        }
+      }
+    }
+  };
+  if (s.dtype == GLX_F32) add((const float*)t.src);
+  else if (s.dtype == GLX_BF16) add((const __bf16*)t.src);
+  else add((const _Float16*)t.src);
   __shared__ double red[256];
   red[threadIdx.x] = sum;
   __syncthreads();
@@ -101,7 +116,9 @@ __global__ __launch_bounds__(256) void k_ns_planes(NsMats s) {
   int k = 0;
   while (k + 1 < s.count && (int)blockIdx.x >= s.mat[k + 1].tblock0) ++k;
   const NsMat& t = s.mat[k];
-  red[threadIdx.x] = (int)threadIdx.x < t.nparts ? t.parts[threadIdx.x] : 0.0;
+  double mine = 0.0;
+  for (int i = threadIdx.x; i < t.nparts; i += 256) mine += t.parts[i];
+  red[threadIdx.x] = mine;
   __syncthreads();
   for (int o = 128; o > 0; o >>= 1) {
     if ((int)threadIdx.x < o) red[threadIdx.x] += red[threadIdx.x + o];
@@ -109,19 +126,22 @@ __global__ __launch_bounds__(256) void k_ns_planes(NsMats s) {
   }
   const int b = blockIdx.x - t.tblock0, tiles_n = t.np / 64;
   const double norm = sqrt(red[0]), rho = norm / (norm + s.eps);
-  auto scale = [&](int st) {                                   // brings min(xb, qb rho) into [2^14, 2^15)
+  // the planes hold G 2^k with |G| 2^k in [2^14, 2^15): 16-bit values exactly, in the hi plane alone
+  const int k0 = norm > 0.0 ? 14 - ilogb(norm) : 60, kx = k0 > 120 ? 120 : (k0 < -120 ? -120 : k0);
+  const float up = ldexpf(1.f, kx);
+  if (b == 0 && (int)threadIdx.x < s.steps) {
+    // X = planes / xscale; later X in front of step st: min(xb, qb rho) 2^e in [2^14, 2^15)
+    const int st = threadIdx.x;
     const float bound = fminf(s.xb[st], (float)(s.qb[st] * rho));
-    int e = bound > 0.f ? 14 - ilogbf(bound) : 60;
-    return ldexpf(1.f, e > 60 ? 60 : e);
-  };
-  const float inv = (float)((double)scale(0) / (norm + s.eps));
-  if (b == 0 && (int)threadIdx.x < s.steps) t.xscale[threadIdx.x] = scale(threadIdx.x);
+    const int e = bound > 0.f ? 14 - ilogbf(bound) : 60;
+    t.xscale[st] = st == 0 ? (float)((double)up * (norm + s.eps)) : ldexpf(1.f, e > 60 ? 60 : e);
+  }
   const int i0 = b / tiles_n * 64, j0 = b % tiles_n * 64;      // of X
   const int c = threadIdx.x & 63;
 #pragma unroll 4
   for (int r = threadIdx.x >> 6; r < 64; r += 4) {
     const int row = t.tall ? j0 + r : i0 + r, col = t.tall ? i0 + c : j0 + c;       // of the caller's matrix
-    const float v = row < t.rows && col < t.cols ? ns_elem(t.src, row * t.ld + col, s.dtype) * inv : 0.f;
+    const float v = row < t.rows && col < t.cols ? ns_elem(t.src, row * t.ld + col, s.dtype) * up : 0.f;
     if (t.tall) tile[c][r] = v; else tile[r][c] = v;
   }
   __syncthreads();
@@ -140,19 +160,24 @@ __global__ __launch_bounds__(256) void k_ns_planes(NsMats s) {
     }
     const long long o = (long long)(i0 + r) * t.np + j0 + c8, ot = (long long)(j0 + r) * t.mp + i0 + c8;
     *reinterpret_cast<nh8*>(t.x + o) = h;
-    *reinterpret_cast<nh8*>(t.x + plane + o) = l;
     *reinterpret_cast<nh8*>(t.xt + ot) = th;
-    *reinterpret_cast<nh8*>(t.xt + plane + ot) = tl;
+    if (s.dtype == GLX_F32) {
+      *reinterpret_cast<nh8*>(t.x + plane + o) = l;
+      *reinterpret_cast<nh8*>(t.xt + plane + ot) = tl;
+    }
   }
 }
 
 // ------------------------------------------------------------------------------------------------ the products
-// A block forms a TILE x TILE tile with four waves of (TILE / 2)^2, k in steps of NS_K through two LDS stages; a staged row is
-// NS_K fp16 = four 16-byte chunks whose order is rotated by the row so that the 32 rows an operand read touches spread over the banks.
-template <int TILE>
+// A block forms a TILE x TILE tile with four waves of (TILE / 2)^2, k in steps of KS through two LDS stages; the order of a
+// staged row's 16-byte chunks is rotated by the row, so that the 32 rows an operand read touches spread over the banks.  PROD
+// products per pair of operands: 3 both split, 2 where B's lo plane is empty, 1 where neither is used.
+template <int TILE, int PROD>
 __global__ __launch_bounds__(256) void k_ns_gemm(NsOps s) {
-  constexpr int W = TILE / 2, F = W / 32, CH = TILE * 4 / 256;       // a wave's tile, its 32-wide parts, chunks per thread and plane
-  __shared__ __attribute__((aligned(16))) char smem[2][2][2][TILE * NS_K * 2];       // stage, operand, plane
+  constexpr int KS = TILE == 64 ? 64 : 32, C = KS / 8, RB = KS * 2;  // k elements of a stage, its chunks and bytes per row
+  constexpr int PA = PROD > 1 ? 2 : 1, PB = PROD > 2 ? 2 : 1;        // planes of the operands
+  constexpr int W = TILE / 2, F = W / 32, CH = TILE * C / 256;       // a wave's tile, its 32-wide parts, chunks per thread and plane
+  __shared__ __attribute__((aligned(16))) char smem[2][PA + PB][TILE * RB];          // stage, plane
   int k = 0;
   while (k + 1 < s.count && (int)blockIdx.x >= s.op[k + 1].block0) ++k;
   const NsOp& t = s.op[k];
@@ -172,30 +197,30 @@ __global__ __launch_bounds__(256) void k_ns_gemm(NsOps s) {
   const float xin = t.xin ? t.xin[0] : 1.f, alpha = t.alpha / (t.xpow == 2 ? xin * xin : xin), scale = t.xout ? t.xout[0] : t.scale;
   const int k0 = split * t.kper, k1 = k0 + t.kper < t.K ? k0 + t.kper : t.K;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wi = wave >> 1, wj = wave & 1, half = lane >> 5, l32 = lane & 31;
-  const _Float16* src[2] = {t.a + (long long)ti * TILE * t.K, t.b + (long long)tj * TILE * t.K};
-  const long long plane[2] = {(long long)t.mp * t.K, (long long)t.np * t.K};
-  nh8 stage[2][2][CH];
+  const _Float16* src[PA + PB];
+#pragma unroll
+  for (int p = 0; p < PA; ++p) src[p] = t.a + ((long long)p * t.mp + ti * TILE) * t.K;
+#pragma unroll
+  for (int p = 0; p < PB; ++p) src[PA + p] = t.b + ((long long)p * t.np + tj * TILE) * t.K;
+  nh8 stage[PA + PB][CH];
+  auto place = [](int r, int ch) { return r * RB + (C == 8 ? (ch ^ r) & 7 : (ch ^ (r >> 1)) & 3) * 16; };
   auto fetch = [&](int kk) {
 #pragma unroll
-    for (int o = 0; o < 2; ++o)
+    for (int p = 0; p < PA + PB; ++p)
 #pragma unroll
-      for (int p = 0; p < 2; ++p)
-#pragma unroll
-        for (int c = 0; c < CH; ++c) {
-          const int q = threadIdx.x + c * 256, r = q >> 2, ch = q & 3;
-          stage[o][p][c] = *reinterpret_cast<const nh8*>(src[o] + p * plane[o] + (long long)r * t.K + kk + ch * 8);
-        }
+      for (int c = 0; c < CH; ++c) {
+        const int q = threadIdx.x + c * 256;
+        stage[p][c] = *reinterpret_cast<const nh8*>(src[p] + (long long)(q / C) * t.K + kk + (q % C) * 8);
+      }
   };
   auto put = [&](int buf) {
 #pragma unroll
-    for (int o = 0; o < 2; ++o)
+    for (int p = 0; p < PA + PB; ++p)
 #pragma unroll
-      for (int p = 0; p < 2; ++p)
-#pragma unroll
-        for (int c = 0; c < CH; ++c) {
-          const int q = threadIdx.x + c * 256, r = q >> 2, ch = q & 3;
-          *reinterpret_cast<nh8*>(&smem[buf][o][p][r * 64 + ((ch ^ (r >> 1)) & 3) * 16]) = stage[o][p][c];
-        }
+      for (int c = 0; c < CH; ++c) {
+        const int q = threadIdx.x + c * 256;
+        *reinterpret_cast<nh8*>(&smem[buf][p][place(q / C, q % C)]) = stage[p][c];
+      }
   };
   nf16 acc[F][F];
 #pragma unroll
@@ -205,26 +230,26 @@ __global__ __launch_bounds__(256) void k_ns_gemm(NsOps s) {
   if (k0 < k1) { fetch(k0); put(0); }
   __syncthreads();
   int buf = 0;
-  for (int kk = k0; kk < k1; kk += NS_K) {
-    const bool more = kk + NS_K < k1;
-    if (more) fetch(kk + NS_K);
+  for (int kk = k0; kk < k1; kk += KS) {
+    const bool more = kk + KS < k1;
+    if (more) fetch(kk + KS);
 #pragma unroll
-    for (int ks = 0; ks < NS_K / 16; ++ks) {
-      nh8 fa[2][F], fb[2][F];
+    for (int ks = 0; ks < KS / 16; ++ks) {
+      nh8 fa[PA][F], fb[PB][F];
+      const int ch = ks * 2 + half;
 #pragma unroll
-      for (int p = 0; p < 2; ++p)
+      for (int f = 0; f < F; ++f) {
 #pragma unroll
-        for (int f = 0; f < F; ++f) {
-          const int ra = wi * W + f * 32 + l32, rb = wj * W + f * 32 + l32, ch = ks * 2 + half;
-          fa[p][f] = *reinterpret_cast<const nh8*>(&smem[buf][0][p][ra * 64 + ((ch ^ (ra >> 1)) & 3) * 16]);
-          fb[p][f] = *reinterpret_cast<const nh8*>(&smem[buf][1][p][rb * 64 + ((ch ^ (rb >> 1)) & 3) * 16]);
-        }
+        for (int p = 0; p < PA; ++p) fa[p][f] = *reinterpret_cast<const nh8*>(&smem[buf][p][place(wi * W + f * 32 + l32, ch)]);
+#pragma unroll
+        for (int p = 0; p < PB; ++p) fb[p][f] = *reinterpret_cast<const nh8*>(&smem[buf][PA + p][place(wj * W + f * 32 + l32, ch)]);
+      }
 #pragma unroll
       for (int i = 0; i < F; ++i)
 #pragma unroll
         for (int j = 0; j < F; ++j) {
-          acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fa[1][i], fb[0][j], acc[i][j], 0, 0, 0);
-          acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fa[0][i], fb[1][j], acc[i][j], 0, 0, 0);
+          if (PROD > 1) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fa[PA - 1][i], fb[0][j], acc[i][j], 0, 0, 0);
+          if (PROD > 2) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fa[0][i], fb[PB - 1][j], acc[i][j], 0, 0, 0);
           acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fa[0][i], fb[0][j], acc[i][j], 0, 0, 0);
         }
     }
@@ -305,122 +330,9 @@ __global__ __launch_bounds__(256) void k_ns_join(NsOps s, int tile) {
   ((_Float16*)t.out)[plane + e] = w;
 }
 
-// ------------------------------------------------------------------------------------------------ a segment of a small matrix
-// One block per matrix of up to 32 MT rows: wave w owns the columns 32 w .. 32 w + 31 of A, H and Q in registers, in the layout
-// the MFMA leaves them in, which is also a B operand whose k order is permuted (the A operand is read in that order from LDS).
-// Every product is [matrix in LDS] x [own columns]: A A, A P, P (A P), P Q -- only A and P ever pass through LDS.  (P (A P), not
-// P (P A): errors between directions of small and large singular values grow by p_small p_large a step, not by p_small^2.)
-struct NsSmall { const _Float16* g; _Float16* q; int mp; };
-struct NsSmalls { NsSmall m[NS_MATS]; int count, steps; float a, b, c; float gs[8], ps[8], hs[8], qs[8]; };     // scales by step
-
-template <int MT>
-__device__ __forceinline__ void ns_panel(const char* lds, const nf16 (&own)[MT], float scale, float alpha, nf16 (&out)[MT]) {
-  constexpr int LD = MT * 64 + 16, PL = MT * 32 * LD;
-  const int lane = threadIdx.x & 63, half = lane >> 5, l32 = lane & 31;
-#pragma unroll
-  for (int i = 0; i < MT; ++i) out[i] = (nf16)(0.f);
-#pragma unroll
-  for (int kt = 0; kt < MT; ++kt)
-#pragma unroll
-    for (int ks = 0; ks < 2; ++ks) {
-      nh8 bh, bl;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        _Float16 u, w;
-        ns_split(own[kt][ks * 8 + e] * scale, u, w);
-        bh[e] = u; bl[e] = w;
-      }
-#pragma unroll
-      for (int i = 0; i < MT; ++i) {
-        const char* p = lds + (i * 32 + l32) * LD + (kt * 32 + ks * 16 + half * 4) * 2;
-        const nh4 h0 = *reinterpret_cast<const nh4*>(p), h1 = *reinterpret_cast<const nh4*>(p + 16);
-        const nh4 l0 = *reinterpret_cast<const nh4*>(p + PL), l1 = *reinterpret_cast<const nh4*>(p + PL + 16);
-        const nh8 ah = {h0[0], h0[1], h0[2], h0[3], h1[0], h1[1], h1[2], h1[3]};
-        const nh8 al = {l0[0], l0[1], l0[2], l0[3], l1[0], l1[1], l1[2], l1[3]};
-        out[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(al, bh, out[i], 0, 0, 0);
-        out[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ah, bl, out[i], 0, 0, 0);
-        out[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ah, bh, out[i], 0, 0, 0);
-      }
-    }
-#pragma unroll
-  for (int i = 0; i < MT; ++i)
-#pragma unroll
-    for (int e = 0; e < 16; ++e) out[i][e] *= alpha;
-}
-// own columns -> the planes in LDS (or global memory), row = own column (the matrices are symmetric)
-template <int MT>
-__device__ __forceinline__ void ns_panel_put(char* dst, int ld, long long plane, const nf16 (&own)[MT], float scale) {
-  const int lane = threadIdx.x & 63, half = lane >> 5, col = (threadIdx.x >> 6) * 32 + (lane & 31);
-#pragma unroll
-  for (int i = 0; i < MT; ++i)
-#pragma unroll
-    for (int g = 0; g < 4; ++g) {
-      nh4 h, l;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        _Float16 u, w;
-        ns_split(own[i][g * 4 + e] * scale, u, w);
-        h[e] = u; l[e] = w;
-      }
-      char* p = dst + (long long)col * ld + (i * 32 + g * 8 + half * 4) * 2;
-      *reinterpret_cast<nh4*>(p) = h;
-      *reinterpret_cast<nh4*>(p + plane) = l;
-    }
-}
-
-template <int MT>
-__global__ __launch_bounds__(MT * 64) void k_ns_small(NsSmalls s) {
-  constexpr int LD = MT * 64 + 16, PL = MT * 32 * LD, MP = MT * 32;
-  __shared__ __attribute__((aligned(16))) char lds[2 * PL];
-  const NsSmall& t = s.m[blockIdx.x];
-  const int lane = threadIdx.x & 63, half = lane >> 5, col = (threadIdx.x >> 6) * 32 + (lane & 31);
-  nf16 G[MT], P[MT], Q[MT], H[MT];
-  const float unscale = 1.f / s.gs[0];
-#pragma unroll
-  for (int i = 0; i < MT; ++i)
-#pragma unroll
-    for (int g = 0; g < 4; ++g) {
-      const _Float16* p = t.g + (long long)col * MP + i * 32 + g * 8 + half * 4;
-      const nh4 h = *reinterpret_cast<const nh4*>(p), l = *reinterpret_cast<const nh4*>(p + MP * MP);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) G[i][g * 4 + e] = ((float)h[e] + (float)l[e]) * unscale;
-    }
-  for (int st = 0; st < s.steps; ++st) {
-    const float gs = s.gs[st], ps = s.ps[st];
-    ns_panel_put<MT>(lds, LD, PL, G, gs);
-    __syncthreads();
-    ns_panel<MT>(lds, G, gs, 1.f / (gs * gs), P);
-#pragma unroll
-    for (int i = 0; i < MT; ++i)
-#pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        P[i][e] = s.b * G[i][e] + s.c * P[i][e];
-        if (i * 32 + (e >> 2) * 8 + half * 4 + (e & 3) == col) P[i][e] += s.a;
-      }
-    if (st + 1 < s.steps) ns_panel<MT>(lds, P, ps, 1.f / (gs * ps), H);
-    __syncthreads();
-    ns_panel_put<MT>(lds, LD, PL, P, ps);
-    __syncthreads();
-    if (st == 0) {
-#pragma unroll
-      for (int i = 0; i < MT; ++i) Q[i] = P[i];
-    } else {
-      ns_panel<MT>(lds, Q, s.qs[st - 1], 1.f / (s.qs[st - 1] * ps), P);
-#pragma unroll
-      for (int i = 0; i < MT; ++i) Q[i] = P[i];
-    }
-    if (st + 1 < s.steps) {
-      ns_panel<MT>(lds, H, s.hs[st], 1.f / (s.hs[st] * ps), G);
-      __syncthreads();
-    }
-  }
-  ns_panel_put<MT>((char*)t.q, MP * 2, (long long)MP * MP * 2, Q, s.qs[s.steps - 1]);
-}
-
 // ------------------------------------------------------------------------------------------------ host: programs
 struct NsPlan {                // one matrix
   int rows, cols, m, n, mp, np, tile, tall, seg, splits, kper, nparts;
-  bool small;
   size_t x, xt, x2, xt2, g, h, p[2], q[2], part, parts, xscale;        // byte offsets in the workspace
 };
 struct NsBounds { double g, p, h, q; };       // of one step of a segment: spectral norms of A, P, H = P A and Q behind the step
@@ -453,22 +365,21 @@ static NsPlan ns_plan(int rows, int cols, int dtype, int steps, size_t& at) {
   NsPlan p = {};
   p.rows = rows; p.cols = cols; p.tall = rows > cols;
   p.m = p.tall ? cols : rows; p.n = p.tall ? rows : cols;
-  p.small = p.m <= NS_SMALL;
   // 128-wide tiles once the symmetric products fill the card with them
   p.tile = p.m > 2048 ? 128 : 64;
   p.mp = ns_padded(p.m, p.tile); p.np = ns_padded(p.n, p.tile);
   p.seg = dtype == GLX_BF16 ? 5 : 3;
-  if (!p.small && 4ll * p.n <= 5ll * p.m) p.seg = 1;
+  if (p.m <= 128 || (dtype == GLX_F32 ? p.n < 4ll * p.m : 4ll * p.n <= 5ll * p.m)) p.seg = 1;
   if (p.seg > steps) p.seg = steps;
   const int t = p.mp / p.tile;
   const long long tiles = (long long)t * (t + 1) / 2, ksteps = p.np / NS_K;
   long long splits = 512 / tiles;                       // two blocks per compute unit
-  if (splits > ksteps / 4) splits = ksteps / 4;         // 128 k elements a split, at least
+  if (splits > ksteps / 8) splits = ksteps / 8;         // 512 k elements a split, at least: a join costs as much as those
   if (splits < 1) splits = 1;
   p.kper = (int)((ksteps + splits - 1) / splits) * NS_K;
   p.splits = (int)((p.np + p.kper - 1) / p.kper);
   const long long total = (long long)p.m * p.n;
-  p.nparts = (int)((total + 16383) / 16384);
+  p.nparts = (int)((total + 4095) / 4096);
   if (p.nparts > NS_PARTS) p.nparts = NS_PARTS;
   const size_t X = glx_align((size_t)p.mp * p.np * 4), S = glx_align((size_t)p.mp * p.mp * 4);
   auto take = [&](size_t bytes) { const size_t o = at; at += glx_align(bytes); return o; };
@@ -499,12 +410,17 @@ extern "C" size_t glx_orthogonalize_workspace_bytes(const glx_matrix* mats, int 
 }
 
 struct NsStage {               // what one launch round does, over all matrices
-  std::vector<NsOp> gemm[2], join[2];
-  std::vector<NsSmall> small[2];
-  int steps = 0, first = 0;    // of the small ones
+  std::vector<NsOp> gemm[2][3], join[2];       // by tile; by the products per pair of operands
+  void add(int tile, int prods, const NsOp& o) { gemm[tile == 128][prods - 1].push_back(o); }
 };
 
-static void ns_launch_ops(std::vector<NsOp>& ops, int tile, bool join, hipStream_t st) {
+template <int TILE>
+static void ns_launch_gemm(const NsOps& s, int blocks, int prods, hipStream_t st) {
+  if (prods == 1) hipLaunchKernelGGL((k_ns_gemm<TILE, 1>), dim3(blocks), dim3(256), 0, st, s);
+  else if (prods == 2) hipLaunchKernelGGL((k_ns_gemm<TILE, 2>), dim3(blocks), dim3(256), 0, st, s);
+  else hipLaunchKernelGGL((k_ns_gemm<TILE, 3>), dim3(blocks), dim3(256), 0, st, s);
+}
+static void ns_launch_ops(std::vector<NsOp>& ops, int tile, int prods, hipStream_t st) {       // prods = 0: joins
   for (size_t i = 0; i < ops.size(); i += NS_OPS) {
     NsOps s;
     memset(&s, 0, sizeof(s));
@@ -513,11 +429,11 @@ static void ns_launch_ops(std::vector<NsOp>& ops, int tile, bool join, hipStream
       NsOp& o = s.op[s.count++] = ops[j];
       o.block0 = blocks;
       const int tm = o.mp / tile, tn = o.np / tile;
-      blocks += join ? glx_divup((long long)o.mp * o.mp, 256) : (o.sym ? tm * (tm + 1) / 2 : tm * tn) * o.splits;
+      blocks += prods == 0 ? glx_divup((long long)o.mp * o.mp, 256) : (o.sym ? tm * (tm + 1) / 2 : tm * tn) * o.splits;
     }
-    if (join) hipLaunchKernelGGL(k_ns_join, dim3(blocks), dim3(256), 0, st, s, tile);
-    else if (tile == 128) hipLaunchKernelGGL((k_ns_gemm<128>), dim3(blocks), dim3(256), 0, st, s);
-    else hipLaunchKernelGGL((k_ns_gemm<64>), dim3(blocks), dim3(256), 0, st, s);
+    if (prods == 0) hipLaunchKernelGGL(k_ns_join, dim3(blocks), dim3(256), 0, st, s, tile);
+    else if (tile == 128) ns_launch_gemm<128>(s, blocks, prods, st);
+    else ns_launch_gemm<64>(s, blocks, prods, st);
   }
 }
 
@@ -572,7 +488,9 @@ extern "C" int glx_orthogonalize(const glx_matrix* mats, int count, int dtype, i
   std::vector<NsStage> stages;
   for (int i = 0; i < count; ++i) {
     const NsPlan& p = plans[i];
-    const int kind = p.tile == 128;
+    // bfloat16: single products in the last two steps, where what they lose is no longer amplified (it comes to 1e-3 of the
+    // result, half a step is 4e-3); segments of one step only
+    auto last = [&](int s1) { return dtype == GLX_BF16 && p.seg == 1 && s1 > steps - 2 && steps >= 4; };
     size_t k = 0;
     auto stage = [&]() -> NsStage& {
       if (k == stages.size()) stages.emplace_back();
@@ -596,52 +514,42 @@ extern "C" int glx_orthogonalize(const glx_matrix* mats, int count, int dtype, i
         o.a = o.b = planes(x);
         o.alpha = 1.f; o.scale = gs; o.xin = xs; o.xpow = 2;
         o.mp = o.np = p.mp; o.K = p.np; o.kper = p.kper; o.splits = (short)p.splits; o.sym = 1;
+        const int prods = last(s1) || (s0 == 0 && dtype != GLX_F32) ? 1 : 3;
         if (p.splits > 1) {
           o.kind = NS_PARTIAL; o.out = ws + p.part;
-          stage().gemm[kind].push_back(o);
+          stage().add(p.tile, prods, o);
           NsOp j = {};
           j.a = planes(p.part); j.out = planes(p.g); j.scale = gs; j.mp = j.np = p.mp; j.splits = (short)p.splits;
-          stage().join[kind].push_back(j);
+          stage().join[p.tile == 128].push_back(j);
         } else {
           o.kind = NS_PLANES; o.out = planes(p.g);
-          stage().gemm[kind].push_back(o);
-          stage();                                     // (every matrix keeps a place for the join: small ones meet in one launch)
+          stage().add(p.tile, prods, o);
         }
       }
       size_t q = p.q[0];
       float qs = 0.f;
-      if (p.small) {
-        NsStage& g = stage();
-        NsSmall m = {planes(p.g), planes(q), p.mp};
-        g.small[p.mp == 128].push_back(m);
-        g.steps = s1 - s0; g.first = s0;
-        qs = ns_scale(qbound(s0, s1 - 1));
-      } else {
-        for (int s = s0; s < s1; ++s) {
-          const float ps = ns_scale(pmax[s]), hs = ns_scale(hmax[s]);
-          const size_t P = p.p[(s - s0) & 1];
-          NsOp o = square(p.g, gs, p.g, gs, P, ps);    // P = a I + b A + c A A
-          o.alpha *= c; o.d = planes(p.g); o.beta = b / gs; o.diag = a;
-          stage().gemm[kind].push_back(o);
-          if (s == s0) {
-            q = P; qs = ps;
-          } else {                                     // (beside H where a step follows)
-            const float nqs = ns_scale(qbound(s0, s));
-            const size_t nq = p.q[(s - s0) & 1];
-            NsOp oq = square(P, ps, q, qs, nq, nqs);
-            NsStage& g = stage();
-            g.gemm[kind].push_back(oq);
-            q = nq; qs = nqs;
-            --k;
-          }
-          if (s + 1 < s1) {
-            stage().gemm[kind].push_back(square(P, ps, p.g, gs, p.h, hs));
-            const float ngs = ns_scale(lam[s + 1]);
-            stage().gemm[kind].push_back(square(p.h, hs, P, ps, p.g, ngs));
-            gs = ngs;
-          } else if (s > s0) {
-            ++k;
-          }
+      for (int s = s0; s < s1; ++s) {
+        const float ps = ns_scale(pmax[s]), hs = ns_scale(hmax[s]);
+        const size_t P = p.p[(s - s0) & 1];
+        NsOp o = square(p.g, gs, p.g, gs, P, ps);      // P = a I + b A + c A A
+        o.alpha *= c; o.d = planes(p.g); o.beta = b / gs; o.diag = a;
+        stage().add(p.tile, last(s1) ? 1 : 3, o);
+        if (s == s0) {
+          q = P; qs = ps;
+        } else {                                       // (beside H where a step follows)
+          const float nqs = ns_scale(qbound(s0, s));
+          const size_t nq = p.q[(s - s0) & 1];
+          stage().add(p.tile, 3, square(P, ps, q, qs, nq, nqs));
+          q = nq; qs = nqs;
+          --k;
+        }
+        if (s + 1 < s1) {
+          stage().add(p.tile, 3, square(P, ps, p.g, gs, p.h, hs));
+          const float ngs = ns_scale(lam[s + 1]);
+          stage().add(p.tile, 3, square(p.h, hs, P, ps, p.g, ngs));
+          gs = ngs;
+        } else if (s > s0) {
+          ++k;
         }
       }
       {                                                // X <- Q X
@@ -655,7 +563,7 @@ extern "C" int glx_orthogonalize(const glx_matrix* mats, int count, int dtype, i
         } else {
           o.kind = NS_XPLANES; o.out = planes(x2); o.out2 = planes(xt2); o.xout = (const float*)(ws + p.xscale) + s1;
         }
-        stage().gemm[kind].push_back(o);
+        stage().add(p.tile, last(s1) ? 1 : s0 == 0 && dtype != GLX_F32 ? 2 : 3, o);
         size_t y = x; x = x2; x2 = y;
         y = xt; xt = xt2; xt2 = y;
       }
@@ -663,20 +571,8 @@ extern "C" int glx_orthogonalize(const glx_matrix* mats, int count, int dtype, i
   }
   for (auto& g : stages) {
     for (int t = 0; t < 2; ++t) {
-      ns_launch_ops(g.gemm[t], t ? 128 : 64, false, st);
-      ns_launch_ops(g.join[t], t ? 128 : 64, true, st);
-      for (size_t i = 0; i < g.small[t].size(); i += NS_MATS) {
-        NsSmalls s;
-        memset(&s, 0, sizeof(s));
-        for (size_t j = i; j < g.small[t].size() && j < i + NS_MATS; ++j) s.m[s.count++] = g.small[t][j];
-        s.steps = g.steps; s.a = a; s.b = b; s.c = c;
-        for (int k = 0; k < g.steps; ++k) {
-          s.gs[k] = ns_scale(lam[g.first + k]); s.ps[k] = ns_scale(pmax[g.first + k]); s.hs[k] = ns_scale(hmax[g.first + k]);
-          s.qs[k] = ns_scale(qbound(g.first, g.first + k));
-        }
-        if (t) hipLaunchKernelGGL((k_ns_small<4>), dim3(s.count), dim3(256), 0, st, s);
-        else hipLaunchKernelGGL((k_ns_small<2>), dim3(s.count), dim3(128), 0, st, s);
-      }
+      for (int n = 0; n < 3; ++n) ns_launch_ops(g.gemm[t][n], t ? 128 : 64, n + 1, st);
+      ns_launch_ops(g.join[t], t ? 128 : 64, 0, st);
     }
   }
   GLX_LAUNCH_CHECK();
