@@ -12,7 +12,10 @@ _HERE = os.path.dirname(os.path.abspath(__file__))
 # GLX_HIP_LIB: another build of the same sources (tools/build_variant.sh: kernel experiments A/B'd on one box)
 LIB_PATH = os.environ.get("GLX_HIP_LIB") or os.path.join(_HERE, "csrc", "libglenet_hip.so")
 
+TORCH_LIB_PATH = os.path.join(_HERE, "csrc", "libglenet_torch.so")
+
 _lib = None
+_torch_ops = None
 
 c_void_p, c_int, c_float, c_size_t, c_int64 = (
     ctypes.c_void_p, ctypes.c_int, ctypes.c_float, ctypes.c_size_t, ctypes.c_int64)
@@ -54,6 +57,23 @@ def load():
     lib.glx_index_words.restype = c_int64
     _lib = lib
     return lib
+
+
+def torch_ops():
+    """torch.ops.glenet: the differentiable operators' bindings (csrc/host/glx_torch.cpp) on this process' HIP library."""
+    global _torch_ops
+    if _torch_ops is None:
+        lib = load()
+        if not os.path.exists(TORCH_LIB_PATH):
+            raise GlxError("libglenet_torch.so not found at %s -- run `python -c 'import __graft_entry__ as g; g.build()'`"
+                           % TORCH_LIB_PATH)
+        torch.ops.load_library(TORCH_LIB_PATH)
+        names = ("glx_last_error", "glx_layer_norm_forward", "glx_layer_norm_workspace_bytes", "glx_layer_norm_backward",
+                 "glx_attention_workspace_bytes", "glx_attention_forward", "glx_attention_backward_workspace_bytes",
+                 "glx_attention_backward")
+        torch.ops.glenet.bind([ctypes.cast(getattr(lib, n), c_void_p).value for n in names])
+        _torch_ops = torch.ops.glenet
+    return _torch_ops
 
 
 def _arg(a):

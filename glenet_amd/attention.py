@@ -1,91 +1,15 @@
-"""Cross attention of stacked frames (csrc/glx_attention.hip, csrc/glx_attention_bwd.hip), beside the operators of
+"""Cross attention of stacked frames (csrc/glx_attention.hip, csrc/glx_attention_bwd.hip, bound in
+csrc/host/glx_torch.cpp), beside the operators of
 pcdet_ops.pointnet2.pointnet2_stack that gather a frame's points at query points: here every query weighs ALL of its frame's
 encoder states (points, voxels, RoI grid points; another number of them per frame) by softmax(scale q k^T).
 
 Two layouts.  Stacked, as (N1 + N2 + .., H, D) with int32 counts per frame on the device (no read-back: the call can be
 recorded), or a padded batch (B, L, H, D).  key_mask says which encoder states take part; masked ones are never read."""
-import ctypes
 import math
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import _lib
-
-
-class _Attention(ctypes.Structure):        # glx_attention
-    _fields_ = ([(n, ctypes.c_void_p) for n in ("q", "k", "v", "out", "lse", "key_mask", "q_cnt", "k_cnt")]
-                + [(n, ctypes.c_int64) for n in ("q_rows", "k_rows", "q_len", "k_len", "q_stride", "q_head_stride", "k_stride",
-                                                 "k_head_stride", "v_stride", "v_head_stride")]
-                + [(n, ctypes.c_int32) for n in ("frames", "heads", "kv_heads", "dim", "dtype")] + [("scale", ctypes.c_float)])
-
-
-def _stack(t):
-    """(.., rows, heads, dim) as stacked rows with unit stride inside a head -> (tensor, row stride, head stride)."""
-    if t.dim() == 4:
-        b, n = t.shape[:2]
-        if b > 1 and n > 0 and t.stride(0) != n * t.stride(1):
-            t = t.contiguous()
-        row = t.stride(1) if n != 1 else t.stride(0)       # one row per frame: the frames' stride is the rows'
-    else:
-        row = t.stride(0)
-    if t.shape[-1] > 1 and t.stride(-1) != 1:
-        t = t.contiguous()
-        row = t.shape[-2] * t.shape[-1]
-    return t, row, t.stride(-2)
-
-
-def _ptr(t):
-    return t.data_ptr() if t is not None else None
-
-
-def _descriptor(q, k, v, q_cnt, k_cnt, key_mask, scale, out, lse):
-    d = _Attention()
-    d.q, d.k, d.v, d.out, d.lse, d.key_mask, d.q_cnt, d.k_cnt = (_ptr(t) for t in (q[0], k[0], v[0], out, lse, key_mask, q_cnt, k_cnt))
-    heads, dim = q[0].shape[-2:]
-    d.q_rows, d.k_rows = q[0].numel() // (heads * dim), k[0].numel() // (k[0].shape[-2] * dim)
-    if q_cnt is None:
-        d.frames, d.q_len, d.k_len = q[0].shape[0], q[0].shape[1], k[0].shape[1]
-    else:
-        d.frames = q_cnt.shape[0]
-    _, d.q_stride, d.q_head_stride = q
-    _, d.k_stride, d.k_head_stride = k
-    _, d.v_stride, d.v_head_stride = v
-    d.heads, d.kv_heads, d.dim, d.dtype, d.scale = heads, k[0].shape[-2], dim, _lib.dtype_code(q[0].dtype), scale
-    return d
-
-
-class _CrossAttention(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, q, k, v, q_cnt, k_cnt, key_mask, scale):
-        dev = q.device
-        out = torch.empty(q.shape, dtype=q.dtype, device=dev)
-        keep = any(ctx.needs_input_grad)
-        lse = torch.empty(q.shape[:-1], dtype=torch.float32, device=dev) if keep else None
-        d = _descriptor(_stack(q), _stack(k), _stack(v), q_cnt, k_cnt, key_mask, scale, out, lse)
-        n = _lib.query("glx_attention_workspace_bytes", ctypes.byref(d))
-        ws = torch.empty(n, dtype=torch.uint8, device=dev) if n > 256 else None
-        _lib.call_on(dev, "glx_attention_forward", ctypes.byref(d), ws, _lib.size_arg(n))
-        if keep:
-            ctx.save_for_backward(q, k, v, q_cnt, k_cnt, key_mask, out, lse)
-            ctx.scale = scale
-        return out
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, go):
-        q, k, v, q_cnt, k_cnt, key_mask, out, lse = ctx.saved_tensors
-        dev = q.device
-        dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=dev) if need else None
-                      for t, need in zip((q, k, v), ctx.needs_input_grad))
-        g, gs, gh = _stack(go)
-        sq, sk, sv = _stack(q), _stack(k), _stack(v)
-        d = _descriptor(sq, sk, sv, q_cnt, k_cnt, key_mask, ctx.scale, out, lse)
-        n = _lib.query("glx_attention_backward_workspace_bytes", ctypes.byref(d))
-        ws = torch.empty(n, dtype=torch.uint8, device=dev)
-        _lib.call_on(dev, "glx_attention_backward", ctypes.byref(d), g, ctypes.c_int64(gs), ctypes.c_int64(gh), dq, dk, dv, ws,
-                     _lib.size_arg(n))
-        return dq, dk, dv, None, None, None, None
 
 
 def cross_attention(q, k, v, q_batch_cnt=None, k_batch_cnt=None, key_mask=None, scale=None):
@@ -129,4 +53,4 @@ def cross_attention(q, k, v, q_batch_cnt=None, k_batch_cnt=None, key_mask=None, 
     _lib.check_device(who, q, k, v, q_batch_cnt, k_batch_cnt, key_mask)
     if q.numel() // dim >= 1 << 31 or k.numel() // dim >= 1 << 31:
         raise ValueError("%s: more than 2^31 rows x heads" % who)
-    return _CrossAttention.apply(q, k, v, q_batch_cnt, k_batch_cnt, key_mask, scale)
+    return _lib.torch_ops().cross_attention.default(q, k, v, q_batch_cnt, k_batch_cnt, key_mask, scale)

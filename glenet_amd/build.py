@@ -35,6 +35,26 @@ def build_host(force=False):
     return HOST_LIB
 
 
+TORCH_SRC = os.path.join(CSRC, "host", "glx_torch.cpp")
+TORCH_LIB = os.path.join(CSRC, "libglenet_torch.so")
+
+
+def build_torch(force=False):
+    """libglenet_torch.so: torch bindings of the differentiable operators (host code, g++)."""
+    hdr = os.path.join(HERE, "..", "include", "glenet_hip.h")
+    if force or _stale(TORCH_LIB, [TORCH_SRC, hdr]):
+        import importlib.util
+        root = os.path.dirname(importlib.util.find_spec("torch").origin)
+        rocm = os.path.dirname(os.path.dirname(HIPCC))
+        r = subprocess.run([os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", "-D__HIP_PLATFORM_AMD__", "-DUSE_ROCM",
+                            "-I" + os.path.join(root, "include"), "-I" + os.path.join(root, "include", "torch", "csrc", "api", "include"),
+                            "-I" + os.path.join(rocm, "include"), "-o", TORCH_LIB, TORCH_SRC, "-L" + os.path.join(root, "lib"),
+                            "-lc10", "-ltorch_cpu", "-lc10_hip", "-ltorch_hip"], capture_output=True, text=True)
+        if r.returncode != 0:
+            raise RuntimeError("g++ failed on glx_torch.cpp:\n%s\n%s" % (r.stdout, r.stderr))
+    return TORCH_LIB
+
+
 def sources():
     return sorted(f for f in os.listdir(CSRC) if f.endswith(".hip"))
 
@@ -66,9 +86,10 @@ def build(force=False, verbose=False):
         if verbose and r.stderr.strip():
             print(r.stderr, file=sys.stderr)
 
-    if jobs:
-        with ThreadPoolExecutor(max_workers=min(len(jobs), 6)) as ex:
-            list(ex.map(run, jobs))
+    with ThreadPoolExecutor(max_workers=7) as ex:
+        torch_lib = ex.submit(build_torch, force)
+        list(ex.map(run, jobs))
+        torch_lib.result()
     if jobs or force or _stale(LIB, objs):
         run([HIPCC, "--offload-arch=gfx950", "-shared", "-fPIC", "-o", LIB] + objs)
     build_host(force)

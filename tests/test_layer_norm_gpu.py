@@ -213,3 +213,17 @@ def test_layer_norm_module(dev):
     assert float((y.detach().mean(-1)).abs().max()) < 1e-5
     with pytest.raises(ValueError):
         m(torch.randn(4, 47, device=dev))
+
+
+def test_gradients_are_not_differentiated_again(dev):
+    """Asking for a second derivative says so; a first one under create_graph is what it was."""
+    from glenet_amd.attention import cross_attention
+    from glenet_amd.norm import layer_norm
+    x = torch.randn(5, 1, 24, device=dev, requires_grad=True)
+    cnt = torch.tensor([5], dtype=torch.int32, device=dev)
+    for f in (lambda: layer_norm(x), lambda: cross_attention(x, x, x, cnt, cnt)):
+        want, = torch.autograd.grad(f().square().sum(), x)
+        got, = torch.autograd.grad(f().square().sum(), x, create_graph=True)
+        assert torch.equal(want, got)
+        with pytest.raises(RuntimeError, match="once"):
+            torch.autograd.grad(got.sum(), x)

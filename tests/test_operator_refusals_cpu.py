@@ -99,8 +99,14 @@ def test_attention_c_entry_refuses():
     import ctypes
 
     from glenet_amd import _lib
-    from glenet_amd.attention import _Attention
     lib = _lib.load()
+
+    class _Attention(ctypes.Structure):        # glx_attention
+        _fields_ = ([(n, ctypes.c_void_p) for n in ("q", "k", "v", "out", "lse", "key_mask", "q_cnt", "k_cnt")]
+                    + [(n, ctypes.c_int64) for n in ("q_rows", "k_rows", "q_len", "k_len", "q_stride", "q_head_stride", "k_stride",
+                                                     "k_head_stride", "v_stride", "v_head_stride")]
+                    + [(n, ctypes.c_int32) for n in ("frames", "heads", "kv_heads", "dim", "dtype")] + [("scale", ctypes.c_float)])
+
 
     def call(backward=False, **kw):
         d = _Attention(q=64, k=64, v=64, out=64, lse=64, q_rows=2000, k_rows=8000, q_len=1000, k_len=4000, q_stride=64, q_head_stride=16,
