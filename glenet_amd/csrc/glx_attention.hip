@@ -11,13 +11,12 @@
 
 template <typename T, int DP, int RW>
 __global__ __launch_bounds__(256) void k_xa_forward(XaArgs a) {
-  constexpr int KW = 4 / RW, BN = XA_KEYS * (KW == 4 && sizeof(T) == 2 ? 2 : 1), SUB = BN / 32 / KW > 0 ? BN / 32 / KW : 1;
-  constexpr int KU = BN / 32 < KW ? BN / 32 : KW;          // waves of a row tile that have keys of a staged tile
+  constexpr int KW = 4 / RW, BN = KW == 4 ? 128 : 64, SUB = BN / 32 / KW;
   constexpr int KS = DP / 16, DT = DP / 32;
   typedef XaTile<T, DP> Tile;
   constexpr int TB = BN * Tile::LD;
   constexpr int JB = KW > 1 ? 4 * 32 * (DP + 1) * 4 : 0;
-  constexpr int STAGES = 4 * TB <= 140 * 1024 ? 2 : 1;
+  constexpr int STAGES = 4 * TB <= 80 * 1024 ? 2 : 1;        // two blocks per compute unit before two buffers per block
   constexpr int BYTES = STAGES * 2 * TB > JB ? STAGES * 2 * TB : JB;
   __shared__ __attribute__((aligned(16))) char smem[BYTES];
   __shared__ float sm[4][32], sl[4][32];
@@ -39,21 +38,23 @@ __global__ __launch_bounds__(256) void k_xa_forward(XaArgs a) {
     const T* p = (const T*)a.q + (f.q0 + qi) * a.sq + head * a.hq;
 #pragma unroll
     for (int s = 0; s < KS; ++s) {
+      Q[s] = typename XaFrag<T>::vec{};
       if (live) Q[s] = xa_row<T>(p, s * 16 + half * 8, a.dim);
-      else Q[s] = typename XaFrag<T>::vec{};
+      if (a.scale2 < 0.f) Q[s] = -Q[s];                      // the maximum is taken of unscaled scores
     }
   }
   xf16 O[DT];
 #pragma unroll
   for (int i = 0; i < DT; ++i) O[i] = (xf16)(0.f);
-  float m = -INFINITY, l = 0.f;
+  const float scale2 = fabsf(a.scale2);
+  float m = -INFINITY, l = 0.f;                               // m unscaled
   XaStage<T, DP, BN, 256> ks, vs;
-  unsigned long long ok[2], nok[2];
+  unsigned long long ok[2] = {0, 0}, nok[2] = {0, 0};
   auto fetch = [&](int t) {
     const int k0 = t * BN;
 #pragma unroll
     for (int h = 0; h < BN / 64; ++h) nok[h] = xa_valid(a.mask, f.k0 + k0 + h * 64, f.nk - k0 - h * 64);
-    auto on = [&](int r) { return (nok[BN == 64 ? 0 : r >> 6] >> (r & 63)) & 1; };
+    auto on = [&](int r) { return (nok[r >> 6] >> (r & 63)) & 1; };
     ks.fetch([&](int r) { return on(r) ? kbase + (long long)(k0 + r) * a.sk : (const T*)nullptr; }, a.dim);
     vs.fetch([&](int r) { return on(r) ? vbase + (long long)(k0 + r) * a.sv : (const T*)nullptr; }, a.dim);
   };
@@ -69,44 +70,63 @@ __global__ __launch_bounds__(256) void k_xa_forward(XaArgs a) {
     if (more) fetch(t + 1);
     const char* tk = smem + (STAGES == 2 ? buf * 2 * TB : 0);
     const char* tv = tk + TB;
-    if (KU == KW || kw < KU) {
+    unsigned valid[SUB];
+    bool some = false, every = true;
+#pragma unroll
+    for (int u = 0; u < SUB; ++u) {
+      const int c0 = (u * KW + kw) * 32;                      // first of this wave's 32 keys
+      valid[u] = (unsigned)(ok[c0 >> 6] >> (c0 & 63));
+      some |= valid[u] != 0;
+      every &= valid[u] == 0xffffffffu;
+    }
+    if (some) {
+      xf16 s[SUB];
+      float top = -INFINITY;
 #pragma unroll
       for (int u = 0; u < SUB; ++u) {
-        const int c0 = (u * KU + kw) * 32;                    // first of this wave's 32 keys in the tile
-        const unsigned valid = (unsigned)(ok[BN == 64 ? 0 : c0 >> 6] >> (c0 & 63));
-        if (!valid) continue;
-        xf16 s = (xf16)(0.f);
+        s[u] = (xf16)(0.f);
 #pragma unroll
-        for (int k = 0; k < KS; ++k) xa_mma(s, xa_along<T, DP>(tk, c0 + l32, k, half), Q[k]);
-        float top = -INFINITY;
-        if (valid == 0xffffffffu) {
+        for (int k = 0; k < KS; ++k) xa_mma(s[u], xa_along<T, DP>(tk, (u * KW + kw) * 32 + l32, k, half), Q[k]);
+      }
+      if (!every) {
 #pragma unroll
-          for (int i = 0; i < 16; ++i) { s[i] *= a.scale2; top = fmaxf(top, s[i]); }
-        } else {
-          const unsigned mine = valid >> (half * 4);
+        for (int u = 0; u < SUB; ++u)
 #pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            s[i] = (mine >> ((i >> 2) * 8 + (i & 3))) & 1 ? s[i] * a.scale2 : -INFINITY;
-            top = fmaxf(top, s[i]);
-          }
-        }
-        top = fmaxf(top, __shfl_xor(top, 32, 64));
-        const float now = fmaxf(m, top), at = now == -INFINITY ? 0.f : now;
-        const float shrink = exp2f(m - at);
+          for (int i = 0; i < 16; ++i)
+            if (!((valid[u] >> (half * 4 + (i >> 2) * 8 + (i & 3))) & 1)) s[u][i] = -INFINITY;
+      }
+#pragma unroll
+      for (int u = 0; u < SUB; ++u)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) top = fmaxf(top, s[u][i]);
+      top = fmaxf(top, __shfl_xor(top, 32, 64));
+      // m follows the maximum only where p would pass 2^8: then O and l shrink, else the tile is added as it is
+      if (__any((top - m) * scale2 > 8.f || m == -INFINITY)) {
+        const float now = fmaxf(m, top), shrink = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((m - now) * scale2);
         m = now;
-        float sum = 0.f;
-#pragma unroll
-        for (int i = 0; i < 16; ++i) { s[i] = exp2f(s[i] - at); sum += s[i]; }
-        l = l * shrink + sum;
+        l *= shrink;
 #pragma unroll
         for (int i = 0; i < DT; ++i)
 #pragma unroll
           for (int e = 0; e < 16; ++e) O[i][e] *= shrink;
+      }
+      // (16-bit: one fused operation; its rounding of m scale2 is a factor that p and l share.  fp32 keeps 2^0 = 1 exactly)
+      const float ref = m == -INFINITY ? 0.f : m, at = ref * scale2;
+#pragma unroll
+      for (int u = 0; u < SUB; ++u) {
+        float sum = 0.f;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          s[u][i] = __builtin_amdgcn_exp2f(sizeof(T) == 2 ? __builtin_fmaf(s[u][i], scale2, -at) : (s[u][i] - ref) * scale2);
+          if (!every && scale2 == 0.f && !((valid[u] >> (half * 4 + (i >> 2) * 8 + (i & 3))) & 1)) s[u][i] = 0.f;
+          sum += s[u][i];
+        }
+        l += sum;
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
-          const typename XaFrag<T>::vec p = xa_pack<T>(s, c);
+          const typename XaFrag<T>::vec p = xa_pack<T>(s[u], c);
 #pragma unroll
-          for (int i = 0; i < DT; ++i) xa_mma(O[i], xa_down<T, DP>(tv, c0 + c * 16, i * 32, lane), p);
+          for (int i = 0; i < DT; ++i) xa_mma(O[i], xa_down<T, DP>(tv, (u * KW + kw) * 32 + c * 16, i * 32, lane), p);
         }
       }
     }
@@ -120,6 +140,7 @@ __global__ __launch_bounds__(256) void k_xa_forward(XaArgs a) {
     buf ^= 1;
   }
   l += __shfl_xor(l, 32, 64);
+  m = m == -INFINITY ? m : m * scale2;
   if (KW > 1) {                                               // the waves of a row tile, joined in order
     if (half == 0) { sm[wave][l32] = m; sl[wave][l32] = l; }
     __syncthreads();
@@ -128,7 +149,7 @@ __global__ __launch_bounds__(256) void k_xa_forward(XaArgs a) {
     for (int i = 0; i < KW; ++i) top = fmaxf(top, sm[rw * KW + i][l32]);
     const float at = top == -INFINITY ? 0.f : top;
     float* x = (float*)smem + wave * 32 * (DP + 1);
-    const float w = exp2f(m - at);
+    const float w = __builtin_amdgcn_exp2f(m - at);
     float all = 0.f;
 #pragma unroll
     for (int i = 0; i < KW; ++i) all += sl[rw * KW + i][l32] * exp2f(sm[rw * KW + i][l32] - at);
@@ -214,7 +235,7 @@ __global__ __launch_bounds__(256) void k_xa_join(XaArgs a) {
 // ------------------------------------------------------------------------------------------------ host
 int xa_splits(long long blocks, long long keys_per_frame) {
   if (blocks < 1) blocks = 1;
-  long long s = 1024 / blocks, most = keys_per_frame / 256;        // 256 keys a split, at least
+  long long s = 512 / blocks, most = keys_per_frame / 256;        // 256 keys a split, at least
   s = s < most ? s : most;
   return (int)(s < 1 ? 1 : (s > 256 ? 256 : s));
 }

@@ -138,7 +138,7 @@ __global__ __launch_bounds__(256) void k_xa_dq(XaArgs a) {
         const unsigned mine = valid >> (half * 4);
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
-          const float p = exp2f(s[i] * a.scale2 - lse) * (d[i] - delta);
+          const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], a.scale2, -lse)) * (d[i] - delta);
           s[i] = (mine >> ((i >> 2) * 8 + (i & 3))) & 1 ? p : 0.f;
         }
         xa_range<T, DT>(s, D, e);
@@ -278,7 +278,7 @@ __global__ __launch_bounds__(256) void k_xa_dkv(XaArgs a) {
         const xf4 de = *reinterpret_cast<const xf4*>(&srow[buf][1][u * 32 + g * 8 + half * 4]);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const float p = exp2f(s[g * 4 + i] * a.scale2 - ls[i]);
+          const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[g * 4 + i], a.scale2, -ls[i]));
           s[g * 4 + i] = valid ? p : 0.f;
           d[g * 4 + i] = valid ? p * (d[g * 4 + i] - de[i]) : 0.f;
         }
