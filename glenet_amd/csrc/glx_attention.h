@@ -29,6 +29,7 @@ struct XaArgs {
   long long sq, hq, sk, hk, sv, hv, sg, hg;      // elements between rows and between heads of q, k, v, go
   long long nq, nk;
   int frames, lq, lk, heads, kvheads, group, dim, splits;
+  int dma;                          // bits: rows of q, k, v, go are whole 16-byte chunks
   float scale, scale2;              // scale2 = scale log2(e)
 };
 
@@ -46,40 +47,48 @@ __device__ __forceinline__ void xa_mma(xf16& c, const XaFrag<float>::vec& a, con
   for (int i = 0; i < 8; ++i) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a[i], b[i], c, 0, 0, 0);
 }
 
-// A staged tile: rows of DP values, 16 bytes of padding (the 32 rows of an operand read spread over the banks)
+// A staged tile: rows of DP values without padding, the 16-byte chunks of a row in an order of the row's own.  Reads along the
+// rows take one chunk of 16 consecutive rows at a time, transposing reads four chunks (64 bytes) of 4 consecutive rows: chunk c
+// of row r lies at c ^ swap(r) so that both cover all 64 banks.  (Rows padded by 16 bytes left the transposing reads with
+// four-way conflicts: dK and dV of 4096 x 16384, 2 x 8 heads of 128, bf16, 2271 us instead of 1831.)
 template <typename T, int DP> struct XaTile {
-  static constexpr int LD = DP * (int)sizeof(T) + 16, E = 16 / (int)sizeof(T), CPR = DP / E;
+  static constexpr int LD = DP * (int)sizeof(T), E = 16 / (int)sizeof(T), CPR = DP / E;
+  static __device__ __forceinline__ int swap(int r) {
+    if (sizeof(T) == 4) return DP % 64 == 0 ? r & 15 : (r >> 1) & 7;
+    return ((r >> 2) & 3) ^ (DP == 128 ? (r & 3) << 2 : DP == 64 ? (r & 2) << 1 : 0);
+  }
+  static __device__ __forceinline__ int at(int r, int c) { return r * LD + (c ^ swap(r)) * 16; }
 };
 
 // eight values along a row: the operand whose k index is d; row = l32, k = 16 ks + 8 half + 0..7
 template <typename T, int DP>
 __device__ __forceinline__ typename XaFrag<T>::vec xa_along(const char* tile, int row, int ks, int half) {
-  const char* p = tile + row * XaTile<T, DP>::LD + (ks * 16 + half * 8) * (int)sizeof(T);
   if constexpr (sizeof(T) == 2) {
-    return *reinterpret_cast<const typename XaFrag<T>::vec*>(p);
+    return *reinterpret_cast<const typename XaFrag<T>::vec*>(tile + XaTile<T, DP>::at(row, ks * 2 + half));
   } else {
-    const xf4 a = *reinterpret_cast<const xf4*>(p), b = *reinterpret_cast<const xf4*>(p + 16);
+    const xf4 a = *reinterpret_cast<const xf4*>(tile + XaTile<T, DP>::at(row, ks * 4 + half * 2));
+    const xf4 b = *reinterpret_cast<const xf4*>(tile + XaTile<T, DP>::at(row, ks * 4 + half * 2 + 1));
     return {a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
   }
 }
 // eight values down the rows row0 + 4 half + {0..3, 8..11}, column d0 + l32: the operand whose k index is the row
 template <typename T, int DP>
 __device__ __forceinline__ typename XaFrag<T>::vec xa_down(const char* tile, int row0, int d0, int lane) {
-  constexpr int LD = XaTile<T, DP>::LD;
+  typedef XaTile<T, DP> Tile;
   const int half = lane >> 5;
   if constexpr (sizeof(T) == 2) {
     // a 16-lane group reads 4 rows x 16 columns and every lane gets a column's four values
     typedef xs4 __attribute__((address_space(3))) * lds_p;
-    const char* p = tile + (row0 + half * 4 + ((lane >> 2) & 3)) * LD + (d0 + (lane & 16) + (lane & 3) * 4) * 2;
-    const xs4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_p)(p));
-    const xs4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_p)(p + 8 * LD));
+    const int row = row0 + half * 4 + ((lane >> 2) & 3), c = d0 / 8 + ((lane >> 3) & 2) + ((lane >> 1) & 1), b = (lane & 1) * 8;
+    const xs4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_p)(tile + Tile::at(row, c) + b));
+    const xs4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_p)(tile + Tile::at(row + 8, c) + b));
     const xs8 v = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
     return __builtin_bit_cast(typename XaFrag<T>::vec, v);
   } else {
-    const char* p = tile + (row0 + half * 4) * LD + (d0 + (lane & 31)) * 4;
+    const int c = (d0 + (lane & 31)) >> 2, b = (lane & 3) * 4;
     typename XaFrag<T>::vec v;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = *reinterpret_cast<const float*>(p + ((i >> 2) * 8 + (i & 3)) * LD);
+    for (int i = 0; i < 8; ++i) v[i] = *reinterpret_cast<const float*>(tile + Tile::at(row0 + half * 4 + (i >> 2) * 8 + (i & 3), c) + b);
     return v;
   }
 }
@@ -102,39 +111,70 @@ __device__ __forceinline__ typename XaFrag<T>::vec xa_row(const T* p, int d, int
 }
 
 // ------------------------------------------------------------------------------------------------ staging
-// ROWS rows through registers into LDS.  row(r) gives a row's address or NULL (zeros: a masked or absent row is never read).
-template <typename T, int DP, int ROWS, int THREADS>
-struct XaStage {
-  static constexpr int E = XaTile<T, DP>::E, CPR = XaTile<T, DP>::CPR, LD = XaTile<T, DP>::LD;
-  static constexpr int N = (ROWS * CPR + THREADS - 1) / THREADS;
+// ROWS rows of a tensor into a tile.  Rows that are whole 16-byte chunks go straight from memory to LDS (no registers, no LDS
+// writes; a lane fetches the chunk that belongs at its place): `place` keeps the thread's offsets within a tile, `issue` starts the
+// transfers of the rows below n and lets the places behind them repeat the last one, `settle` waits for the thread's own transfers
+// and clears the places of rows that are not there or masked -- so those never reach a product, whatever they hold.  Other rows
+// take the way through registers, element by element where they are ragged.  rowoff(r): elements from the tile's base to row r.
+template <typename T, int DP, int ROWS>
+struct XaLoad {
+  static constexpr int E = XaTile<T, DP>::E, CPR = XaTile<T, DP>::CPR, N = ROWS * CPR / 256;
+  static_assert(ROWS * CPR % 256 == 0, "whole rounds of the block");
   typedef typename GlxVec<T, E>::vec vec;
-  vec r[N];
+  int off[N];                 // bytes
+  static __device__ __forceinline__ int row_of(int i) { return ((int)threadIdx.x + i * 256) / CPR; }
+  static __device__ __forceinline__ int chunk_of(int i) {
+    const int r = row_of(i);
+    return ((int)threadIdx.x + i * 256 - r * CPR) ^ XaTile<T, DP>::swap(r);
+  }
   template <typename F>
-  __device__ __forceinline__ void fetch(F row, int D) {
+  __device__ __forceinline__ void place(F rowoff, int D) {
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const int c = threadIdx.x + i * THREADS, rr = c / CPR, d = (c - rr * CPR) * E;
+    for (int i = 0; i < N; ++i) off[i] = (int)((rowoff(row_of(i)) + (chunk_of(i) * E < D ? chunk_of(i) * E : 0)) * (int)sizeof(T));
+  }
+  template <typename F, typename V>
+  __device__ __forceinline__ void issue(char* tile, const T* base, F rowoff, V valid, int n, int D, bool dma) const {
+    if (dma) {
+      char* to = tile + __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6) * 1024;
+      if (n >= ROWS) {
 #pragma unroll
-      for (int e = 0; e < E; ++e) r[i][e] = (T)0.f;
-      if (ROWS * CPR % THREADS && rr >= ROWS) continue;
-      const T* p = row(rr);
-      if (!p) continue;
-      if (d + E <= D) {
-        r[i] = GlxVec<T, E>::load(p + d);
+        for (int i = 0; i < N; ++i)
+          __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)((const char*)base + (unsigned)off[i]),
+                                           (__attribute__((address_space(3))) void*)(to + i * 4096), 16, 0, 0);
       } else {
 #pragma unroll
-        for (int e = 0; e < E; ++e)
-          if (d + e < D) r[i][e] = p[d + e];
+        for (int i = 0; i < N; ++i) {
+          const int r = row_of(i) < n ? row_of(i) : n - 1, c = chunk_of(i) * E < D ? chunk_of(i) * E : 0;
+          __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(base + rowoff(r) + c),
+                                           (__attribute__((address_space(3))) void*)(to + i * 4096), 16, 0, 0);
+        }
+      }
+    } else {
+#pragma unroll 1
+      for (int i = 0; i < N; ++i) {
+        const int r = row_of(i), d = chunk_of(i) * E;
+        vec v = {};
+        if (r < n && valid(r)) {
+          const T* p = base + rowoff(r) + d;
+          if (d + E <= D) {
+            v = GlxVec<T, E>::load(p);
+          } else {
+#pragma unroll
+            for (int e = 0; e < E; ++e)
+              if (d + e < D) v[e] = p[e];
+          }
+        }
+        *reinterpret_cast<vec*>(tile + (threadIdx.x + i * 256) * 16) = v;
       }
     }
   }
-  __device__ __forceinline__ void put(char* tile) const {
+  template <typename V>
+  __device__ __forceinline__ void settle(char* tile, V valid, bool all) const {
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    if (all) return;
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const int c = threadIdx.x + i * THREADS, rr = c / CPR;
-      if (ROWS * CPR % THREADS && rr >= ROWS) continue;
-      *reinterpret_cast<vec*>(tile + rr * LD + (c - rr * CPR) * 16) = r[i];
-    }
+    for (int i = 0; i < N; ++i)
+      if (!valid(row_of(i))) *reinterpret_cast<vec*>(tile + (threadIdx.x + i * 256) * 16) = vec{};
   }
 };
 
@@ -202,6 +242,13 @@ __device__ __forceinline__ XaPlace xa_place(const XaArgs& a, long long t, int un
 __device__ __forceinline__ unsigned long long xa_valid(const unsigned char* mask, long long k0, int n) {
   const int lane = threadIdx.x & 63;
   return __ballot(lane < n && (!mask || mask[k0 + lane] != 0));
+}
+
+// host: rows of `tile` consecutive places start at 16-byte boundaries, are whole chunks and lie within 31 bits of each other
+static inline bool xa_chunked(const void* p, long long row, long long head, int dim, int dtype) {
+  const long long e = (long long)glx_elem_size(dtype);
+  return ((uintptr_t)p & 15) == 0 && dim * e % 16 == 0 && row * e % 16 == 0 && head * e % 16 == 0 && row >= 0 && head >= 0
+         && row * e < (1ll << 22) && head * e < (1ll << 22);
 }
 
 // host: upper bound of the tiles that xa_place hands out

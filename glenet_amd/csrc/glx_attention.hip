@@ -11,13 +11,12 @@
 
 template <typename T, int DP, int RW>
 __global__ __launch_bounds__(256) void k_xa_forward(XaArgs a) {
-  constexpr int KW = 4 / RW, BN = KW == 4 ? 128 : 64, SUB = BN / 32 / KW;
+  constexpr int KW = 4 / RW, BN = KW == 4 ? 128 : 64, SUB = BN / 32 / KW;          // keys of a staged tile, of them 32 SUB a wave's
   constexpr int KS = DP / 16, DT = DP / 32;
   typedef XaTile<T, DP> Tile;
   constexpr int TB = BN * Tile::LD;
   constexpr int JB = KW > 1 ? 4 * 32 * (DP + 1) * 4 : 0;
-  constexpr int STAGES = 4 * TB <= 80 * 1024 ? 2 : 1;        // two blocks per compute unit before two buffers per block
-  constexpr int BYTES = STAGES * 2 * TB > JB ? STAGES * 2 * TB : JB;
+  constexpr int BYTES = 4 * TB > JB ? 4 * TB : JB;
   __shared__ __attribute__((aligned(16))) char smem[BYTES];
   __shared__ float sm[4][32], sl[4][32];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5, l32 = lane & 31;
@@ -48,27 +47,35 @@ __global__ __launch_bounds__(256) void k_xa_forward(XaArgs a) {
   for (int i = 0; i < DT; ++i) O[i] = (xf16)(0.f);
   const float scale2 = fabsf(a.scale2);
   float m = -INFINITY, l = 0.f;                               // m unscaled
-  XaStage<T, DP, BN, 256> ks, vs;
+  XaLoad<T, DP, BN> kl, vl;
+  const bool kdma = a.dma & 2, vdma = a.dma & 4;
+  auto koff = [&](int r) { return (long long)r * a.sk; };
+  auto voff = [&](int r) { return (long long)r * a.sv; };
+  kl.place(koff, a.dim);
+  vl.place(voff, a.dim);
   unsigned long long ok[2] = {0, 0}, nok[2] = {0, 0};
-  auto fetch = [&](int t) {
-    const int k0 = t * BN;
+  auto on = [&](int r) { return (bool)((nok[r >> 6] >> (r & 63)) & 1); };
+  auto load = [&](int t, char* to) {
+    const int k0 = t * BN, n = f.nk - k0;
 #pragma unroll
-    for (int h = 0; h < BN / 64; ++h) nok[h] = xa_valid(a.mask, f.k0 + k0 + h * 64, f.nk - k0 - h * 64);
-    auto on = [&](int r) { return (nok[r >> 6] >> (r & 63)) & 1; };
-    ks.fetch([&](int r) { return on(r) ? kbase + (long long)(k0 + r) * a.sk : (const T*)nullptr; }, a.dim);
-    vs.fetch([&](int r) { return on(r) ? vbase + (long long)(k0 + r) * a.sv : (const T*)nullptr; }, a.dim);
+    for (int h = 0; h < BN / 64; ++h) nok[h] = xa_valid(a.mask, f.k0 + k0 + h * 64, n - h * 64);
+    kl.issue(to, kbase + (long long)k0 * a.sk, koff, on, n, a.dim, kdma);
+    vl.issue(to + TB, vbase + (long long)k0 * a.sv, voff, on, n, a.dim, vdma);
   };
+  // (masked scores are replaced, so only the values' rows have to be clean)
+  auto settle = [&](char* to) { vl.settle(to + TB, on, nok[0] == ~0ull && nok[BN / 64 - 1] == ~0ull); };
   if (t0 < t1) {
-    fetch(t0);
-    ks.put(smem); vs.put(smem + TB);
+    load(t0, smem);
+    settle(smem);
   }
   ok[0] = nok[0]; ok[1] = nok[1];
   __syncthreads();
   int buf = 0;
   for (int t = t0; t < t1; ++t) {
     const bool more = t + 1 < t1;
-    if (more) fetch(t + 1);
-    const char* tk = smem + (STAGES == 2 ? buf * 2 * TB : 0);
+    char* next = smem + (buf ^ 1) * 2 * TB;
+    if (more) load(t + 1, next);
+    const char* tk = smem + buf * 2 * TB;
     const char* tv = tk + TB;
     unsigned valid[SUB];
     bool some = false, every = true;
@@ -130,11 +137,7 @@ __global__ __launch_bounds__(256) void k_xa_forward(XaArgs a) {
         }
       }
     }
-    if (STAGES == 1) __syncthreads();
-    if (more) {
-      char* n = smem + (STAGES == 2 ? (buf ^ 1) * 2 * TB : 0);
-      ks.put(n); vs.put(n + TB);
-    }
+    if (more) settle(next);
     ok[0] = nok[0]; ok[1] = nok[1];
     __syncthreads();
     buf ^= 1;
@@ -245,7 +248,8 @@ static XaForward xa_forward_plan(const glx_attention* t) {
   const int group = t->heads / t->kv_heads;
   const bool counts = t->q_cnt != nullptr;
   const long long rows = counts ? t->q_rows * group / (t->frames > 0 ? t->frames : 1) : (long long)t->q_len * group;
-  p.rw = rows <= 64 ? 1 : 4;
+  // (fp32 rows beyond 64: the keys of four waves do not fit LDS twice)
+  p.rw = rows <= 64 ? (t->dtype == GLX_F32 && t->dim > 64 ? 2 : 1) : 4;
   p.tiles = xa_tiles(t->q_rows * group, t->frames, (int)(t->q_len * group), counts, p.rw * 32);
   const long long blocks = (counts ? t->q_rows * group / (p.rw * 32) + 1 : p.tiles) * t->kv_heads;
   p.splits = xa_splits(blocks, t->frames > 0 ? t->k_rows / t->frames : 0);
@@ -274,6 +278,10 @@ XaArgs xa_args(const glx_attention* t) {
   a.nq = t->q_rows; a.nk = t->k_rows;
   a.frames = t->frames; a.lq = (int)t->q_len; a.lk = (int)t->k_len; a.heads = t->heads; a.kvheads = t->kv_heads;
   a.group = t->heads / t->kv_heads; a.dim = t->dim; a.splits = 1;
+  a.dma = xa_chunked(t->q, a.sq, a.hq, a.dim, t->dtype) | xa_chunked(t->k, a.sk, 0, a.dim, t->dtype) << 1
+          | xa_chunked(t->v, a.sv, 0, a.dim, t->dtype) << 2;
+  if (a.hk * glx_elem_size(t->dtype) % 16) a.dma &= ~2;
+  if (a.hv * glx_elem_size(t->dtype) % 16) a.dma &= ~4;
   a.scale = t->scale; a.scale2 = t->scale * 1.4426950408889634f;
   return a;
 }
@@ -287,7 +295,8 @@ extern "C" size_t glx_attention_workspace_bytes(const glx_attention* t) {
 template <typename T, int DP>
 static void xa_launch_forward(const XaForward& p, const XaArgs& a, hipStream_t st) {
   const dim3 grid((unsigned)(p.tiles * p.splits), a.kvheads);
-  if (p.rw == 1) hipLaunchKernelGGL((k_xa_forward<T, DP, 1>), grid, dim3(256), 0, st, a);
+  constexpr int SMALL = sizeof(T) == 4 && DP > 64 ? 2 : 1;
+  if (p.rw == SMALL) hipLaunchKernelGGL((k_xa_forward<T, DP, SMALL>), grid, dim3(256), 0, st, a);
   else hipLaunchKernelGGL((k_xa_forward<T, DP, 4>), grid, dim3(256), 0, st, a);
 }
 template <typename T>

@@ -55,13 +55,12 @@ __device__ __forceinline__ float xa_unrange(int e) {
 // ------------------------------------------------------------------------------------------------ dQ, delta
 template <typename T, int DP, int RW>
 __global__ __launch_bounds__(256) void k_xa_dq(XaArgs a) {
-  constexpr int KW = 4 / RW, BN = XA_KEYS, KU = BN / 32 < KW ? BN / 32 : KW, SUB = BN / 32 / KU;
+  constexpr int KW = 4 / RW, BN = KW == 4 ? 128 : 64, SUB = BN / 32 / KW;
   constexpr int KS = DP / 16, DT = DP / 32;
   typedef XaTile<T, DP> Tile;
   constexpr int TB = BN * Tile::LD;
   constexpr int JB = KW > 1 ? 4 * 32 * (DP + 1) * 4 : 0;
-  constexpr int STAGES = 4 * TB <= 140 * 1024 ? 2 : 1;
-  constexpr int BYTES = STAGES * 2 * TB > JB ? STAGES * 2 * TB : JB;
+  constexpr int BYTES = 4 * TB > JB ? 4 * TB : JB;
   __shared__ __attribute__((aligned(16))) char smem[BYTES];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5, l32 = lane & 31;
   const int rw = wave / KW, kw = wave % KW;
@@ -103,31 +102,41 @@ __global__ __launch_bounds__(256) void k_xa_dq(XaArgs a) {
 #pragma unroll
   for (int i = 0; i < DT; ++i) D[i] = (xf16)(0.f);
   int e = 999;
-  XaStage<T, DP, BN, 256> ks, vs;
-  unsigned long long ok = 0, nok = 0;
-  auto fetch = [&](int t) {
-    const int k0 = t * BN;
-    nok = xa_valid(a.mask, f.k0 + k0, f.nk - k0);
-    ks.fetch([&](int r) { return (nok >> r) & 1 ? kbase + (long long)(k0 + r) * a.sk : (const T*)nullptr; }, a.dim);
-    vs.fetch([&](int r) { return (nok >> r) & 1 ? vbase + (long long)(k0 + r) * a.sv : (const T*)nullptr; }, a.dim);
+  XaLoad<T, DP, BN> kl, vl;
+  const bool kdma = a.dma & 2, vdma = a.dma & 4;
+  auto koff = [&](int r) { return (long long)r * a.sk; };
+  auto voff = [&](int r) { return (long long)r * a.sv; };
+  kl.place(koff, a.dim);
+  vl.place(voff, a.dim);
+  unsigned long long ok[2] = {0, 0}, nok[2] = {0, 0};
+  auto on = [&](int r) { return (bool)((nok[r >> 6] >> (r & 63)) & 1); };
+  auto load = [&](int t, char* to) {
+    const int k0 = t * BN, n = f.nk - k0;
+#pragma unroll
+    for (int h = 0; h < BN / 64; ++h) nok[h] = xa_valid(a.mask, f.k0 + k0 + h * 64, n - h * 64);
+    kl.issue(to, kbase + (long long)k0 * a.sk, koff, on, n, a.dim, kdma);
+    vl.issue(to + TB, vbase + (long long)k0 * a.sv, voff, on, n, a.dim, vdma);
   };
+  // (masked products with the values are replaced, so only the keys' rows have to be clean)
+  auto settle = [&](char* to) { kl.settle(to, on, nok[0] == ~0ull && nok[BN / 64 - 1] == ~0ull); };
   if (t0 < t1) {
-    fetch(t0);
-    ks.put(smem); vs.put(smem + TB);
+    load(t0, smem);
+    settle(smem);
   }
-  ok = nok;
+  ok[0] = nok[0]; ok[1] = nok[1];
   __syncthreads();
   int buf = 0;
   for (int t = t0; t < t1; ++t) {
     const bool more = t + 1 < t1;
-    if (more) fetch(t + 1);
-    const char* tk = smem + (STAGES == 2 ? buf * 2 * TB : 0);
+    char* next = smem + (buf ^ 1) * 2 * TB;
+    if (more) load(t + 1, next);
+    const char* tk = smem + buf * 2 * TB;
     const char* tv = tk + TB;
-    if (kw < KU) {
+    {
 #pragma unroll
       for (int u = 0; u < SUB; ++u) {
-        const int c0 = (u * KU + kw) * 32;
-        const unsigned valid = (unsigned)(ok >> c0);
+        const int c0 = (u * KW + kw) * 32;
+        const unsigned valid = (unsigned)(ok[c0 >> 6] >> (c0 & 63));
         if (!valid) continue;
         xf16 s = (xf16)(0.f), d = (xf16)(0.f);
 #pragma unroll
@@ -150,12 +159,8 @@ __global__ __launch_bounds__(256) void k_xa_dq(XaArgs a) {
         }
       }
     }
-    if (STAGES == 1) __syncthreads();
-    if (more) {
-      char* n = smem + (STAGES == 2 ? (buf ^ 1) * 2 * TB : 0);
-      ks.put(n); vs.put(n + TB);
-    }
-    ok = nok;
+    if (more) settle(next);
+    ok[0] = nok[0]; ok[1] = nok[1];
     __syncthreads();
     buf ^= 1;
   }
@@ -178,7 +183,7 @@ __global__ __launch_bounds__(256) void k_xa_dq(XaArgs a) {
         for (int k = 0; k < 16; ++k) {
           float v = 0.f;
 #pragma unroll
-          for (int j = 0; j < KU; ++j) v += x[j * 32 * (DP + 1) + l32 * (DP + 1) + i * 32 + (k >> 2) * 8 + half * 4 + (k & 3)];
+          for (int j = 0; j < KW; ++j) v += x[j * 32 * (DP + 1) + l32 * (DP + 1) + i * 32 + (k >> 2) * 8 + half * 4 + (k & 3)];
           D[i][k] = v;
         }
     }
@@ -214,7 +219,7 @@ __global__ __launch_bounds__(256) void k_xa_dkv(XaArgs a) {
   const XaPlace f = xa_place(a, blockIdx.x / a.splits, 128, true);
   if (f.tile < 0) return;
   const int rows = f.nq * a.group, key = f.tile * 128 + wave * 32 + l32;
-  const int tiles = (rows + BM - 1) / BM;
+  const int step = a.group <= BM ? BM / a.group * a.group : BM, tiles = (rows + step - 1) / step;
   const int t0 = (int)((long long)tiles * split / a.splits), t1 = (int)((long long)tiles * (split + 1) / a.splits);
   const bool there = key < f.nk, valid = there && (!a.mask || a.mask[f.k0 + key] != 0);
   typename XaFrag<T>::vec K[KS], V[KS];
@@ -233,35 +238,60 @@ __global__ __launch_bounds__(256) void k_xa_dkv(XaArgs a) {
 #pragma unroll
   for (int i = 0; i < DT; ++i) dK[i] = dV[i] = (xf16)(0.f);
   int e = 999;
-  XaStage<T, DP, BM, 256> qs, gs;
+  XaLoad<T, DP, BM> ql, gl;
+  const bool qdma = (a.dma & 1) && a.group <= BM, gdma = (a.dma & 8) && a.group <= BM;
+  // a tile holds whole queries, so that a thread's rows are the same distance from every tile's first query
+  auto qoff = [&](int r) {
+    const int qi = r / a.group;
+    return qi * a.sq + (r - qi * a.group) * a.hq;
+  };
+  auto goff = [&](int r) {
+    const int qi = r / a.group;
+    return qi * a.sg + (r - qi * a.group) * a.hg;
+  };
+  ql.place(qoff, a.dim);
+  gl.place(goff, a.dim);
   float lse = INFINITY, delta = 0.f;
-  auto fetch = [&](int t) {
-    const int r0 = t * BM;
-    auto place = [&](const void* base, long long s, long long h, int r) -> const T* {
-      if (r0 + r >= rows) return nullptr;
-      const int qi = (int)((unsigned)(r0 + r) / (unsigned)a.group);
-      return (const T*)base + (f.q0 + qi) * s + (hk * a.group + (r0 + r - qi * a.group)) * h;
+  int there_next = 0;                                          // rows of the tile on its way
+  auto load = [&](int t, int buf) {
+    const long long r0 = (long long)t * step;
+    const int n = rows - r0 < step ? (int)(rows - r0) : step;
+    there_next = n;
+    auto on = [&](int r) { return r < n; };
+    char* to = smem + buf * 2 * TB;
+    const long long q0 = f.q0 + r0 / a.group;
+    const int g0 = hk * a.group + (int)(r0 % a.group);        // (0 behind hk but for groups wider than a tile)
+    // groups wider than a tile start within a query: their offsets are not those of `place`
+    auto qwide = [&](int r) {
+      const int qi = (int)((r0 + r) / a.group);
+      return (qi - r0 / a.group) * a.sq + ((r0 + r - (long long)qi * a.group) - r0 % a.group) * a.hq;
     };
-    qs.fetch([&](int r) { return place(a.q, a.sq, a.hq, r); }, a.dim);
-    gs.fetch([&](int r) { return place(a.go, a.sg, a.hg, r); }, a.dim);
+    auto gwide = [&](int r) {
+      const int qi = (int)((r0 + r) / a.group);
+      return (qi - r0 / a.group) * a.sg + ((r0 + r - (long long)qi * a.group) - r0 % a.group) * a.hg;
+    };
+    ql.issue(to, (const T*)a.q + q0 * a.sq + g0 * a.hq, qwide, on, n, a.dim, qdma);
+    gl.issue(to + TB, (const T*)a.go + q0 * a.sg + g0 * a.hg, gwide, on, n, a.dim, gdma);
     lse = INFINITY; delta = 0.f;
-    if ((int)threadIdx.x < BM && r0 + (int)threadIdx.x < rows) {
-      const int r = r0 + threadIdx.x, qi = (int)((unsigned)r / (unsigned)a.group);
+    if ((int)threadIdx.x < n) {
+      const long long r = r0 + threadIdx.x, qi = r / a.group;
       const long long at = (f.q0 + qi) * a.heads + hk * a.group + (r - qi * a.group);
       lse = a.lse[at]; delta = a.delta[at];
     }
   };
-  auto put = [&](int buf) {
-    qs.put(smem + buf * 2 * TB);
-    gs.put(smem + buf * 2 * TB + TB);
+  auto settle = [&](int buf) {
+    auto on = [&](int r) { return r < there_next; };
+    char* to = smem + buf * 2 * TB;
+    ql.settle(to, on, there_next == BM);
+    gl.settle(to + TB, on, there_next == BM);
     if ((int)threadIdx.x < BM) { srow[buf][0][threadIdx.x] = lse; srow[buf][1][threadIdx.x] = delta; }
   };
-  if (t0 < t1) { fetch(t0); put(0); }
+  if (t0 < t1) { load(t0, 0); settle(0); }
   __syncthreads();
   int buf = 0;
   for (int t = t0; t < t1; ++t) {
     const bool more = t + 1 < t1;
-    if (more) fetch(t + 1);
+    if (more) load(t + 1, buf ^ 1);
     const char* tq = smem + buf * 2 * TB;
     const char* tg = tq + TB;
 #pragma unroll
@@ -298,7 +328,7 @@ __global__ __launch_bounds__(256) void k_xa_dkv(XaArgs a) {
         }
       }
     }
-    if (more) put(buf ^ 1);
+    if (more) settle(buf ^ 1);
     __syncthreads();
     buf ^= 1;
   }
@@ -342,7 +372,7 @@ static XaBackward xa_backward_plan(const glx_attention* t) {
   const int group = t->heads / t->kv_heads, fr = t->frames > 0 ? t->frames : 1;
   const bool counts = t->q_cnt != nullptr;
   const long long rows = t->q_rows * group / fr, keys = t->k_rows / fr;
-  p.rw = rows <= 128 ? 1 : 4;
+  p.rw = rows <= 128 ? (t->dtype == GLX_F32 && t->dim > 64 ? 2 : 1) : 4;       // as in the forward pass
   p.qtiles = xa_tiles(t->q_rows * group, t->frames, (int)(t->q_len * group), counts, p.rw * 32);
   p.ktiles = xa_tiles(t->k_rows, t->frames, (int)t->k_len, counts, 128);
   p.qsplits = xa_splits((counts ? t->q_rows * group / (p.rw * 32) + 1 : p.qtiles) * t->kv_heads, keys);
@@ -364,7 +394,8 @@ static void xa_launch_backward(const XaBackward& p, XaArgs& a, char* ws, hipStre
     const dim3 grid((unsigned)(p.qtiles * p.qsplits), a.kvheads);
     a.splits = p.qsplits;
     a.part = (float*)(ws + p.qpart);
-    if (p.rw == 1) hipLaunchKernelGGL((k_xa_dq<T, DP, 1>), grid, dim3(256), 0, st, a);
+    constexpr int SMALL = sizeof(T) == 4 && DP > 64 ? 2 : 1;
+    if (p.rw == SMALL) hipLaunchKernelGGL((k_xa_dq<T, DP, SMALL>), grid, dim3(256), 0, st, a);
     else hipLaunchKernelGGL((k_xa_dq<T, DP, 4>), grid, dim3(256), 0, st, a);
     if (a.dq && p.qsplits > 1) {
       const long long n = a.nq * a.heads * a.dim, blocks = (n + 1023) / 1024;
@@ -404,6 +435,7 @@ extern "C" int glx_attention_backward(const glx_attention* t, const void* grad_o
   XaArgs a = xa_args(t);
   a.go = grad_out; a.sg = g_stride; a.hg = g_head_stride;
   a.dq = dq; a.dk = dk; a.dv = dv;
+  a.dma |= xa_chunked(grad_out, g_stride, g_head_stride, a.dim, t->dtype) << 3;
   a.delta = (float*)workspace;
   hipStream_t st = (hipStream_t)stream;
   if (t->dtype == GLX_F32) xa_backward_of<float>(p, a, (char*)workspace, st);
