@@ -33,6 +33,12 @@ struct XaArgs {
   float scale, scale2;              // scale2 = scale log2(e)
 };
 
+// waves per SIMD that the registers are kept for: two where LDS holds two blocks (else the compiler takes all 512 for one)
+template <typename T, int DP>
+constexpr int xa_waves(int row_waves) {
+  return 4 * (row_waves == 1 ? 128 : 64) * DP * (int)sizeof(T) <= 80 * 1024 ? 2 : 1;
+}
+
 // ------------------------------------------------------------------------------------------------ operands
 template <typename T> struct XaFrag { typedef T vec __attribute__((ext_vector_type(8))); };
 
@@ -183,7 +189,7 @@ struct XaPlace { long long q0, k0; int nq, nk, tile; };      // tile: index with
 
 // which frame holds the tile `t` when every frame has ceil(size / unit) tiles, size = its rows (queries x G) or its keys; the
 // rows behind the last frame count as a frame whose other side is empty.  Counts are clamped into the tensors.
-__device__ __forceinline__ XaPlace xa_place(const XaArgs& a, long long t, int unit, bool keys) {
+__device__ __forceinline__ XaPlace xa_find(const XaArgs& a, long long t, int unit, bool keys) {
   XaPlace p = {0, 0, 0, 0, -1};
   if (!a.qcnt) {
     const long long size = keys ? a.lk : (long long)a.lq * a.group, per = (size + unit - 1) / unit;
@@ -236,6 +242,17 @@ __device__ __forceinline__ XaPlace xa_place(const XaArgs& a, long long t, int un
   p.q0 = q0; p.k0 = k0; p.tile = (int)(t - tiles0);
   (keys ? p.nk : p.nq) = (int)left;
   return p;
+}
+
+__device__ __forceinline__ long long xa_uniform(long long v) {
+  const unsigned lo = __builtin_amdgcn_readfirstlane((unsigned)v), hi = __builtin_amdgcn_readfirstlane((unsigned)((unsigned long long)v >> 32));
+  return (long long)((unsigned long long)hi << 32 | lo);
+}
+// xa_find in scalar registers: what follows from the place -- bases, loop bounds, branches -- is then the wave's, not a lane's
+__device__ __forceinline__ XaPlace xa_place(const XaArgs& a, long long t, int unit, bool keys) {
+  const XaPlace p = xa_find(a, t, unit, keys);
+  return {xa_uniform(p.q0), xa_uniform(p.k0), __builtin_amdgcn_readfirstlane(p.nq), __builtin_amdgcn_readfirstlane(p.nk),
+          __builtin_amdgcn_readfirstlane(p.tile)};
 }
 
 // bit j: key k0 + j exists (j < n) and is not masked; the same in every lane

@@ -10,7 +10,7 @@
 #include "glx_attention.h"
 
 template <typename T, int DP, int RW>
-__global__ __launch_bounds__(256) void k_xa_forward(XaArgs a) {
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(xa_waves<T, DP>(RW)))) void k_xa_forward(XaArgs a) {
   constexpr int KW = 4 / RW, BN = KW == 4 ? 128 : 64, SUB = BN / 32 / KW;          // keys of a staged tile, of them 32 SUB a wave's
   constexpr int KS = DP / 16, DT = DP / 32;
   typedef XaTile<T, DP> Tile;
@@ -19,7 +19,7 @@ __global__ __launch_bounds__(256) void k_xa_forward(XaArgs a) {
   constexpr int BYTES = 4 * TB > JB ? 4 * TB : JB;
   __shared__ __attribute__((aligned(16))) char smem[BYTES];
   __shared__ float sm[4][32], sl[4][32];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5, l32 = lane & 31;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5, l32 = lane & 31;
   const int rw = wave / KW, kw = wave % KW;
   const int hk = blockIdx.y;
   const int split = blockIdx.x % a.splits;

@@ -54,7 +54,7 @@ __device__ __forceinline__ float xa_unrange(int e) {
 
 // ------------------------------------------------------------------------------------------------ dQ, delta
 template <typename T, int DP, int RW>
-__global__ __launch_bounds__(256) void k_xa_dq(XaArgs a) {
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(xa_waves<T, DP>(RW)))) void k_xa_dq(XaArgs a) {
   constexpr int KW = 4 / RW, BN = KW == 4 ? 128 : 64, SUB = BN / 32 / KW;
   constexpr int KS = DP / 16, DT = DP / 32;
   typedef XaTile<T, DP> Tile;
@@ -62,7 +62,7 @@ __global__ __launch_bounds__(256) void k_xa_dq(XaArgs a) {
   constexpr int JB = KW > 1 ? 4 * 32 * (DP + 1) * 4 : 0;
   constexpr int BYTES = 4 * TB > JB ? 4 * TB : JB;
   __shared__ __attribute__((aligned(16))) char smem[BYTES];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5, l32 = lane & 31;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5, l32 = lane & 31;
   const int rw = wave / KW, kw = wave % KW;
   const int hk = blockIdx.y;
   const int split = blockIdx.x % a.splits;
@@ -213,7 +213,7 @@ __global__ __launch_bounds__(256) void k_xa_dkv(XaArgs a) {
   constexpr int TB = BM * Tile::LD;
   __shared__ __attribute__((aligned(16))) char smem[2 * 2 * TB];
   __shared__ __attribute__((aligned(16))) float srow[2][2][BM];         // stage; lse, delta
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5, l32 = lane & 31;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5, l32 = lane & 31;
   const int hk = blockIdx.y;
   const int split = blockIdx.x % a.splits;
   const XaPlace f = xa_place(a, blockIdx.x / a.splits, 128, true);
