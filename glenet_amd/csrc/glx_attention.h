@@ -116,6 +116,12 @@ __device__ __forceinline__ typename XaFrag<T>::vec xa_row(const T* p, int d, int
   return v;
 }
 
+// The compiler places an operand's read in front of its product and waits for it there; with one or two waves per SIMD that
+// leaves the matrix units idle most of the time.  So the loops below are written as steps -- one or two products, the reads for
+// the step XA_AHEAD later, a share of the exponentials -- that are not reordered among each other.
+#define XA_AHEAD 2
+#define XA_STEP() __builtin_amdgcn_sched_barrier(0)
+
 // ------------------------------------------------------------------------------------------------ staging
 // ROWS rows of a tensor into a tile.  Rows that are whole 16-byte chunks go straight from memory to LDS (no registers, no LDS
 // writes; a lane fetches the chunk that belongs at its place): `place` keeps the thread's offsets within a tile, `issue` starts the
@@ -141,19 +147,19 @@ struct XaLoad {
   template <typename F, typename V>
   __device__ __forceinline__ void issue(char* tile, const T* base, F rowoff, V valid, int n, int D, bool dma) const {
     if (dma) {
-      char* to = tile + __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6) * 1024;
-      if (n >= ROWS) {
+      const unsigned to = (unsigned)(unsigned long long)(const __attribute__((address_space(3))) char*)tile + (threadIdx.x >> 6) * 1024;
 #pragma unroll
-        for (int i = 0; i < N; ++i)
-          __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)((const char*)base + (unsigned)off[i]),
-                                           (__attribute__((address_space(3))) void*)(to + i * 4096), 16, 0, 0);
-      } else {
-#pragma unroll
-        for (int i = 0; i < N; ++i) {
+      for (int i = 0; i < N; ++i) {
+        int o = off[i];
+        if (n < ROWS) {
           const int r = row_of(i) < n ? row_of(i) : n - 1, c = chunk_of(i) * E < D ? chunk_of(i) * E : 0;
-          __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(base + rowoff(r) + c),
-                                           (__attribute__((address_space(3))) void*)(to + i * 4096), 16, 0, 0);
+          o = (int)((rowoff(r) + c) * (int)sizeof(T));
         }
+        // (no register is written, and the compiler, which would wait for all transfers in front of any transposing read, does
+        // not see them: `settle` waits.  64 lanes x 16 bytes from base + o to LDS at the wave's place.)
+        asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1"
+                     ::"v"(o), "s"(base), "s"(__builtin_amdgcn_readfirstlane(to + i * 4096))
+                     : "memory", "m0");
       }
     } else {
 #pragma unroll 1

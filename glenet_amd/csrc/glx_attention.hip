@@ -242,17 +242,23 @@ int xa_splits(long long blocks, long long keys_per_frame) {
   s = s < most ? s : most;
   return (int)(s < 1 ? 1 : (s > 256 ? 256 : s));
 }
+// row tiles of four waves, or of one (two: fp32 heads beyond 64, the keys of four waves do not fit LDS twice) where the large
+// ones would leave compute units without work even when the keys are split; `rw`, tiles, splits over `keys` states per frame
+void xa_rows_plan(const glx_attention* t, int* rw, long long* tiles, int* splits) {
+  const int group = t->heads / t->kv_heads, fr = t->frames > 0 ? t->frames : 1, small = t->dtype == GLX_F32 && t->dim > 64 ? 2 : 1;
+  const bool counts = t->q_cnt != nullptr;
+  const long long keys = t->k_rows / fr, rows = t->q_rows * group;
+  for (*rw = 4;; *rw = small) {
+    *tiles = xa_tiles(rows, t->frames, (int)(t->q_len * group), counts, *rw * 32);
+    const long long blocks = (counts ? rows / (*rw * 32) + 1 : *tiles) * t->kv_heads;
+    *splits = xa_splits(blocks, keys);
+    if (*rw == small || (rows > 64 * fr && blocks * *splits >= 256)) return;
+  }
+}
 struct XaForward { int rw, splits; long long tiles; };
 static XaForward xa_forward_plan(const glx_attention* t) {
   XaForward p;
-  const int group = t->heads / t->kv_heads;
-  const bool counts = t->q_cnt != nullptr;
-  const long long rows = counts ? t->q_rows * group / (t->frames > 0 ? t->frames : 1) : (long long)t->q_len * group;
-  // (fp32 rows beyond 64: the keys of four waves do not fit LDS twice)
-  p.rw = rows <= 64 ? (t->dtype == GLX_F32 && t->dim > 64 ? 2 : 1) : 4;
-  p.tiles = xa_tiles(t->q_rows * group, t->frames, (int)(t->q_len * group), counts, p.rw * 32);
-  const long long blocks = (counts ? t->q_rows * group / (p.rw * 32) + 1 : p.tiles) * t->kv_heads;
-  p.splits = xa_splits(blocks, t->frames > 0 ? t->k_rows / t->frames : 0);
+  xa_rows_plan(t, &p.rw, &p.tiles, &p.splits);
   return p;
 }
 

@@ -14,9 +14,12 @@
 // later tile would pass it).
 #include "glx_attention.h"
 
+#include <type_traits>
+
 #define XA_PSCALE 4096.f      // fp16: of P
 
 int xa_splits(long long blocks, long long keys_per_frame);
+void xa_rows_plan(const glx_attention* t, int* rw, long long* tiles, int* splits);
 int xa_check(const char* who, const glx_attention* t);
 XaArgs xa_args(const glx_attention* t);
 
@@ -207,7 +210,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(xa_waves<T,
 // ------------------------------------------------------------------------------------------------ dK, dV
 template <typename T, int DP>
 __global__ __launch_bounds__(256) void k_xa_dkv(XaArgs a) {
-  constexpr int BM = sizeof(T) == 2 ? 64 : 32;
+  constexpr int BM = sizeof(T) == 2 ? 64 : 32, PARTS = BM / 32;
   constexpr int KS = DP / 16, DT = DP / 32;
   typedef XaTile<T, DP> Tile;
   constexpr int TB = BM * Tile::LD;
@@ -289,42 +292,79 @@ __global__ __launch_bounds__(256) void k_xa_dkv(XaArgs a) {
   if (t0 < t1) { load(t0, 0); settle(0); }
   __syncthreads();
   int buf = 0;
+  auto sweep = [&](auto masked) {
+  constexpr bool MASKED = decltype(masked)::value;
   for (int t = t0; t < t1; ++t) {
     const bool more = t + 1 < t1;
     if (more) load(t + 1, buf ^ 1);
     const char* tq = smem + buf * 2 * TB;
     const char* tg = tq + TB;
-#pragma unroll
-    for (int u = 0; u < BM / 32; ++u) {
-      xf16 s = (xf16)(0.f), d = (xf16)(0.f);
-#pragma unroll
-      for (int k = 0; k < KS; ++k) {
-        xa_mma(s, xa_along<T, DP>(tq, u * 32 + l32, k, half), K[k]);
-        xa_mma(d, xa_along<T, DP>(tg, u * 32 + l32, k, half), V[k]);
-      }
+    xf16 s[PARTS], d[PARTS];
+    xf4 ls[4], de[4];
+    auto stats = [&](int u) {
 #pragma unroll
       for (int g = 0; g < 4; ++g) {
-        const xf4 ls = *reinterpret_cast<const xf4*>(&srow[buf][0][u * 32 + g * 8 + half * 4]);
-        const xf4 de = *reinterpret_cast<const xf4*>(&srow[buf][1][u * 32 + g * 8 + half * 4]);
+        ls[g] = *reinterpret_cast<const xf4*>(&srow[buf][0][u * 32 + g * 8 + half * 4]);
+        de[g] = *reinterpret_cast<const xf4*>(&srow[buf][1][u * 32 + g * 8 + half * 4]);
+      }
+    };
+    auto weigh = [&](int u, int i) {
+      const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[u][i], a.scale2, -ls[i >> 2][i & 3]));
+      const float q = p * (d[u][i] - de[i >> 2][i & 3]);
+      s[u][i] = MASKED && !valid ? 0.f : __is_same(T, _Float16) ? p * XA_PSCALE : p;
+      d[u][i] = MASKED && !valid ? 0.f : q;
+    };
+    // steps: the two score products of part u, k by k; its two gradient products, eight rows and 32 channels at a time.  Part u's
+    // scores are weighed beside the products that follow them
+    constexpr int GS = 2 * DT, STEPS = PARTS * (KS + GS);
+    typename XaFrag<T>::vec ring[XA_AHEAD + 1][2];
+    auto read = [&](int n) {
+      const int r = n % (XA_AHEAD + 1);
+      if (n < PARTS * KS) {
+        const int row = n / KS * 32 + l32;
+        ring[r][0] = xa_along<T, DP>(tq, row, n % KS, half);
+        ring[r][1] = xa_along<T, DP>(tg, row, n % KS, half);
+      } else {
+        const int g = n - PARTS * KS, row = g / GS * 32 + g % GS / DT * 16;
+        ring[r][0] = xa_down<T, DP>(tg, row, g % DT * 32, lane);
+        ring[r][1] = xa_down<T, DP>(tq, row, g % DT * 32, lane);
+      }
+    };
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[g * 4 + i], a.scale2, -ls[i]));
-          s[g * 4 + i] = valid ? p : 0.f;
-          d[g * 4 + i] = valid ? p * (d[g * 4 + i] - de[i]) : 0.f;
+    for (int n = 0; n < XA_AHEAD; ++n) read(n);
+    typename XaFrag<T>::vec p, q;
+#pragma unroll
+    for (int n = 0; n < STEPS; ++n) {
+      const int r = n % (XA_AHEAD + 1);
+      if (n + XA_AHEAD < STEPS) read(n + XA_AHEAD);
+      if (n == (PARTS > 1 ? KS - 1 : 0)) stats(0);
+      XA_STEP();
+      if (n < PARTS * KS) {
+        const int u = n / KS, k = n % KS;
+        if (k == 0) s[u] = d[u] = (xf16)(0.f);
+        xa_mma(s[u], ring[r][0], K[k]);
+        xa_mma(d[u], ring[r][1], V[k]);
+        if (u > 0) {
+#pragma unroll
+          for (int i = k * 16 / KS; i < (k + 1) * 16 / KS; ++i) weigh(u - 1, i);
         }
-      }
-      if constexpr (__is_same(T, _Float16)) {
+      } else {
+        const int g = n - PARTS * KS, u = g / GS, j = g % GS;
+        if (g == 0) {
+          if (PARTS == 1) {
 #pragma unroll
-        for (int i = 0; i < 16; ++i) s[i] *= XA_PSCALE;
-      }
-      xa_range<T, DT>(d, dK, e);
+            for (int i = 0; i < 16; ++i) weigh(0, i);
+          } else {
+            stats(1);
+          }
+        }
+        if (j == 0) xa_range<T, DT>(d[u], dK, e);
+        if (j % DT == 0) { p = xa_pack<T>(s[u], j / DT); q = xa_pack<T>(d[u], j / DT); }
+        xa_mma(dV[j % DT], ring[r][0], p);
+        xa_mma(dK[j % DT], ring[r][1], q);
+        if (PARTS > 1 && u == 0) {
 #pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        const typename XaFrag<T>::vec p = xa_pack<T>(s, c), q = xa_pack<T>(d, c);
-#pragma unroll
-        for (int i = 0; i < DT; ++i) {
-          xa_mma(dV[i], xa_down<T, DP>(tg, u * 32 + c * 16, i * 32, lane), p);
-          xa_mma(dK[i], xa_down<T, DP>(tq, u * 32 + c * 16, i * 32, lane), q);
+          for (int i = j * 16 / GS; i < (j + 1) * 16 / GS; ++i) weigh(PARTS - 1, i);
         }
       }
     }
@@ -332,6 +372,10 @@ __global__ __launch_bounds__(256) void k_xa_dkv(XaArgs a) {
     __syncthreads();
     buf ^= 1;
   }
+  };
+  // (all waves of the block take the same way: they meet at the barriers inside)
+  if (__syncthreads_and(valid)) sweep(std::false_type());
+  else sweep(std::true_type());
   if (!there) return;
   const float ksize = a.scale * xa_unrange<T>(e), vsize = __is_same(T, _Float16) ? 1.f / XA_PSCALE : 1.f;
   const long long at = (f.k0 + key) * a.kvheads + hk, n = a.nk * a.kvheads * a.dim;
@@ -371,11 +415,9 @@ static XaBackward xa_backward_plan(const glx_attention* t) {
   XaBackward p;
   const int group = t->heads / t->kv_heads, fr = t->frames > 0 ? t->frames : 1;
   const bool counts = t->q_cnt != nullptr;
-  const long long rows = t->q_rows * group / fr, keys = t->k_rows / fr;
-  p.rw = rows <= 128 ? (t->dtype == GLX_F32 && t->dim > 64 ? 2 : 1) : 4;       // as in the forward pass
-  p.qtiles = xa_tiles(t->q_rows * group, t->frames, (int)(t->q_len * group), counts, p.rw * 32);
+  const long long rows = t->q_rows * group / fr;
+  xa_rows_plan(t, &p.rw, &p.qtiles, &p.qsplits);
   p.ktiles = xa_tiles(t->k_rows, t->frames, (int)t->k_len, counts, 128);
-  p.qsplits = xa_splits((counts ? t->q_rows * group / (p.rw * 32) + 1 : p.qtiles) * t->kv_heads, keys);
   p.ksplits = xa_splits((counts ? t->k_rows / 128 + 1 : p.ktiles) * t->kv_heads, rows);
   p.delta = 0;
   p.qpart = glx_align((size_t)t->q_rows * t->heads * sizeof(float));
