@@ -22,8 +22,8 @@
 #include <vector>
 
 #define NS_K 64                // the k range of a split comes in multiples of this
-#define NS_OPS 32              // products of one launch (kernel arguments: 120 bytes each)
-#define NS_MATS 36             // matrices of one prologue launch
+#define NS_OPS 39              // products of one launch (kernel arguments: 96 bytes each)
+#define NS_MATS 40             // matrices of one prologue launch
 #define NS_STEPS 64            // at most
 #define NS_PARTS 1024          // partial sums of squares per matrix, at most
 
@@ -34,34 +34,38 @@ typedef float nf4 __attribute__((ext_vector_type(4)));
 
 enum { NS_PLANES, NS_PARTIAL, NS_XPLANES, NS_FINAL };
 
-// out = epilogue(alpha A B^T): A (mp, K), B (np, K) planes, lo plane behind the hi plane
+// out = epilogue(alpha A B^T): A (mp, K), B (np, K) planes, lo plane behind the hi plane.  Places in the workspace in units of
+// 256 bytes, 0: none (the first unit stays empty)
 struct NsOp {
-  const _Float16* a; const _Float16* b;
-  const _Float16* d;           // NS_PLANES: + beta D, D (mp, mp) planes, or NULL
-  void* out; void* out2;       // NS_PLANES: planes (mp, mp); NS_PARTIAL: fp32 [splits][mp][mp]; NS_XPLANES: planes (mp, np) and
-                               // their transpose (np, mp); NS_FINAL: the caller's matrix
-  const float* xin; const float* xout;      // device scales of the X planes that are read (`xpow` of the operands) / written
+  unsigned a, b, d;            // d: NS_PLANES: + beta D, D (mp, mp) planes
+  unsigned out, out2;          // NS_PLANES: planes (mp, mp); NS_PARTIAL: fp32 [splits][mp][mp]; NS_XPLANES: planes (mp, np) and
+                               // their transpose (np, mp)
+  unsigned xin, xout;          // scales of the X planes that are read (`xpow` of the operands) / written, floats
   float alpha, beta, diag, scale;
-  int mp, np, K, kper;         // kper: k elements of a split
-  int m, n;
+  int mp, np, K, m, n;
   long long ldd;               // NS_FINAL: elements between the caller's rows
-  int block0;
-  short splits;
-  unsigned char kind, sym, tall, dtype, xpow;
+  void* dst;                   // ... its matrix
+  unsigned short splits, kper; // kper: k elements of a split, in NS_K
+  unsigned char kind, sym, tall, dtype, xpow, xstep, xnext;
 };
-struct NsOps { NsOp op[NS_OPS]; int count; };
+struct NsOps { int first[NS_OPS]; NsOp op[NS_OPS]; int count; char* ws; };       // first[k]: first block of op k
 
 struct NsMat {
   const void* src; long long ld;       // the caller's matrix, `rows` x `cols`
   _Float16* x; _Float16* xt;           // planes (mp, np) and (np, mp)
   double* parts; float* xscale;        // sums of squares; the scale of X's planes in front of every step
   int rows, cols, mp, np, tall, nparts;
-  int block0, tblock0;                 // first block of the norm launch / of the plane launch
 };
 // xb[s], qb[s]: bounds of |X| in front of step s, and of |X| / |X_0|
-struct NsMats { NsMat mat[NS_MATS]; int count, dtype, steps; double eps; float xb[NS_STEPS], qb[NS_STEPS]; };
-static_assert(sizeof(NsMats) <= 4000 && sizeof(NsOps) <= 4000, "kernel arguments");
+struct NsMats { int first[NS_MATS], tfirst[NS_MATS]; NsMat mat[NS_MATS]; int count, dtype, steps; double eps; float xb[NS_STEPS], qb[NS_STEPS]; };
+static_assert(sizeof(NsMats) <= 4032 && sizeof(NsOps) <= 4032, "kernel arguments");
 
+// the entry whose blocks hold this one: the first blocks side by side, one read for a wave (kernel arguments lie in host memory;
+// a search through the entries themselves costs a round trip each)
+__device__ __forceinline__ int ns_entry(const int* first, int count) {
+  const int lane = threadIdx.x & 63;
+  return __popcll(__ballot(lane < count && (int)blockIdx.x >= first[lane < count ? lane : 0])) - 1;
+}
 __device__ __forceinline__ void ns_split(float v, _Float16& hi, _Float16& lo) {
   hi = (_Float16)v;
   lo = (_Float16)(v - (float)hi);
@@ -72,10 +76,9 @@ __device__ __forceinline__ float ns_elem(const void* p, long long i, int dtype) 
 
 // ------------------------------------------------------------------------------------------------ |G|_F and the planes of X
 __global__ __launch_bounds__(256) void k_ns_norm(NsMats s) {
-  int k = 0;
-  while (k + 1 < s.count && (int)blockIdx.x >= s.mat[k + 1].block0) ++k;
+  const int k = ns_entry(s.first, s.count);
   const NsMat& t = s.mat[k];
-  const int part = blockIdx.x - t.block0;
+  const int part = blockIdx.x - s.first[k];
   double sum = 0.0;
   auto add = [&](auto* src) {
     typedef GlxVec<__remove_cvref(decltype(*src)), 4> V;
@@ -113,8 +116,7 @@ __global__ __launch_bounds__(256) void k_ns_norm(NsMats s) {
 __global__ __launch_bounds__(256) void k_ns_planes(NsMats s) {
   __shared__ float tile[64][65];
   __shared__ double red[256];
-  int k = 0;
-  while (k + 1 < s.count && (int)blockIdx.x >= s.mat[k + 1].tblock0) ++k;
+  const int k = ns_entry(s.tfirst, s.count);
   const NsMat& t = s.mat[k];
   double mine = 0.0;
   for (int i = threadIdx.x; i < t.nparts; i += 256) mine += t.parts[i];
@@ -124,7 +126,7 @@ __global__ __launch_bounds__(256) void k_ns_planes(NsMats s) {
     if ((int)threadIdx.x < o) red[threadIdx.x] += red[threadIdx.x + o];
     __syncthreads();
   }
-  const int b = blockIdx.x - t.tblock0, tiles_n = t.np / 64;
+  const int b = blockIdx.x - s.tfirst[k], tiles_n = t.np / 64;
   const double norm = sqrt(red[0]), rho = norm / (norm + s.eps);
   // the planes hold G 2^k with |G| 2^k in [2^14, 2^15): 16-bit values exactly, in the hi plane alone
   const int k0 = norm > 0.0 ? 14 - ilogb(norm) : 60, kx = k0 > 120 ? 120 : (k0 < -120 ? -120 : k0);
@@ -169,19 +171,21 @@ __global__ __launch_bounds__(256) void k_ns_planes(NsMats s) {
 }
 
 // ------------------------------------------------------------------------------------------------ the products
-// A block forms a TILE x TILE tile with four waves of (TILE / 2)^2, k in steps of KS through two LDS stages; the order of a
+// A block forms a TILE x TILE tile with four waves of (TILE / 2)^2, k in steps of KS that go from memory to LDS without registers,
+// several ahead (small products are all latency: four stages bring 256 x 256 in one round trip, 8.9 -> XX us); the order of a
 // staged row's 16-byte chunks is rotated by the row, so that the 32 rows an operand read touches spread over the banks.  PROD
 // products per pair of operands: 3 both split, 2 where B's lo plane is empty, 1 where neither is used.
 template <int TILE, int PROD>
 __global__ __launch_bounds__(256) void k_ns_gemm(NsOps s) {
   constexpr int KS = TILE == 64 ? 64 : 32, C = KS / 8, RB = KS * 2;  // k elements of a stage, its chunks and bytes per row
+  constexpr int STAGES = TILE == 64 ? 4 : 2;
   constexpr int PA = PROD > 1 ? 2 : 1, PB = PROD > 2 ? 2 : 1;        // planes of the operands
   constexpr int W = TILE / 2, F = W / 32, CH = TILE * C / 256;       // a wave's tile, its 32-wide parts, chunks per thread and plane
-  __shared__ __attribute__((aligned(16))) char smem[2][PA + PB][TILE * RB];          // stage, plane
-  int k = 0;
-  while (k + 1 < s.count && (int)blockIdx.x >= s.op[k + 1].block0) ++k;
-  const NsOp& t = s.op[k];
-  int b = blockIdx.x - t.block0;
+  constexpr int LOADS = (PA + PB) * CH;                              // transfers per wave and stage
+  __shared__ __attribute__((aligned(16))) char smem[STAGES][PA + PB][TILE * RB];
+  const int entry = ns_entry(s.first, s.count);
+  const NsOp& t = s.op[entry];
+  int b = blockIdx.x - s.first[entry];
   const int tm = t.mp / TILE, tn = t.np / TILE;
   const int per = t.sym ? tm * (tm + 1) / 2 : tm * tn, split = b / per;
   b -= split * per;
@@ -194,45 +198,48 @@ __global__ __launch_bounds__(256) void k_ns_gemm(NsOps s) {
   } else {
     ti = b / tn; tj = b - ti * tn;
   }
-  const float xin = t.xin ? t.xin[0] : 1.f, alpha = t.alpha / (t.xpow == 2 ? xin * xin : xin), scale = t.xout ? t.xout[0] : t.scale;
-  const int k0 = split * t.kper, k1 = k0 + t.kper < t.K ? k0 + t.kper : t.K;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wi = wave >> 1, wj = wave & 1, half = lane >> 5, l32 = lane & 31;
+  auto at = [&](unsigned place) { return s.ws + (size_t)place * 256; };
+  const float xin = t.xin ? ((const float*)at(t.xin))[t.xstep] : 1.f, alpha = t.alpha / (t.xpow == 2 ? xin * xin : xin), scale = t.xout ? ((const float*)at(t.xout))[t.xnext] : t.scale;
+  const int kper = t.kper * NS_K, k0 = split * kper, k1 = k0 + kper < t.K ? k0 + kper : t.K;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wi = wave >> 1, wj = wave & 1, half = lane >> 5, l32 = lane & 31;
   const _Float16* src[PA + PB];
 #pragma unroll
-  for (int p = 0; p < PA; ++p) src[p] = t.a + ((long long)p * t.mp + ti * TILE) * t.K;
+  for (int p = 0; p < PA; ++p) src[p] = (const _Float16*)at(t.a) + ((long long)p * t.mp + ti * TILE) * t.K;
 #pragma unroll
-  for (int p = 0; p < PB; ++p) src[PA + p] = t.b + ((long long)p * t.np + tj * TILE) * t.K;
-  nh8 stage[PA + PB][CH];
+  for (int p = 0; p < PB; ++p) src[PA + p] = (const _Float16*)at(t.b) + ((long long)p * t.np + tj * TILE) * t.K;
   auto place = [](int r, int ch) { return r * RB + (C == 8 ? (ch ^ r) & 7 : (ch ^ (r >> 1)) & 3) * 16; };
-  auto fetch = [&](int kk) {
+  // memory -> LDS: a lane fetches the chunk that belongs at its place (the compiler does not see these transfers: `arrived`)
+  int off[CH];
+#pragma unroll
+  for (int c = 0; c < CH; ++c) {
+    const int q = threadIdx.x + c * 256, r = q / C, ch = C == 8 ? (q ^ r) & 7 : (q ^ (r >> 1)) & 3;
+    off[c] = (r * t.K + ch * 8) * 2;
+  }
+  auto fetch = [&](int n) {
+    const unsigned to = (unsigned)(unsigned long long)(__attribute__((address_space(3))) char*)smem[n % STAGES][0] + (wave << 10);
 #pragma unroll
     for (int p = 0; p < PA + PB; ++p)
 #pragma unroll
-      for (int c = 0; c < CH; ++c) {
-        const int q = threadIdx.x + c * 256;
-        stage[p][c] = *reinterpret_cast<const nh8*>(src[p] + (long long)(q / C) * t.K + kk + (q % C) * 8);
-      }
-  };
-  auto put = [&](int buf) {
-#pragma unroll
-    for (int p = 0; p < PA + PB; ++p)
-#pragma unroll
-      for (int c = 0; c < CH; ++c) {
-        const int q = threadIdx.x + c * 256;
-        *reinterpret_cast<nh8*>(&smem[buf][p][place(q / C, q % C)]) = stage[p][c];
-      }
+      for (int c = 0; c < CH; ++c)
+        asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1"
+                     ::"v"(off[c]), "s"(src[p] + k0 + n * KS), "s"(to + p * (TILE * RB) + c * 4096)
+                     : "memory", "m0");
   };
   nf16 acc[F][F];
 #pragma unroll
   for (int i = 0; i < F; ++i)
 #pragma unroll
     for (int j = 0; j < F; ++j) acc[i][j] = (nf16)(0.f);
-  if (k0 < k1) { fetch(k0); put(0); }
-  __syncthreads();
-  int buf = 0;
-  for (int kk = k0; kk < k1; kk += KS) {
-    const bool more = kk + KS < k1;
-    if (more) fetch(kk + KS);
+  const int stages = (k1 - k0) / KS;
+  for (int n = 0; n < STAGES && n < stages; ++n) fetch(n);
+  for (int n = 0; n < stages; ++n) {
+    // stage n is there once at most the later ones are on their way; its slot's last readers have passed the barrier of n - 1
+    if (n == 0 && stages >= STAGES) asm volatile("s_waitcnt vmcnt(%0)" ::"n"((STAGES - 1) * LOADS) : "memory");
+    else if (n > 0 && n + STAGES - 2 < stages) asm volatile("s_waitcnt vmcnt(%0)" ::"n"((STAGES - 2) * LOADS) : "memory");
+    else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+    if (n > 0 && n + STAGES - 1 < stages) fetch(n + STAGES - 1);
+    const int buf = n % STAGES;
 #pragma unroll
     for (int ks = 0; ks < KS / 16; ++ks) {
       nh8 fa[PA][F], fb[PB][F];
@@ -253,86 +260,98 @@ __global__ __launch_bounds__(256) void k_ns_gemm(NsOps s) {
           acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fa[0][i], fb[0][j], acc[i][j], 0, 0, 0);
         }
     }
-    if (more) put(buf ^ 1);
-    __syncthreads();
-    buf ^= 1;
   }
   // a lane's accumulators: column l32, rows 8 g + 4 half + 0..3 of the 32 x 32 part
 #pragma unroll
   for (int i = 0; i < F; ++i)
 #pragma unroll
-    for (int j = 0; j < F; ++j)
+    for (int j = 0; j < F; ++j) {
+      const int row0 = ti * TILE + wi * W + i * 32 + half * 4, col = tj * TILE + wj * W + j * 32 + l32;
+      if (t.kind == NS_PARTIAL) {
+        float* o = (float*)at(t.out) + (long long)split * t.mp * t.mp;
 #pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        const int row = ti * TILE + wi * W + i * 32 + g * 8 + half * 4, col = tj * TILE + wj * W + j * 32 + l32;
-        nf4 v;
+        for (int g = 0; g < 4; ++g)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] = acc[i][j][g * 4 + e] * alpha;
-        if (t.kind == NS_PARTIAL) {
-          float* o = (float*)t.out + (long long)split * t.mp * t.mp;
+          for (int e = 0; e < 4; ++e) o[(long long)(row0 + g * 8 + e) * t.mp + col] = acc[i][j][g * 4 + e] * alpha;
+      } else if (t.kind == NS_FINAL) {
 #pragma unroll
-          for (int e = 0; e < 4; ++e) o[(long long)(row + e) * t.mp + col] = v[e];
-        } else if (t.kind == NS_FINAL) {
+        for (int g = 0; g < 4; ++g)
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            if (row + e >= t.m || col >= t.n) continue;
-            const long long at = t.tall ? (long long)col * t.ldd + row + e : (long long)(row + e) * t.ldd + col;
-            if (t.dtype == GLX_F32) ((float*)t.out)[at] = v[e];
-            else if (t.dtype == GLX_BF16) ((__bf16*)t.out)[at] = (__bf16)v[e];
-            else ((_Float16*)t.out)[at] = (_Float16)v[e];
+            const int row = row0 + g * 8 + e;
+            if (row >= t.m || col >= t.n) continue;
+            const float v = acc[i][j][g * 4 + e] * alpha;
+            const long long to = t.tall ? (long long)col * t.ldd + row : (long long)row * t.ldd + col;
+            if (t.dtype == GLX_F32) ((float*)t.dst)[to] = v;
+            else if (t.dtype == GLX_BF16) ((__bf16*)t.dst)[to] = (__bf16)v;
+            else ((_Float16*)t.dst)[to] = (_Float16)v;
           }
-        } else {
-          const int ldo = t.kind == NS_PLANES ? t.mp : t.np;
-          const long long po = (long long)t.mp * ldo;
-          if (t.d) {
+      } else {
+        const int ldo = t.kind == NS_PLANES ? t.mp : t.np;
+        const long long po = (long long)t.mp * ldo;
+        float v[16];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const _Float16* d = t.d + (long long)(row + e) * t.mp + col;
-              v[e] += t.beta * ((float)d[0] + (float)d[(long long)t.mp * t.mp]);
-              if (row + e == col) v[e] += t.diag;
-            }
+        for (int e = 0; e < 16; ++e) v[e] = acc[i][j][e] * alpha;
+        if (t.d) {                                             // (D is symmetric: its column's four values lie side by side)
+          const _Float16* d = (const _Float16*)at(t.d) + (long long)col * t.mp + row0;
+          nh4 dh[4], dl[4];
+#pragma unroll
+          for (int g = 0; g < 4; ++g) {
+            dh[g] = *reinterpret_cast<const nh4*>(d + g * 8);
+            dl[g] = *reinterpret_cast<const nh4*>(d + (long long)t.mp * t.mp + g * 8);
           }
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            v[e] += t.beta * ((float)dh[e >> 2][e & 3] + (float)dl[e >> 2][e & 3]);
+            if (row0 + (e >> 2) * 8 + (e & 3) == col) v[e] += t.diag;
+          }
+        }
+        // the planes themselves, and X's transposed planes or a symmetric product's mirrored tile (the diagonal's holds both)
+        const bool own = t.kind == NS_XPLANES || ti != tj;
+        _Float16* o = (_Float16*)at(t.out);
+        _Float16* x = (_Float16*)at(t.kind == NS_XPLANES ? t.out2 : t.out) + (long long)col * t.mp + row0;
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
           nh4 h, l;
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             _Float16 u, w;
-            ns_split(v[e] * scale, u, w);
+            ns_split(v[g * 4 + e] * scale, u, w);
             h[e] = u; l[e] = w;
-            _Float16* o = (_Float16*)t.out + (long long)(row + e) * ldo + col;
-            o[0] = u; o[po] = w;
+            if (own) {
+              _Float16* to = o + (long long)(row0 + g * 8 + e) * ldo + col;
+              to[0] = u; to[po] = w;
+            }
           }
-          // the transpose: X's other planes, or the mirrored tile of a symmetric product
-          if (t.kind == NS_XPLANES || ti != tj) {
-            _Float16* o = (_Float16*)(t.kind == NS_XPLANES ? t.out2 : t.out) + (long long)col * t.mp + row;
-            *reinterpret_cast<nh4*>(o) = h;
-            *reinterpret_cast<nh4*>(o + po) = l;
-          }
+          *reinterpret_cast<nh4*>(x + g * 8) = h;
+          *reinterpret_cast<nh4*>(x + po + g * 8) = l;
         }
       }
+    }
 }
 
 // the splits' sum of a Gram matrix (tiles on and below the diagonal were formed) as planes of the whole matrix
 __global__ __launch_bounds__(256) void k_ns_join(NsOps s, int tile) {
-  int k = 0;
-  while (k + 1 < s.count && (int)blockIdx.x >= s.op[k + 1].block0) ++k;
+  const int k = ns_entry(s.first, s.count);
   const NsOp& t = s.op[k];
-  const long long e = (long long)(blockIdx.x - t.block0) * 256 + threadIdx.x, plane = (long long)t.mp * t.mp;
+  const long long e = (long long)(blockIdx.x - s.first[k]) * 256 + threadIdx.x, plane = (long long)t.mp * t.mp;
   if (e >= plane) return;
   int r = (int)(e / t.mp), c = (int)(e - (long long)r * t.mp);
   if (c / tile > r / tile) { const int x = r; r = c; c = x; }
-  const float* p = (const float*)t.a + (long long)r * t.mp + c;
+  const float* p = (const float*)(s.ws + (size_t)t.a * 256) + (long long)r * t.mp + c;
   float v = 0.f;
 #pragma unroll 8
   for (int q = 0; q < t.splits; ++q) v += p[q * plane];
   _Float16 u, w;
   ns_split(v * t.scale, u, w);
-  ((_Float16*)t.out)[e] = u;
-  ((_Float16*)t.out)[plane + e] = w;
+  _Float16* out = (_Float16*)(s.ws + (size_t)t.out * 256);
+  out[e] = u;
+  out[plane + e] = w;
 }
 
 // ------------------------------------------------------------------------------------------------ host: programs
 struct NsPlan {                // one matrix
-  int rows, cols, m, n, mp, np, tile, tall, seg, splits, kper, nparts;
+  int rows, cols, m, n, mp, np, tile, xtile, tall, seg, splits, kper, nparts;       // tile: of symmetric products, xtile: of Q X
   size_t x, xt, x2, xt2, g, h, p[2], q[2], part, parts, xscale;        // byte offsets in the workspace
 };
 struct NsBounds { double g, p, h, q; };       // of one step of a segment: spectral norms of A, P, H = P A and Q behind the step
@@ -365,9 +384,12 @@ static NsPlan ns_plan(int rows, int cols, int dtype, int steps, size_t& at) {
   NsPlan p = {};
   p.rows = rows; p.cols = cols; p.tall = rows > cols;
   p.m = p.tall ? cols : rows; p.n = p.tall ? rows : cols;
-  // 128-wide tiles once the symmetric products fill the card with them
-  p.tile = p.m > 2048 ? 128 : 64;
-  p.mp = ns_padded(p.m, p.tile); p.np = ns_padded(p.n, p.tile);
+  // 128-wide tiles where they still fill the card: they read half as much from LDS per product
+  const int pad = p.m > 1024 ? 128 : 64;
+  p.mp = ns_padded(p.m, pad); p.np = ns_padded(p.n, pad);
+  const long long wide = p.mp / 128, across = p.np / 128;
+  p.tile = pad == 128 && wide * (wide + 1) / 2 >= 200 ? 128 : 64;
+  p.xtile = pad == 128 && wide * across >= 200 ? 128 : 64;
   p.seg = dtype == GLX_BF16 ? 5 : 3;
   if (p.m <= 128 || (dtype == GLX_F32 ? p.n < 4ll * p.m : 4ll * p.n <= 5ll * p.m)) p.seg = 1;
   if (p.seg > steps) p.seg = steps;
@@ -404,7 +426,7 @@ static int ns_check(const char* who, const glx_matrix* mats, int count, int dtyp
 
 extern "C" size_t glx_orthogonalize_workspace_bytes(const glx_matrix* mats, int count, int dtype, int steps) {
   if (ns_check("glx_orthogonalize_workspace_bytes", mats, count, dtype, steps) != GLX_OK) return 0;
-  size_t at = 0;
+  size_t at = 256;
   for (int i = 0; i < count; ++i) ns_plan(mats[i].rows, mats[i].cols, dtype, steps, at);
   return at + 256;
 }
@@ -420,14 +442,15 @@ static void ns_launch_gemm(const NsOps& s, int blocks, int prods, hipStream_t st
   else if (prods == 2) hipLaunchKernelGGL((k_ns_gemm<TILE, 2>), dim3(blocks), dim3(256), 0, st, s);
   else hipLaunchKernelGGL((k_ns_gemm<TILE, 3>), dim3(blocks), dim3(256), 0, st, s);
 }
-static void ns_launch_ops(std::vector<NsOp>& ops, int tile, int prods, hipStream_t st) {       // prods = 0: joins
+static void ns_launch_ops(std::vector<NsOp>& ops, char* ws, int tile, int prods, hipStream_t st) {       // prods = 0: joins
   for (size_t i = 0; i < ops.size(); i += NS_OPS) {
     NsOps s;
     memset(&s, 0, sizeof(s));
+    s.ws = ws;
     int blocks = 0;
     for (size_t j = i; j < ops.size() && j < i + NS_OPS; ++j) {
+      s.first[s.count] = blocks;
       NsOp& o = s.op[s.count++] = ops[j];
-      o.block0 = blocks;
       const int tm = o.mp / tile, tn = o.np / tile;
       blocks += prods == 0 ? glx_divup((long long)o.mp * o.mp, 256) : (o.sym ? tm * (tm + 1) / 2 : tm * tn) * o.splits;
     }
@@ -449,8 +472,9 @@ extern "C" int glx_orthogonalize(const glx_matrix* mats, int count, int dtype, i
   GLX_REQUIRE(ns_bounds(steps, coefficients, lam, pmax, hmax),
               "glx_orthogonalize: these coefficients let singular values grow beyond the arithmetic's range");
   std::vector<NsPlan> plans;
-  size_t need = 0;
+  size_t need = 256;                                   // (place 0 means none)
   for (int i = 0; i < count; ++i) plans.push_back(ns_plan(mats[i].rows, mats[i].cols, dtype, steps, need));
+  GLX_REQUIRE(need < (1ull << 40), "glx_orthogonalize: the list needs a workspace of %zu bytes", need);
   if (!workspace || workspace_bytes < need) {
     glx_set_error("glx_orthogonalize: workspace %zu < %zu bytes", workspace_bytes, need);
     return GLX_EWORKSPACE;
@@ -473,11 +497,11 @@ extern "C" int glx_orthogonalize(const glx_matrix* mats, int count, int dtype, i
     int nb = 0, tb = 0;
     for (int j = i; j < count && j < i + NS_MATS; ++j) {
       const NsPlan& p = plans[j];
+      s.first[s.count] = nb; s.tfirst[s.count] = tb;
       NsMat& t = s.mat[s.count++];
       t.src = mats[j].src; t.ld = mats[j].ld_src;
       t.x = (_Float16*)(ws + p.x); t.xt = (_Float16*)(ws + p.xt); t.parts = (double*)(ws + p.parts); t.xscale = (float*)(ws + p.xscale);
       t.rows = p.rows; t.cols = p.cols; t.mp = p.mp; t.np = p.np; t.tall = p.tall; t.nparts = p.nparts;
-      t.block0 = nb; t.tblock0 = tb;
       nb += p.nparts; tb += p.mp / 64 * (p.np / 64);
     }
     hipLaunchKernelGGL(k_ns_norm, dim3(nb), dim3(256), 0, st, s);
@@ -496,30 +520,30 @@ extern "C" int glx_orthogonalize(const glx_matrix* mats, int count, int dtype, i
       if (k == stages.size()) stages.emplace_back();
       return stages[k++];
     };
-    auto planes = [&](size_t o) { return (_Float16*)(ws + o); };
+    auto planes = [](size_t o) { return (unsigned)(o / 256); };
     auto square = [&](size_t A, float as, size_t B, float bs, size_t out, float scale) {       // out = A B, symmetric
       NsOp o = {};
       o.a = planes(A); o.b = planes(B); o.out = planes(out);
       o.alpha = 1.f / (as * bs); o.scale = scale;
-      o.mp = p.mp; o.np = p.mp; o.K = p.mp; o.kper = p.mp; o.splits = 1; o.kind = NS_PLANES; o.sym = 1;
+      o.mp = p.mp; o.np = p.mp; o.K = p.mp; o.kper = (unsigned short)(p.mp / NS_K); o.splits = 1; o.kind = NS_PLANES; o.sym = 1;
       return o;
     };
     size_t x = p.x, xt = p.xt, x2 = p.x2, xt2 = p.xt2;
     for (int s0 = 0; s0 < steps; s0 += p.seg) {
       const int s1 = s0 + p.seg < steps ? s0 + p.seg : steps;
-      const float* xs = (const float*)(ws + p.xscale) + s0;
+      const unsigned xs = planes(p.xscale);
       float gs = ns_scale(lam[s0]);
       {                                                // A = X X^T
         NsOp o = {};
         o.a = o.b = planes(x);
-        o.alpha = 1.f; o.scale = gs; o.xin = xs; o.xpow = 2;
-        o.mp = o.np = p.mp; o.K = p.np; o.kper = p.kper; o.splits = (short)p.splits; o.sym = 1;
+        o.alpha = 1.f; o.scale = gs; o.xin = xs; o.xpow = 2; o.xstep = (unsigned char)s0;
+        o.mp = o.np = p.mp; o.K = p.np; o.kper = (unsigned short)(p.kper / NS_K); o.splits = (unsigned short)p.splits; o.sym = 1;
         const int prods = last(s1) || (s0 == 0 && dtype != GLX_F32) ? 1 : 3;
         if (p.splits > 1) {
-          o.kind = NS_PARTIAL; o.out = ws + p.part;
+          o.kind = NS_PARTIAL; o.out = planes(p.part);
           stage().add(p.tile, prods, o);
           NsOp j = {};
-          j.a = planes(p.part); j.out = planes(p.g); j.scale = gs; j.mp = j.np = p.mp; j.splits = (short)p.splits;
+          j.a = planes(p.part); j.out = planes(p.g); j.scale = gs; j.mp = j.np = p.mp; j.splits = (unsigned short)p.splits;
           stage().join[p.tile == 128].push_back(j);
         } else {
           o.kind = NS_PLANES; o.out = planes(p.g);
@@ -555,15 +579,15 @@ extern "C" int glx_orthogonalize(const glx_matrix* mats, int count, int dtype, i
       {                                                // X <- Q X
         NsOp o = {};
         o.a = planes(q); o.b = planes(xt);
-        o.alpha = 1.f / qs; o.xin = xs; o.xpow = 1;
-        o.mp = p.mp; o.np = p.np; o.K = p.mp; o.kper = p.mp; o.splits = 1;
+        o.alpha = 1.f / qs; o.xin = xs; o.xpow = 1; o.xstep = (unsigned char)s0;
+        o.mp = p.mp; o.np = p.np; o.K = p.mp; o.kper = (unsigned short)(p.mp / NS_K); o.splits = 1;
         if (s1 == steps) {
-          o.kind = NS_FINAL; o.out = mats[i].dst; o.ldd = mats[i].ld_dst;
+          o.kind = NS_FINAL; o.dst = mats[i].dst; o.ldd = mats[i].ld_dst;
           o.m = p.m; o.n = p.n; o.tall = (unsigned char)p.tall; o.dtype = (unsigned char)dtype;
         } else {
-          o.kind = NS_XPLANES; o.out = planes(x2); o.out2 = planes(xt2); o.xout = (const float*)(ws + p.xscale) + s1;
+          o.kind = NS_XPLANES; o.out = planes(x2); o.out2 = planes(xt2); o.xout = xs; o.xnext = (unsigned char)s1;
         }
-        stage().add(p.tile, last(s1) ? 1 : s0 == 0 && dtype != GLX_F32 ? 2 : 3, o);
+        stage().add(p.xtile, last(s1) ? 1 : s0 == 0 && dtype != GLX_F32 ? 2 : 3, o);
         size_t y = x; x = x2; x2 = y;
         y = xt; xt = xt2; xt2 = y;
       }
@@ -571,8 +595,8 @@ extern "C" int glx_orthogonalize(const glx_matrix* mats, int count, int dtype, i
   }
   for (auto& g : stages) {
     for (int t = 0; t < 2; ++t) {
-      for (int n = 0; n < 3; ++n) ns_launch_ops(g.gemm[t][n], t ? 128 : 64, n + 1, st);
-      ns_launch_ops(g.join[t], t ? 128 : 64, 0, st);
+      for (int n = 0; n < 3; ++n) ns_launch_ops(g.gemm[t][n], ws, t ? 128 : 64, n + 1, st);
+      ns_launch_ops(g.join[t], ws, t ? 128 : 64, 0, st);
     }
   }
   GLX_LAUNCH_CHECK();
