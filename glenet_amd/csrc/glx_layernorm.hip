@@ -21,6 +21,7 @@ struct LnArgs {
   void* y;                    // forward: y; backward: dx
   float* mean; float* rstd;
   float* part;                // [blocks][2][C]
+  void* dw; void* db;         // written by a backward pass of one block
   long long ldx, ldg, rows, C;
   float eps;
   int wf32;                   // the weights are fp32 (else of x's type)
@@ -85,47 +86,65 @@ __device__ __forceinline__ float ln_sum(float s, float* red) {
   return s;
 }
 
+// one row vector as it lies in memory; beyond the row's end zeros
+template <typename T>
+__device__ __forceinline__ typename GlxVec<T, LnVec<T>::N>::vec ln_raw(const T* __restrict__ p, long long col, long long C) {
+  constexpr int V = LnVec<T>::N;
+  if (col + V <= C) return GlxVec<T, V>::load(p + col);
+  typename GlxVec<T, V>::vec r = {};
+#pragma unroll
+  for (int i = 0; i < V; ++i)
+    if (col + i < C) r[i] = p[col + i];
+  return r;
+}
+
 template <typename T, int L, int NV>
-__global__ __launch_bounds__(L > 256 ? L : 256) void k_ln_forward(LnArgs a) {
-  constexpr int V = LnVec<T>::N, THREADS = L > 256 ? L : 256, G = THREADS / L;
+__global__ __launch_bounds__(256) void k_ln_forward(LnArgs a) {
+  constexpr int V = LnVec<T>::N, G = 256 / L;
   __shared__ float red[2][16];
   const int t = threadIdx.x % L;
   const float inv = 1.f / (float)a.C;
   for (long long row = (long long)blockIdx.x * G + threadIdx.x / L; row < a.rows; row += (long long)gridDim.x * G) {
     const T* x = (const T*)a.x + row * a.ldx;
-    float v[NV][V];
+    typename GlxVec<T, V>::vec r[NV];                          // (as read: half the registers of floats for 16-bit rows)
     float s = 0.f;
 #pragma unroll
-    for (int j = 0; j < NV; ++j) {
-      ln_load<T>(x, (long long)(j * L + t) * V, a.C, 0.f, v[j]);
-#pragma unroll
-      for (int i = 0; i < V; ++i) s += v[j][i];
-    }
-    const float mean = ln_sum<L>(s, red[0]) * inv;
-    s = 0.f;
+    for (int j = 0; j < NV; ++j) r[j] = ln_raw<T>(x, (long long)(j * L + t) * V, a.C);
 #pragma unroll
     for (int j = 0; j < NV; ++j)
 #pragma unroll
-      for (int i = 0; i < V; ++i) {
-        const float d = v[j][i] - mean;
-        s += (long long)(j * L + t) * V + i < a.C ? d * d : 0.f;
+      for (int i = 0; i < V; ++i) s += (float)r[j][i];
+    const float mean = ln_sum<L>(s, red[0]) * inv;
+    s = 0.f;
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      const long long left = a.C - (long long)(j * L + t) * V;
+      if (left >= V) {
+#pragma unroll
+        for (int i = 0; i < V; ++i) { const float d = (float)r[j][i] - mean; s += d * d; }
+      } else {
+#pragma unroll
+        for (int i = 0; i < V; ++i) { const float d = (float)r[j][i] - mean; s += i < left ? d * d : 0.f; }
       }
+    }
     const float rstd = 1.f / sqrtf(ln_sum<L>(s, red[1]) * inv + a.eps);
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
       const long long col = (long long)(j * L + t) * V;
-      float w[V], b[V];
+      if (col >= a.C) break;
+      float v[V], w[V], b[V];
       ln_load_w<T>(a.w, a.wf32, col, a.C, 1.f, w);
       ln_load_w<T>(a.b, a.wf32, col, a.C, 0.f, b);
 #pragma unroll
-      for (int i = 0; i < V; ++i) v[j][i] = (v[j][i] - mean) * rstd * w[i] + b[i];
-      ln_store<T>((T*)a.y + row * a.C, col, a.C, v[j]);
+      for (int i = 0; i < V; ++i) v[i] = ((float)r[j][i] - mean) * rstd * w[i] + b[i];
+      ln_store<T>((T*)a.y + row * a.C, col, a.C, v);
     }
     if (a.mean && t == 0) { a.mean[row] = mean; a.rstd[row] = rstd; }
   }
 }
 
-// rows that no block holds in registers: three passes, the second and third from the caches
+// Wider rows than 256 threads hold in four vectors each: three passes, the second and third from the caches, two blocks per compute
+// unit (512 x 20736 fp32: 23 us, 83 KB a row; held in the registers of 1024 threads, one block per compute unit, 31 us)
 template <typename T>
 __global__ __launch_bounds__(1024) void k_ln_forward_long(LnArgs a) {
   constexpr int V = LnVec<T>::N;
@@ -134,6 +153,7 @@ __global__ __launch_bounds__(1024) void k_ln_forward_long(LnArgs a) {
   for (long long row = blockIdx.x; row < a.rows; row += gridDim.x) {
     const T* x = (const T*)a.x + row * a.ldx;
     float s = 0.f;
+#pragma unroll 4
     for (long long col = (long long)threadIdx.x * V; col < a.C; col += 1024 * V) {
       float v[V];
       ln_load<T>(x, col, a.C, 0.f, v);
@@ -142,6 +162,7 @@ __global__ __launch_bounds__(1024) void k_ln_forward_long(LnArgs a) {
     }
     const float mean = (float)(ln_sum<1024>(s, red[0]) * inv);
     s = 0.f;
+#pragma unroll 4
     for (long long col = (long long)threadIdx.x * V; col < a.C; col += 1024 * V) {
       float v[V];
       ln_load<T>(x, col, a.C, mean, v);
@@ -149,6 +170,7 @@ __global__ __launch_bounds__(1024) void k_ln_forward_long(LnArgs a) {
       for (int i = 0; i < V; ++i) s += (v[i] - mean) * (v[i] - mean);
     }
     const float rstd = 1.f / sqrtf((float)(ln_sum<1024>(s, red[1]) * inv) + a.eps);
+#pragma unroll 4
     for (long long col = (long long)threadIdx.x * V; col < a.C; col += 1024 * V) {
       float v[V], w[V], b[V];
       ln_load<T>(x, col, a.C, 0.f, v);
@@ -162,10 +184,10 @@ __global__ __launch_bounds__(1024) void k_ln_forward_long(LnArgs a) {
   }
 }
 
-// dx of the rows and, SUMS, the block's part of dw / db
+// dx of the rows and, SUMS, the block's part of dw / db (one block: dw / db themselves)
 template <typename T, int L, int NV, bool SUMS>
-__global__ __launch_bounds__(L > 256 ? L : 256) void k_ln_backward(LnArgs a) {
-  constexpr int V = LnVec<T>::N, THREADS = L > 256 ? L : 256, G = THREADS / L;
+__global__ __launch_bounds__(256) void k_ln_backward(LnArgs a) {
+  constexpr int V = LnVec<T>::N, G = 256 / L;
   __shared__ float red[2][16];
   const int t = threadIdx.x % L;
   const float inv = 1.f / (float)a.C;
@@ -212,6 +234,13 @@ __global__ __launch_bounds__(L > 256 ? L : 256) void k_ln_backward(LnArgs a) {
   }
   if (!SUMS) return;
   float* part = a.part + (long long)blockIdx.x * 2 * a.C;
+  auto put = [&](int k, long long c, float v) {                // column c of dw (k = 0) or db
+    if (gridDim.x > 1) part[k * a.C + c] = v;
+    else if (void* out = k ? a.db : a.dw) {
+      if (a.wf32) ((float*)out)[c] = v;
+      else ((T*)out)[c] = (T)v;
+    }
+  };
   if (G > 1) {
     // the wave's groups by shuffles, the block's four waves through LDS
     __shared__ float acc[4][(L < 64 ? L : 64) * NV * V];
@@ -233,19 +262,16 @@ __global__ __launch_bounds__(L > 256 ? L : 256) void k_ln_backward(LnArgs a) {
           for (int i = 0; i < V; ++i) acc[threadIdx.x >> 6][(j * L + t) * V + i] = k ? db[j][i] : dw[j][i];
       }
       __syncthreads();
-      for (int c = threadIdx.x; c < a.C; c += 256) part[k * a.C + c] = acc[0][c] + acc[1][c] + acc[2][c] + acc[3][c];
+      for (int c = threadIdx.x; c < a.C; c += 256) put(k, c, acc[0][c] + acc[1][c] + acc[2][c] + acc[3][c]);
       __syncthreads();
     }
   } else {
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
       const long long col = (long long)(j * L + t) * V;
-      ln_store<float>(part, col, a.C, dw[j]);
-      ln_store<float>(part + a.C, col, a.C, db[j]);
-      if (V == 8) {
-        ln_store<float>(part, col + 4, a.C, dw[j] + V / 2);
-        ln_store<float>(part + a.C, col + 4, a.C, db[j] + V / 2);
-      }
+#pragma unroll
+      for (int i = 0; i < V; ++i)
+        if (col + i < a.C) { put(0, col + i, dw[j][i]); put(1, col + i, db[j][i]); }
     }
   }
 }
@@ -260,6 +286,7 @@ __global__ __launch_bounds__(1024) void k_ln_backward_long(LnArgs a) {
     const T* gy = (const T*)a.gy + row * a.ldg;
     const float mean = a.mean[row], rstd = a.rstd[row];
     float s1 = 0.f, s2 = 0.f;
+#pragma unroll 4
     for (long long col = (long long)threadIdx.x * V; col < a.C; col += 1024 * V) {
       float h[V], g[V], w[V];
       ln_load<T>(x, col, a.C, mean, h);
@@ -274,6 +301,7 @@ __global__ __launch_bounds__(1024) void k_ln_backward_long(LnArgs a) {
     }
     s1 = (float)(ln_sum<1024>(s1, red[0]) * inv);
     s2 = (float)(ln_sum<1024>(s2, red[1]) * inv);
+#pragma unroll 4
     for (long long col = (long long)threadIdx.x * V; col < a.C; col += 1024 * V) {
       float h[V], g[V], w[V];
       ln_load<T>(x, col, a.C, mean, h);
@@ -354,14 +382,15 @@ static LnPlan ln_plan(long long rows, long long C, int dtype) {
   const int V = dtype == GLX_F32 ? 4 : 8;
   const long long nvec = (C + V - 1) / V;
   LnPlan p = {};
-  static const int forms[][2] = {{8, 1}, {16, 1}, {32, 1}, {64, 1}, {64, 2}, {64, 4}, {256, 2}, {256, 4}, {1024, 2}, {1024, 4}, {1024, 8}};
+  static const int forms[][2] = {{8, 1}, {16, 1}, {32, 1}, {64, 1}, {64, 2}, {64, 4}, {256, 2}, {256, 4}};
   for (auto& f : forms)
     if (nvec <= (long long)f[0] * f[1]) { p.L = f[0]; p.NV = f[1]; break; }
-  const int G = p.L && p.L <= 256 ? 256 / p.L : 1;
-  p.fused = p.L && p.L <= 256;
+  const int G = p.L ? 256 / p.L : 1;
+  p.fused = p.L;
   const long long groups = (rows + G - 1) / G;
-  long long want = groups / 8;                        // eight visits a group: the parts stay small beside the rows
-  want = want < 256 ? 256 : (want > LN_BLOCKS ? LN_BLOCKS : want);
+  // eight visits a group: the parts stay small beside the rows.  Up to four groups one block does it all, without parts or a join
+  long long want = groups / 8;
+  want = p.fused && groups <= 4 ? 1 : want < 256 ? 256 : (want > LN_BLOCKS ? LN_BLOCKS : want);
   p.blocks = (int)(groups < want ? groups : want);
   if (p.fused) {
     p.parts = p.blocks;
@@ -372,17 +401,18 @@ static LnPlan ln_plan(long long rows, long long C, int dtype) {
     if (splits < 1) splits = 1;
     p.rows_per = (rows + splits - 1) / splits;
     p.parts = rows ? (int)((rows + p.rows_per - 1) / p.rows_per) : 0;
+    if (p.parts == 1) p.parts = 2;                    // (an empty second part: these are always joined)
   }
   return p;
 }
 
 template <typename T>
 static void ln_launch_forward(const LnPlan& p, const LnArgs& a, hipStream_t st) {
-  const int G = p.L && p.L <= 256 ? 256 / p.L : 1;
+  const int G = p.L ? 256 / p.L : 1;
   const long long groups = (a.rows + G - 1) / G;
   const dim3 grid((unsigned)(groups < 8 * LN_BLOCKS ? groups : 8 * LN_BLOCKS));
-#define LN_F(L_, N_) if (p.L == L_ && p.NV == N_) { hipLaunchKernelGGL((k_ln_forward<T, L_, N_>), grid, dim3(L_ > 256 ? L_ : 256), 0, st, a); return; }
-  LN_F(8, 1) LN_F(16, 1) LN_F(32, 1) LN_F(64, 1) LN_F(64, 2) LN_F(64, 4) LN_F(256, 2) LN_F(256, 4) LN_F(1024, 2) LN_F(1024, 4) LN_F(1024, 8)
+#define LN_F(L_, N_) if (p.L == L_ && p.NV == N_) { hipLaunchKernelGGL((k_ln_forward<T, L_, N_>), grid, dim3(256), 0, st, a); return; }
+  LN_F(8, 1) LN_F(16, 1) LN_F(32, 1) LN_F(64, 1) LN_F(64, 2) LN_F(64, 4) LN_F(256, 2) LN_F(256, 4)
 #undef LN_F
   hipLaunchKernelGGL((k_ln_forward_long<T>), grid, dim3(1024), 0, st, a);
 }
@@ -395,11 +425,8 @@ static void ln_launch_backward(const LnPlan& p, const LnArgs& a, bool sums, hipS
     else hipLaunchKernelGGL((k_ln_backward<T, L_, N_, false>), grid, dim3(256), 0, st, a);                                        \
     return;                                                                                                                       \
   }
-#define LN_W(N_) if (p.L == 1024 && p.NV == N_) { if (a.y) hipLaunchKernelGGL((k_ln_backward<T, 1024, N_, false>), grid, dim3(1024), 0, st, a); }
   LN_B(8, 1) LN_B(16, 1) LN_B(32, 1) LN_B(64, 1) LN_B(64, 2) LN_B(64, 4) LN_B(256, 2) LN_B(256, 4)
-  LN_W(2) LN_W(4) LN_W(8)
 #undef LN_B
-#undef LN_W
   if (p.L == 0 && a.y) hipLaunchKernelGGL((k_ln_backward_long<T>), grid, dim3(1024), 0, st, a);
   if (sums) {
     constexpr int V = LnVec<T>::N;
@@ -433,9 +460,10 @@ extern "C" int glx_layer_norm_forward(const void* x, int64_t ldx, int dtype, con
 }
 
 extern "C" size_t glx_layer_norm_workspace_bytes(int64_t rows, int64_t width) {
-  if (rows <= 0 || width <= 0) return 256;
+  if (rows <= 0 || width <= 0) return 0;
   const LnPlan p = ln_plan(rows, width, GLX_F32), q = ln_plan(rows, width, GLX_BF16);
-  return glx_align((size_t)(p.parts > q.parts ? p.parts : q.parts) * 2 * width * sizeof(float));
+  const int parts = p.parts > q.parts ? p.parts : q.parts;
+  return parts > 1 ? glx_align((size_t)parts * 2 * width * sizeof(float)) : 0;
 }
 
 extern "C" int glx_layer_norm_backward(const void* gy, int64_t ldg, const void* x, int64_t ldx, int dtype, const void* weight,
@@ -445,13 +473,13 @@ extern "C" int glx_layer_norm_backward(const void* gy, int64_t ldg, const void* 
   const bool sums = dweight || dbias;
   GLX_REQUIRE(!sums || wdtype == GLX_F32 || wdtype == dtype, "glx_layer_norm_backward: weight gradients of type %d", wdtype);
   GLX_REQUIRE(rows == 0 || (gy && x && mean && rstd && ldx >= 0 && ldg >= 0), "glx_layer_norm_backward: bad pointers");
-  if (sums && rows > 0 && (!workspace || workspace_bytes < glx_layer_norm_workspace_bytes(rows, width))) {
+  if (sums && workspace_bytes < glx_layer_norm_workspace_bytes(rows, width)) {
     glx_set_error("glx_layer_norm_backward: workspace %zu < %zu bytes", workspace_bytes, glx_layer_norm_workspace_bytes(rows, width));
     return GLX_EWORKSPACE;
   }
   if (!sums && (!dx || rows == 0)) return GLX_OK;
   LnArgs a = {};
-  a.x = x; a.gy = gy; a.w = weight; a.y = dx; a.mean = (float*)mean; a.rstd = (float*)rstd; a.part = (float*)workspace;
+  a.x = x; a.gy = gy; a.w = weight; a.y = dx; a.mean = (float*)mean; a.rstd = (float*)rstd; a.part = (float*)workspace; a.dw = dweight; a.db = dbias;
   a.ldx = ldx; a.ldg = ldg; a.rows = rows; a.C = width; a.wf32 = wdtype == GLX_F32;
   const LnPlan p = ln_plan(rows, width, dtype);
   hipStream_t st = (hipStream_t)stream;
@@ -460,7 +488,7 @@ extern "C" int glx_layer_norm_backward(const void* gy, int64_t ldg, const void* 
     else if (dtype == GLX_BF16) ln_launch_backward<__bf16>(p, a, sums, st);
     else ln_launch_backward<_Float16>(p, a, sums, st);
   }
-  if (sums) {
+  if (sums && !(p.fused && p.parts == 1 && rows > 0)) {
     const dim3 grid((unsigned)((2 * width + 15) / 16));
     const int parts = rows > 0 ? p.parts : 0;
     if (wdtype == GLX_F32)

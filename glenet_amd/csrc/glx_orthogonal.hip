@@ -174,7 +174,7 @@ __global__ __launch_bounds__(256) void k_ns_planes(NsMats s) {
 // A block forms a TILE x TILE tile with four waves of (TILE / 2)^2, k in steps of KS that go from memory to LDS without registers,
 // several ahead (small products are all latency: four stages bring 256 x 256 in one round trip, 8.9 -> XX us); the order of a
 // staged row's 16-byte chunks is rotated by the row, so that the 32 rows an operand read touches spread over the banks.  PROD
-// products per pair of operands: 3 both split, 2 where B's lo plane is empty, 1 where neither is used.
+// products per pair of operands: 3 both split (4: with lo lo), 2 where B's lo plane is empty, 1 where neither is used.
 template <int TILE, int PROD>
 __global__ __launch_bounds__(256) void k_ns_gemm(NsOps s) {
   constexpr int KS = TILE == 64 ? 64 : 32, C = KS / 8, RB = KS * 2;  // k elements of a stage, its chunks and bytes per row
@@ -255,6 +255,7 @@ __global__ __launch_bounds__(256) void k_ns_gemm(NsOps s) {
       for (int i = 0; i < F; ++i)
 #pragma unroll
         for (int j = 0; j < F; ++j) {
+          if (PROD > 3) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fa[PA - 1][i], fb[PB - 1][j], acc[i][j], 0, 0, 0);
           if (PROD > 1) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fa[PA - 1][i], fb[0][j], acc[i][j], 0, 0, 0);
           if (PROD > 2) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fa[0][i], fb[PB - 1][j], acc[i][j], 0, 0, 0);
           acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fa[0][i], fb[0][j], acc[i][j], 0, 0, 0);
@@ -432,13 +433,14 @@ extern "C" size_t glx_orthogonalize_workspace_bytes(const glx_matrix* mats, int 
 }
 
 struct NsStage {               // what one launch round does, over all matrices
-  std::vector<NsOp> gemm[2][3], join[2];       // by tile; by the products per pair of operands
+  std::vector<NsOp> gemm[2][4], join[2];       // by tile; by the products per pair of operands
   void add(int tile, int prods, const NsOp& o) { gemm[tile == 128][prods - 1].push_back(o); }
 };
 
 template <int TILE>
 static void ns_launch_gemm(const NsOps& s, int blocks, int prods, hipStream_t st) {
-  if (prods == 1) hipLaunchKernelGGL((k_ns_gemm<TILE, 1>), dim3(blocks), dim3(256), 0, st, s);
+  if (prods == 4) hipLaunchKernelGGL((k_ns_gemm<TILE, 4>), dim3(blocks), dim3(256), 0, st, s);
+  else if (prods == 1) hipLaunchKernelGGL((k_ns_gemm<TILE, 1>), dim3(blocks), dim3(256), 0, st, s);
   else if (prods == 2) hipLaunchKernelGGL((k_ns_gemm<TILE, 2>), dim3(blocks), dim3(256), 0, st, s);
   else hipLaunchKernelGGL((k_ns_gemm<TILE, 3>), dim3(blocks), dim3(256), 0, st, s);
 }
@@ -515,6 +517,9 @@ extern "C" int glx_orthogonalize(const glx_matrix* mats, int count, int dtype, i
     // bfloat16: single products in the last two steps, where what they lose is no longer amplified (it comes to 1e-3 of the
     // result, half a step is 4e-3); segments of one step only
     auto last = [&](int s1) { return dtype == GLX_BF16 && p.seg == 1 && s1 > steps - 2 && steps >= 4; };
+    // lo lo too: fp32 matrices on 64-wide tiles, whose time is latency and LDS (small ones lose up to 1.6 times a plain fp32
+    // product's error without)
+    const int full = dtype == GLX_F32 && p.tile == 64 && p.xtile == 64 ? 4 : 3;
     size_t k = 0;
     auto stage = [&]() -> NsStage& {
       if (k == stages.size()) stages.emplace_back();
@@ -538,7 +543,7 @@ extern "C" int glx_orthogonalize(const glx_matrix* mats, int count, int dtype, i
         o.a = o.b = planes(x);
         o.alpha = 1.f; o.scale = gs; o.xin = xs; o.xpow = 2; o.xstep = (unsigned char)s0;
         o.mp = o.np = p.mp; o.K = p.np; o.kper = (unsigned short)(p.kper / NS_K); o.splits = (unsigned short)p.splits; o.sym = 1;
-        const int prods = last(s1) || (s0 == 0 && dtype != GLX_F32) ? 1 : 3;
+        const int prods = last(s1) || (s0 == 0 && dtype != GLX_F32) ? 1 : full;
         if (p.splits > 1) {
           o.kind = NS_PARTIAL; o.out = planes(p.part);
           stage().add(p.tile, prods, o);
@@ -557,20 +562,20 @@ extern "C" int glx_orthogonalize(const glx_matrix* mats, int count, int dtype, i
         const size_t P = p.p[(s - s0) & 1];
         NsOp o = square(p.g, gs, p.g, gs, P, ps);      // P = a I + b A + c A A
         o.alpha *= c; o.d = planes(p.g); o.beta = b / gs; o.diag = a;
-        stage().add(p.tile, last(s1) ? 1 : 3, o);
+        stage().add(p.tile, last(s1) ? 1 : full, o);
         if (s == s0) {
           q = P; qs = ps;
         } else {                                       // (beside H where a step follows)
           const float nqs = ns_scale(qbound(s0, s));
           const size_t nq = p.q[(s - s0) & 1];
-          stage().add(p.tile, 3, square(P, ps, q, qs, nq, nqs));
+          stage().add(p.tile, full, square(P, ps, q, qs, nq, nqs));
           q = nq; qs = nqs;
           --k;
         }
         if (s + 1 < s1) {
-          stage().add(p.tile, 3, square(P, ps, p.g, gs, p.h, hs));
+          stage().add(p.tile, full, square(P, ps, p.g, gs, p.h, hs));
           const float ngs = ns_scale(lam[s + 1]);
-          stage().add(p.tile, 3, square(p.h, hs, P, ps, p.g, ngs));
+          stage().add(p.tile, full, square(p.h, hs, P, ps, p.g, ngs));
           gs = ngs;
         } else if (s > s0) {
           ++k;
@@ -587,7 +592,7 @@ extern "C" int glx_orthogonalize(const glx_matrix* mats, int count, int dtype, i
         } else {
           o.kind = NS_XPLANES; o.out = planes(x2); o.out2 = planes(xt2); o.xout = xs; o.xnext = (unsigned char)s1;
         }
-        stage().add(p.xtile, last(s1) ? 1 : s0 == 0 && dtype != GLX_F32 ? 2 : 3, o);
+        stage().add(p.xtile, last(s1) ? 1 : s0 == 0 && dtype != GLX_F32 ? 2 : full, o);
         size_t y = x; x = x2; x2 = y;
         y = xt; xt = xt2; xt2 = y;
       }
@@ -595,7 +600,7 @@ extern "C" int glx_orthogonalize(const glx_matrix* mats, int count, int dtype, i
   }
   for (auto& g : stages) {
     for (int t = 0; t < 2; ++t) {
-      for (int n = 0; n < 3; ++n) ns_launch_ops(g.gemm[t][n], ws, t ? 128 : 64, n + 1, st);
+      for (int n = 0; n < 4; ++n) ns_launch_ops(g.gemm[t][n], ws, t ? 128 : 64, n + 1, st);
       ns_launch_ops(g.join[t], ws, t ? 128 : 64, 0, st);
     }
   }
