@@ -159,7 +159,7 @@ struct XaLoad {
         // not see them: `settle` waits.  64 lanes x 16 bytes from base + o to LDS at the wave's place.)
         asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1"
                      ::"v"(o), "s"(base), "s"(__builtin_amdgcn_readfirstlane(to + i * 4096))
-                     : "memory", "m0");
+                     : "memory");
       }
     } else {
 #pragma unroll 1

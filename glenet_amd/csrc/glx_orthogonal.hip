@@ -66,6 +66,8 @@ __device__ __forceinline__ int ns_entry(const int* first, int count) {
   const int lane = threadIdx.x & 63;
   return __popcll(__ballot(lane < count && (int)blockIdx.x >= first[lane < count ? lane : 0])) - 1;
 }
+// elements between the rows of planes of k columns: rows of a power of two bytes would all start in the same cache channels
+__host__ __device__ __forceinline__ int ns_ld(int k) { return k % 256 == 0 ? k + 64 : k; }
 __device__ __forceinline__ void ns_split(float v, _Float16& hi, _Float16& lo) {
   hi = (_Float16)v;
   lo = (_Float16)(v - (float)hi);
@@ -147,7 +149,8 @@ __global__ __launch_bounds__(256) void k_ns_planes(NsMats s) {
     if (t.tall) tile[c][r] = v; else tile[r][c] = v;
   }
   __syncthreads();
-  const long long plane = (long long)t.mp * t.np;
+  const int ldn = ns_ld(t.np), ldm = ns_ld(t.mp);
+  const long long plane = (long long)t.mp * ldn, tplane = (long long)t.np * ldm;
 #pragma unroll
   for (int it = 0; it < 2; ++it) {
     const int q = threadIdx.x + it * 256, r = q >> 3, c8 = (q & 7) * 8;
@@ -160,29 +163,33 @@ __global__ __launch_bounds__(256) void k_ns_planes(NsMats s) {
       ns_split(tile[c8 + e][r], u, v);
       th[e] = u; tl[e] = v;
     }
-    const long long o = (long long)(i0 + r) * t.np + j0 + c8, ot = (long long)(j0 + r) * t.mp + i0 + c8;
+    const long long o = (long long)(i0 + r) * ldn + j0 + c8, ot = (long long)(j0 + r) * ldm + i0 + c8;
     *reinterpret_cast<nh8*>(t.x + o) = h;
     *reinterpret_cast<nh8*>(t.xt + ot) = th;
     if (s.dtype == GLX_F32) {
       *reinterpret_cast<nh8*>(t.x + plane + o) = l;
-      *reinterpret_cast<nh8*>(t.xt + plane + ot) = tl;
+      *reinterpret_cast<nh8*>(t.xt + tplane + ot) = tl;
     }
   }
 }
 
 // ------------------------------------------------------------------------------------------------ the products
-// A block forms a TILE x TILE tile with four waves of (TILE / 2)^2, k in steps of KS that go from memory to LDS without registers,
-// several ahead (small products are all latency: four stages bring 256 x 256 in one round trip, 8.9 -> XX us); the order of a
-// staged row's 16-byte chunks is rotated by the row, so that the 32 rows an operand read touches spread over the banks.  PROD
-// products per pair of operands: 3 both split (4: with lo lo), 2 where B's lo plane is empty, 1 where neither is used.
-template <int TILE, int PROD>
-__global__ __launch_bounds__(256) void k_ns_gemm(NsOps s) {
-  constexpr int KS = TILE == 64 ? 64 : 32, C = KS / 8, RB = KS * 2;  // k elements of a stage, its chunks and bytes per row
-  constexpr int STAGES = TILE == 64 ? 4 : 2;
+// A block forms a TILE x TILE tile.  k comes in steps of KS that go from memory to LDS without registers, STAGES of them ahead (a
+// product is bound by the round trips of what is in flight: four stages bring 256 x 256 in one); the four waves share a step
+// along k, each for the whole tile, so that an operand read from LDS serves two or four products, and their sums are joined through
+// LDS at the end, each wave finishing a quarter.  (With a quarter of the tile per wave the
+// 64-wide form read twice as much from LDS as the matrix units could take.)  The order of a staged row's 16-byte chunks is rotated
+// by the row, so that the 32 rows an operand read touches spread over the banks.  PROD products per pair of operands: 3 both split
+// (4: with lo lo), 2 where B's lo plane is empty, 1 where neither is used.
+template <int TILE, int PROD, int STAGES>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1))) void k_ns_gemm(NsOps s) {
+  constexpr int KS = 64, C = KS / 8, RB = KS * 2;                    // k elements of a stage, its chunks and bytes per row
   constexpr int PA = PROD > 1 ? 2 : 1, PB = PROD > 2 ? 2 : 1;        // planes of the operands
-  constexpr int W = TILE / 2, F = W / 32, CH = TILE * C / 256;       // a wave's tile, its 32-wide parts, chunks per thread and plane
-  constexpr int LOADS = (PA + PB) * CH;                              // transfers per wave and stage
-  __shared__ __attribute__((aligned(16))) char smem[STAGES][PA + PB][TILE * RB];
+  constexpr int F = TILE / 32, H = TILE / 64;                        // 32-wide parts: of the tile, of a quarter of it
+  constexpr int CH = TILE * C / 256, LOADS = (PA + PB) * CH;         // transfers per thread: of a plane, of a stage
+  constexpr int PLANE = TILE * RB, STAGE = (PA + PB) * PLANE;
+  constexpr int JOIN = 4 * H * H * 4096, BYTES = STAGES * STAGE > JOIN ? STAGES * STAGE : JOIN;       // (a quarter per wave)
+  __shared__ __attribute__((aligned(16))) char smem[BYTES];
   const int entry = ns_entry(s.first, s.count);
   const NsOp& t = s.op[entry];
   int b = blockIdx.x - s.first[entry];
@@ -201,29 +208,27 @@ __global__ __launch_bounds__(256) void k_ns_gemm(NsOps s) {
   auto at = [&](unsigned place) { return s.ws + (size_t)place * 256; };
   const float xin = t.xin ? ((const float*)at(t.xin))[t.xstep] : 1.f, alpha = t.alpha / (t.xpow == 2 ? xin * xin : xin), scale = t.xout ? ((const float*)at(t.xout))[t.xnext] : t.scale;
   const int kper = t.kper * NS_K, k0 = split * kper, k1 = k0 + kper < t.K ? k0 + kper : t.K;
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wi = wave >> 1, wj = wave & 1, half = lane >> 5, l32 = lane & 31;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5, l32 = lane & 31;
+  const int ld = ns_ld(t.K);
   const _Float16* src[PA + PB];
 #pragma unroll
-  for (int p = 0; p < PA; ++p) src[p] = (const _Float16*)at(t.a) + ((long long)p * t.mp + ti * TILE) * t.K;
+  for (int p = 0; p < PA; ++p) src[p] = (const _Float16*)at(t.a) + ((long long)p * t.mp + ti * TILE) * ld;
 #pragma unroll
-  for (int p = 0; p < PB; ++p) src[PA + p] = (const _Float16*)at(t.b) + ((long long)p * t.np + tj * TILE) * t.K;
-  auto place = [](int r, int ch) { return r * RB + (C == 8 ? (ch ^ r) & 7 : (ch ^ (r >> 1)) & 3) * 16; };
-  // memory -> LDS: a lane fetches the chunk that belongs at its place (the compiler does not see these transfers: `arrived`)
+  for (int p = 0; p < PB; ++p) src[PA + p] = (const _Float16*)at(t.b) + ((long long)p * t.np + tj * TILE) * ld;
+  auto swap = [](int r, int ch) { return (ch ^ r) & 7; };
+  // memory -> LDS: a lane fetches the chunk that belongs at its place (the compiler does not see these transfers)
   int off[CH];
 #pragma unroll
   for (int c = 0; c < CH; ++c) {
-    const int q = threadIdx.x + c * 256, r = q / C, ch = C == 8 ? (q ^ r) & 7 : (q ^ (r >> 1)) & 3;
-    off[c] = (r * t.K + ch * 8) * 2;
+    const int q = threadIdx.x + c * 256, r = q / C;
+    off[c] = (r * ld + swap(r, q) * 8) * 2;
   }
-  auto fetch = [&](int n) {
-    const unsigned to = (unsigned)(unsigned long long)(__attribute__((address_space(3))) char*)smem[n % STAGES][0] + (wave << 10);
-#pragma unroll
-    for (int p = 0; p < PA + PB; ++p)
-#pragma unroll
-      for (int c = 0; c < CH; ++c)
-        asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1"
-                     ::"v"(off[c]), "s"(src[p] + k0 + n * KS), "s"(to + p * (TILE * RB) + c * 4096)
-                     : "memory", "m0");
+  auto fetch = [&](int n, int x, int slot = -1) {                    // transfer x of stage n
+    const unsigned to = (unsigned)(unsigned long long)(__attribute__((address_space(3))) char*)smem
+                        + (slot < 0 ? n % STAGES : slot) * STAGE + (wave << 10);
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1"
+                 ::"v"(off[x % CH]), "s"(src[x / CH] + k0 + n * KS), "s"(to + x / CH * PLANE + x % CH * 4096)
+                 : "memory");
   };
   nf16 acc[F][F];
 #pragma unroll
@@ -231,49 +236,101 @@ __global__ __launch_bounds__(256) void k_ns_gemm(NsOps s) {
 #pragma unroll
     for (int j = 0; j < F; ++j) acc[i][j] = (nf16)(0.f);
   const int stages = (k1 - k0) / KS;
-  for (int n = 0; n < STAGES && n < stages; ++n) fetch(n);
+  // 64-wide: every slot is filled at once, and again as it falls free.  128-wide: a slot stays free, the transfers for it go out
+  // between the products (one after the other they hold a wave up for as long as the products take), behind the last stage
+  // repeating it into slots that are not read again
+  constexpr bool BETWEEN = TILE == 128;
+  for (int n = 0; n < STAGES - BETWEEN && n < stages; ++n)
+#pragma unroll
+    for (int x = 0; x < LOADS; ++x) fetch(n, x);
   for (int n = 0; n < stages; ++n) {
     // stage n is there once at most the later ones are on their way; its slot's last readers have passed the barrier of n - 1
-    if (n == 0 && stages >= STAGES) asm volatile("s_waitcnt vmcnt(%0)" ::"n"((STAGES - 1) * LOADS) : "memory");
-    else if (n > 0 && n + STAGES - 2 < stages) asm volatile("s_waitcnt vmcnt(%0)" ::"n"((STAGES - 2) * LOADS) : "memory");
+    if (BETWEEN ? stages >= STAGES - 1 : n > 0 && n + STAGES - 2 < stages) asm volatile("s_waitcnt vmcnt(%0)" ::"n"((STAGES - 2) * LOADS) : "memory");
+    else if (!BETWEEN && n == 0 && stages >= STAGES) asm volatile("s_waitcnt vmcnt(%0)" ::"n"((STAGES - 1) * LOADS) : "memory");
     else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();
-    if (n > 0 && n + STAGES - 1 < stages) fetch(n + STAGES - 1);
-    const int buf = n % STAGES;
+    if (!BETWEEN && n > 0 && n + STAGES - 1 < stages) {
 #pragma unroll
-    for (int ks = 0; ks < KS / 16; ++ks) {
-      nh8 fa[PA][F], fb[PB][F];
-      const int ch = ks * 2 + half;
+      for (int x = 0; x < LOADS; ++x) fetch(n + STAGES - 1, x);
+    }
+    const int from = n + STAGES - 1 < stages ? n + STAGES - 1 : stages - 1, slot = (n + STAGES - 1) % STAGES;
+    const char* at = smem + (n % STAGES) * STAGE;
+    const int ch = wave * 2 + half;
+    nh8 fa[2][PA], fb[F][PB];
+    auto rows = [&](int i) {
 #pragma unroll
-      for (int f = 0; f < F; ++f) {
+      for (int p = 0; p < PA; ++p)
+        fa[i & 1][p] = *reinterpret_cast<const nh8*>(at + p * PLANE + (i * 32 + l32) * RB + swap(l32, ch) * 16);
+    };
+    rows(0);
 #pragma unroll
-        for (int p = 0; p < PA; ++p) fa[p][f] = *reinterpret_cast<const nh8*>(&smem[buf][p][place(wi * W + f * 32 + l32, ch)]);
+    for (int j = 0; j < F; ++j)
 #pragma unroll
-        for (int p = 0; p < PB; ++p) fb[p][f] = *reinterpret_cast<const nh8*>(&smem[buf][PA + p][place(wj * W + f * 32 + l32, ch)]);
-      }
+      for (int p = 0; p < PB; ++p)
+        fb[j][p] = *reinterpret_cast<const nh8*>(at + (PA + p) * PLANE + (j * 32 + l32) * RB + swap(l32, ch) * 16);
 #pragma unroll
-      for (int i = 0; i < F; ++i)
+    for (int i = 0; i < F; ++i) {
+      if (i + 1 < F) rows(i + 1);
 #pragma unroll
-        for (int j = 0; j < F; ++j) {
-          if (PROD > 3) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fa[PA - 1][i], fb[PB - 1][j], acc[i][j], 0, 0, 0);
-          if (PROD > 1) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fa[PA - 1][i], fb[0][j], acc[i][j], 0, 0, 0);
-          if (PROD > 2) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fa[0][i], fb[PB - 1][j], acc[i][j], 0, 0, 0);
-          acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fa[0][i], fb[0][j], acc[i][j], 0, 0, 0);
+      for (int q = PROD - 1; q >= 0; --q) {                          // lo lo, hi lo, lo hi, hi hi: smallest first
+        constexpr int GROUPS = F * PROD;
+        const int g = i * PROD + PROD - 1 - q;
+        __builtin_amdgcn_sched_barrier(0);
+        if (BETWEEN) {
+#pragma unroll
+          for (int x = g * LOADS / GROUPS; x < (g + 1) * LOADS / GROUPS; ++x) fetch(from, x, slot);
         }
+#pragma unroll
+        for (int j = 0; j < F; ++j)
+          acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fa[i & 1][q == 3 || q == 1 ? PA - 1 : 0], fb[j][q >= 2 ? PB - 1 : 0], acc[i][j], 0, 0, 0);
+      }
+    }
+  }
+  if (BETWEEN) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  // the waves' sums, a quarter of the tile after the other; wave w keeps quarter w
+  const int wi = wave >> 1, wj = wave & 1;
+  nf16 sum[H][H];
+  float* join = (float*)smem;
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < H; ++i)
+#pragma unroll
+      for (int j = 0; j < H; ++j)
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          const nf16& v = acc[(q >> 1) * H + i][(q & 1) * H + j];
+          *reinterpret_cast<nf4*>(join + (((wave * H + i) * H + j) * 4 + g) * 256 + lane * 4) = nf4{v[g * 4], v[g * 4 + 1], v[g * 4 + 2], v[g * 4 + 3]};
+        }
+    __syncthreads();
+    if (wave == q) {
+#pragma unroll
+      for (int i = 0; i < H; ++i)
+#pragma unroll
+        for (int j = 0; j < H; ++j)
+#pragma unroll
+          for (int g = 0; g < 4; ++g) {
+            nf4 v = nf4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int w = 0; w < 4; ++w) v += *reinterpret_cast<const nf4*>(join + (((w * H + i) * H + j) * 4 + g) * 256 + lane * 4);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) sum[i][j][g * 4 + e] = v[e];
+          }
     }
   }
   // a lane's accumulators: column l32, rows 8 g + 4 half + 0..3 of the 32 x 32 part
 #pragma unroll
-  for (int i = 0; i < F; ++i)
+  for (int i = 0; i < H; ++i)
 #pragma unroll
-    for (int j = 0; j < F; ++j) {
-      const int row0 = ti * TILE + wi * W + i * 32 + half * 4, col = tj * TILE + wj * W + j * 32 + l32;
+    for (int j = 0; j < H; ++j) {
+      const int row0 = ti * TILE + (wi * H + i) * 32 + half * 4, col = tj * TILE + (wj * H + j) * 32 + l32;
       if (t.kind == NS_PARTIAL) {
         float* o = (float*)at(t.out) + (long long)split * t.mp * t.mp;
 #pragma unroll
         for (int g = 0; g < 4; ++g)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) o[(long long)(row0 + g * 8 + e) * t.mp + col] = acc[i][j][g * 4 + e] * alpha;
+          for (int e = 0; e < 4; ++e) o[(long long)(row0 + g * 8 + e) * t.mp + col] = sum[i][j][g * 4 + e] * alpha;
       } else if (t.kind == NS_FINAL) {
 #pragma unroll
         for (int g = 0; g < 4; ++g)
@@ -281,25 +338,25 @@ __global__ __launch_bounds__(256) void k_ns_gemm(NsOps s) {
           for (int e = 0; e < 4; ++e) {
             const int row = row0 + g * 8 + e;
             if (row >= t.m || col >= t.n) continue;
-            const float v = acc[i][j][g * 4 + e] * alpha;
+            const float v = sum[i][j][g * 4 + e] * alpha;
             const long long to = t.tall ? (long long)col * t.ldd + row : (long long)row * t.ldd + col;
             if (t.dtype == GLX_F32) ((float*)t.dst)[to] = v;
             else if (t.dtype == GLX_BF16) ((__bf16*)t.dst)[to] = (__bf16)v;
             else ((_Float16*)t.dst)[to] = (_Float16)v;
           }
       } else {
-        const int ldo = t.kind == NS_PLANES ? t.mp : t.np;
-        const long long po = (long long)t.mp * ldo;
+        const int ldm = ns_ld(t.mp), ldo = t.kind == NS_PLANES ? ldm : ns_ld(t.np);
+        const long long po = (long long)t.mp * ldo, px = (long long)(t.kind == NS_PLANES ? t.mp : t.np) * ldm;
         float v[16];
 #pragma unroll
-        for (int e = 0; e < 16; ++e) v[e] = acc[i][j][e] * alpha;
+        for (int e = 0; e < 16; ++e) v[e] = sum[i][j][e] * alpha;
         if (t.d) {                                             // (D is symmetric: its column's four values lie side by side)
-          const _Float16* d = (const _Float16*)at(t.d) + (long long)col * t.mp + row0;
+          const _Float16* d = (const _Float16*)at(t.d) + (long long)col * ldm + row0;
           nh4 dh[4], dl[4];
 #pragma unroll
           for (int g = 0; g < 4; ++g) {
             dh[g] = *reinterpret_cast<const nh4*>(d + g * 8);
-            dl[g] = *reinterpret_cast<const nh4*>(d + (long long)t.mp * t.mp + g * 8);
+            dl[g] = *reinterpret_cast<const nh4*>(d + (long long)t.mp * ldm + g * 8);
           }
 #pragma unroll
           for (int e = 0; e < 16; ++e) {
@@ -310,7 +367,7 @@ __global__ __launch_bounds__(256) void k_ns_gemm(NsOps s) {
         // the planes themselves, and X's transposed planes or a symmetric product's mirrored tile (the diagonal's holds both)
         const bool own = t.kind == NS_XPLANES || ti != tj;
         _Float16* o = (_Float16*)at(t.out);
-        _Float16* x = (_Float16*)at(t.kind == NS_XPLANES ? t.out2 : t.out) + (long long)col * t.mp + row0;
+        _Float16* x = (_Float16*)at(t.kind == NS_XPLANES ? t.out2 : t.out) + (long long)col * ldm + row0;
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
           nh4 h, l;
@@ -325,7 +382,7 @@ __global__ __launch_bounds__(256) void k_ns_gemm(NsOps s) {
             }
           }
           *reinterpret_cast<nh4*>(x + g * 8) = h;
-          *reinterpret_cast<nh4*>(x + po + g * 8) = l;
+          *reinterpret_cast<nh4*>(x + px + g * 8) = l;
         }
       }
     }
@@ -336,8 +393,10 @@ __global__ __launch_bounds__(256) void k_ns_join(NsOps s, int tile) {
   const int k = ns_entry(s.first, s.count);
   const NsOp& t = s.op[k];
   const long long e = (long long)(blockIdx.x - s.first[k]) * 256 + threadIdx.x, plane = (long long)t.mp * t.mp;
+  const int ld = ns_ld(t.mp);
   if (e >= plane) return;
   int r = (int)(e / t.mp), c = (int)(e - (long long)r * t.mp);
+  const long long to = (long long)r * ld + c;
   if (c / tile > r / tile) { const int x = r; r = c; c = x; }
   const float* p = (const float*)(s.ws + (size_t)t.a * 256) + (long long)r * t.mp + c;
   float v = 0.f;
@@ -346,8 +405,8 @@ __global__ __launch_bounds__(256) void k_ns_join(NsOps s, int tile) {
   _Float16 u, w;
   ns_split(v * t.scale, u, w);
   _Float16* out = (_Float16*)(s.ws + (size_t)t.out * 256);
-  out[e] = u;
-  out[plane + e] = w;
+  out[to] = u;
+  out[(long long)t.mp * ld + to] = w;
 }
 
 // ------------------------------------------------------------------------------------------------ host: programs
@@ -404,11 +463,11 @@ static NsPlan ns_plan(int rows, int cols, int dtype, int steps, size_t& at) {
   const long long total = (long long)p.m * p.n;
   p.nparts = (int)((total + 4095) / 4096);
   if (p.nparts > NS_PARTS) p.nparts = NS_PARTS;
-  const size_t X = glx_align((size_t)p.mp * p.np * 4), S = glx_align((size_t)p.mp * p.mp * 4);
+  const size_t ldn = ns_ld(p.np), ldm = ns_ld(p.mp), X = p.mp * ldn * 4, XT = p.np * ldm * 4, S = p.mp * ldm * 4;
   auto take = [&](size_t bytes) { const size_t o = at; at += glx_align(bytes); return o; };
-  p.x = take(X); p.xt = take(X); p.x2 = take(X); p.xt2 = take(X);
+  p.x = take(X); p.xt = take(XT); p.x2 = take(X); p.xt2 = take(XT);
   p.g = take(S); p.h = take(S); p.p[0] = take(S); p.p[1] = take(S); p.q[0] = take(S); p.q[1] = take(S);
-  p.part = take(p.splits > 1 ? S * p.splits : 256);
+  p.part = take(p.splits > 1 ? (size_t)p.mp * p.mp * 4 * p.splits : 256);
   p.parts = take(NS_PARTS * sizeof(double));
   p.xscale = take(NS_STEPS * sizeof(float));
   return p;
@@ -437,12 +496,13 @@ struct NsStage {               // what one launch round does, over all matrices
   void add(int tile, int prods, const NsOp& o) { gemm[tile == 128][prods - 1].push_back(o); }
 };
 
-template <int TILE>
+template <int TILE, int STAGES>
 static void ns_launch_gemm(const NsOps& s, int blocks, int prods, hipStream_t st) {
-  if (prods == 4) hipLaunchKernelGGL((k_ns_gemm<TILE, 4>), dim3(blocks), dim3(256), 0, st, s);
-  else if (prods == 1) hipLaunchKernelGGL((k_ns_gemm<TILE, 1>), dim3(blocks), dim3(256), 0, st, s);
-  else if (prods == 2) hipLaunchKernelGGL((k_ns_gemm<TILE, 2>), dim3(blocks), dim3(256), 0, st, s);
-  else hipLaunchKernelGGL((k_ns_gemm<TILE, 3>), dim3(blocks), dim3(256), 0, st, s);
+  constexpr int MORE = TILE == 128 ? 2 : 1;             // (fewer planes, more stages in the same LDS)
+  if (prods == 4) hipLaunchKernelGGL((k_ns_gemm<TILE, 4, STAGES>), dim3(blocks), dim3(256), 0, st, s);
+  else if (prods == 3) hipLaunchKernelGGL((k_ns_gemm<TILE, 3, STAGES>), dim3(blocks), dim3(256), 0, st, s);
+  else if (prods == 2) hipLaunchKernelGGL((k_ns_gemm<TILE, 2, STAGES + MORE - 1>), dim3(blocks), dim3(256), 0, st, s);
+  else hipLaunchKernelGGL((k_ns_gemm<TILE, 1, STAGES * MORE>), dim3(blocks), dim3(256), 0, st, s);
 }
 static void ns_launch_ops(std::vector<NsOp>& ops, char* ws, int tile, int prods, hipStream_t st) {       // prods = 0: joins
   for (size_t i = 0; i < ops.size(); i += NS_OPS) {
@@ -457,8 +517,9 @@ static void ns_launch_ops(std::vector<NsOp>& ops, char* ws, int tile, int prods,
       blocks += prods == 0 ? glx_divup((long long)o.mp * o.mp, 256) : (o.sym ? tm * (tm + 1) / 2 : tm * tn) * o.splits;
     }
     if (prods == 0) hipLaunchKernelGGL(k_ns_join, dim3(blocks), dim3(256), 0, st, s, tile);
-    else if (tile == 128) ns_launch_gemm<128>(s, blocks, prods, st);
-    else ns_launch_gemm<64>(s, blocks, prods, st);
+    else if (tile == 128) ns_launch_gemm<128, 2>(s, blocks, prods, st);
+    else if (blocks > 256) ns_launch_gemm<64, 2>(s, blocks, prods, st);        // two blocks per compute unit
+    else ns_launch_gemm<64, 4>(s, blocks, prods, st);
   }
 }
 
