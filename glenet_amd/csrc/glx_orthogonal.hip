@@ -188,7 +188,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1))) void k
   constexpr int F = TILE / 32, H = TILE / 64;                        // 32-wide parts: of the tile, of a quarter of it
   constexpr int CH = TILE * C / 256, LOADS = (PA + PB) * CH;         // transfers per thread: of a plane, of a stage
   constexpr int PLANE = TILE * RB, STAGE = (PA + PB) * PLANE;
-  constexpr int JOIN = 4 * H * H * 4096, BYTES = STAGES * STAGE > JOIN ? STAGES * STAGE : JOIN;       // (a quarter per wave)
+  constexpr int PIECES = TILE == 64 ? 4 : 2, JOIN = PIECES * 4 * H * H * 4096, BYTES = STAGES * STAGE > JOIN ? STAGES * STAGE : JOIN;
   __shared__ __attribute__((aligned(16))) char smem[BYTES];
   const int entry = ns_entry(s.first, s.count);
   const NsOp& t = s.op[entry];
@@ -287,37 +287,47 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1))) void k
     }
   }
   if (BETWEEN) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-  // the waves' sums, a quarter of the tile after the other; wave w keeps quarter w
+  // the waves' sums, all quarters of the tile at once (128-wide: two and two); wave w keeps quarter w
   const int wi = wave >> 1, wj = wave & 1;
   nf16 sum[H][H];
   float* join = (float*)smem;
 #pragma unroll
-  for (int q = 0; q < 4; ++q) {
+  for (int r = 0; r < 4; r += PIECES) {
     __syncthreads();
 #pragma unroll
-    for (int i = 0; i < H; ++i)
+    for (int q = r; q < r + PIECES; ++q)
+      if (wave != q) {
 #pragma unroll
-      for (int j = 0; j < H; ++j)
+        for (int i = 0; i < H; ++i)
 #pragma unroll
-        for (int g = 0; g < 4; ++g) {
-          const nf16& v = acc[(q >> 1) * H + i][(q & 1) * H + j];
-          *reinterpret_cast<nf4*>(join + (((wave * H + i) * H + j) * 4 + g) * 256 + lane * 4) = nf4{v[g * 4], v[g * 4 + 1], v[g * 4 + 2], v[g * 4 + 3]};
-        }
+          for (int j = 0; j < H; ++j)
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+              const nf16& v = acc[(q >> 1) * H + i][(q & 1) * H + j];
+              *reinterpret_cast<nf4*>(join + (((((q - r) * 4 + wave) * H + i) * H + j) * 4 + g) * 256 + lane * 4) =
+                  nf4{v[g * 4], v[g * 4 + 1], v[g * 4 + 2], v[g * 4 + 3]};
+            }
+      }
     __syncthreads();
-    if (wave == q) {
 #pragma unroll
-      for (int i = 0; i < H; ++i)
+    for (int q = r; q < r + PIECES; ++q)
+      if (wave == q) {
 #pragma unroll
-        for (int j = 0; j < H; ++j)
+        for (int i = 0; i < H; ++i)
 #pragma unroll
-          for (int g = 0; g < 4; ++g) {
-            nf4 v = nf4{0.f, 0.f, 0.f, 0.f};
+          for (int j = 0; j < H; ++j)
 #pragma unroll
-            for (int w = 0; w < 4; ++w) v += *reinterpret_cast<const nf4*>(join + (((w * H + i) * H + j) * 4 + g) * 256 + lane * 4);
+            for (int g = 0; g < 4; ++g) {
+              const nf16& own = acc[(q >> 1) * H + i][(q & 1) * H + j];
+              nf4 v = nf4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int e = 0; e < 4; ++e) sum[i][j][g * 4 + e] = v[e];
-          }
-    }
+              for (int w = 0; w < 4; ++w)
+                v += w == q ? nf4{own[g * 4], own[g * 4 + 1], own[g * 4 + 2], own[g * 4 + 3]}
+                            : *reinterpret_cast<const nf4*>(join + (((((q - r) * 4 + w) * H + i) * H + j) * 4 + g) * 256 + lane * 4);
+#pragma unroll
+              for (int e = 0; e < 4; ++e) sum[i][j][g * 4 + e] = v[e];
+            }
+      }
   }
   // a lane's accumulators: column l32, rows 8 g + 4 half + 0..3 of the 32 x 32 part
 #pragma unroll
@@ -388,25 +398,41 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1))) void k
     }
 }
 
-// the splits' sum of a Gram matrix (tiles on and below the diagonal were formed) as planes of the whole matrix
-__global__ __launch_bounds__(256) void k_ns_join(NsOps s, int tile) {
+// the splits' sum of a Gram matrix (64-wide tiles on and below the diagonal were formed) as planes of the whole matrix: a block per 16
+// rows of a tile, and the mirrored columns through LDS
+__global__ __launch_bounds__(256) void k_ns_join(NsOps s) {
+  __shared__ float tile[16][68];
   const int k = ns_entry(s.first, s.count);
   const NsOp& t = s.op[k];
-  const long long e = (long long)(blockIdx.x - s.first[k]) * 256 + threadIdx.x, plane = (long long)t.mp * t.mp;
-  const int ld = ns_ld(t.mp);
-  if (e >= plane) return;
-  int r = (int)(e / t.mp), c = (int)(e - (long long)r * t.mp);
-  const long long to = (long long)r * ld + c;
-  if (c / tile > r / tile) { const int x = r; r = c; c = x; }
-  const float* p = (const float*)(s.ws + (size_t)t.a * 256) + (long long)r * t.mp + c;
-  float v = 0.f;
-#pragma unroll 8
-  for (int q = 0; q < t.splits; ++q) v += p[q * plane];
-  _Float16 u, w;
-  ns_split(v * t.scale, u, w);
+  const int b = blockIdx.x - s.first[k], tri = b >> 2;
+  int ti = (int)((sqrtf(8.f * tri + 1.f) - 1.f) * 0.5f);
+  while ((ti + 1) * (ti + 2) / 2 <= tri) ++ti;
+  while (ti * (ti + 1) / 2 > tri) --ti;
+  const int tj = tri - ti * (ti + 1) / 2, r0 = ti * 64 + (b & 3) * 16, c0 = tj * 64, ld = ns_ld(t.mp);
+  const long long plane = (long long)t.mp * t.mp, lo = (long long)t.mp * ld;
   _Float16* out = (_Float16*)(s.ws + (size_t)t.out * 256);
-  out[to] = u;
-  out[(long long)t.mp * ld + to] = w;
+  const int r = threadIdx.x >> 4, c = (threadIdx.x & 15) * 4;
+  const float* p = (const float*)(s.ws + (size_t)t.a * 256) + (long long)(r0 + r) * t.mp + c0 + c;
+  nf4 v = nf4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll 8
+  for (int q = 0; q < t.splits; ++q) v += *reinterpret_cast<const nf4*>(p + q * plane);
+  auto put = [&](long long to, nf4 x) {
+    nh4 h, l;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      _Float16 u, w;
+      ns_split(x[e] * t.scale, u, w);
+      h[e] = u; l[e] = w;
+    }
+    *reinterpret_cast<nh4*>(out + to) = h;
+    *reinterpret_cast<nh4*>(out + lo + to) = l;
+  };
+  put((long long)(r0 + r) * ld + c0 + c, v);
+  if (ti == tj) return;
+  *reinterpret_cast<nf4*>(&tile[r][c]) = v;
+  __syncthreads();
+  const int col = threadIdx.x >> 2, rr = (threadIdx.x & 3) * 4;
+  put((long long)(c0 + col) * ld + r0 + rr, nf4{tile[rr][col], tile[rr + 1][col], tile[rr + 2][col], tile[rr + 3][col]});
 }
 
 // ------------------------------------------------------------------------------------------------ host: programs
@@ -455,7 +481,8 @@ static NsPlan ns_plan(int rows, int cols, int dtype, int steps, size_t& at) {
   if (p.seg > steps) p.seg = steps;
   const int t = p.mp / p.tile;
   const long long tiles = (long long)t * (t + 1) / 2, ksteps = p.np / NS_K;
-  long long splits = 512 / tiles;                       // two blocks per compute unit
+  // (only where a quarter of the compute units would have a tile: every part is read again by the join)
+  long long splits = p.tile == 64 && tiles <= 64 ? 256 / tiles : 1;
   if (splits > ksteps / 8) splits = ksteps / 8;         // 512 k elements a split, at least: a join costs as much as those
   if (splits < 1) splits = 1;
   p.kper = (int)((ksteps + splits - 1) / splits) * NS_K;
@@ -492,7 +519,7 @@ extern "C" size_t glx_orthogonalize_workspace_bytes(const glx_matrix* mats, int 
 }
 
 struct NsStage {               // what one launch round does, over all matrices
-  std::vector<NsOp> gemm[2][4], join[2];       // by tile; by the products per pair of operands
+  std::vector<NsOp> gemm[2][4], join;       // by tile; by the products per pair of operands
   void add(int tile, int prods, const NsOp& o) { gemm[tile == 128][prods - 1].push_back(o); }
 };
 
@@ -514,9 +541,9 @@ static void ns_launch_ops(std::vector<NsOp>& ops, char* ws, int tile, int prods,
       s.first[s.count] = blocks;
       NsOp& o = s.op[s.count++] = ops[j];
       const int tm = o.mp / tile, tn = o.np / tile;
-      blocks += prods == 0 ? glx_divup((long long)o.mp * o.mp, 256) : (o.sym ? tm * (tm + 1) / 2 : tm * tn) * o.splits;
+      blocks += prods == 0 ? tm * (tm + 1) / 2 * 4 : (o.sym ? tm * (tm + 1) / 2 : tm * tn) * o.splits;
     }
-    if (prods == 0) hipLaunchKernelGGL(k_ns_join, dim3(blocks), dim3(256), 0, st, s, tile);
+    if (prods == 0) hipLaunchKernelGGL(k_ns_join, dim3(blocks), dim3(256), 0, st, s);
     else if (tile == 128) ns_launch_gemm<128, 2>(s, blocks, prods, st);
     else if (blocks > 256) ns_launch_gemm<64, 2>(s, blocks, prods, st);        // two blocks per compute unit
     else ns_launch_gemm<64, 4>(s, blocks, prods, st);
@@ -610,7 +637,7 @@ extern "C" int glx_orthogonalize(const glx_matrix* mats, int count, int dtype, i
           stage().add(p.tile, prods, o);
           NsOp j = {};
           j.a = planes(p.part); j.out = planes(p.g); j.scale = gs; j.mp = j.np = p.mp; j.splits = (unsigned short)p.splits;
-          stage().join[p.tile == 128].push_back(j);
+          stage().join.push_back(j);
         } else {
           o.kind = NS_PLANES; o.out = planes(p.g);
           stage().add(p.tile, prods, o);
@@ -662,8 +689,8 @@ extern "C" int glx_orthogonalize(const glx_matrix* mats, int count, int dtype, i
   for (auto& g : stages) {
     for (int t = 0; t < 2; ++t) {
       for (int n = 0; n < 4; ++n) ns_launch_ops(g.gemm[t][n], ws, t ? 128 : 64, n + 1, st);
-      ns_launch_ops(g.join[t], ws, t ? 128 : 64, 0, st);
     }
+    ns_launch_ops(g.join, ws, 64, 0, st);
   }
   GLX_LAUNCH_CHECK();
   return GLX_OK;
