@@ -1,15 +1,24 @@
-"""Cross attention of stacked frames (csrc/glx_attention.hip, csrc/glx_attention_bwd.hip, bound in
-csrc/host/glx_torch.cpp), beside the operators of
-pcdet_ops.pointnet2.pointnet2_stack that gather a frame's points at query points: here every query weighs ALL of its frame's
-encoder states (points, voxels, RoI grid points; another number of them per frame) by softmax(scale q k^T).
+"""Cross attention of stacked frames (csrc/glx_attention.hip, csrc/glx_attention_bwd.hip, bound in csrc/host/glx_torch.cpp),
+beside the operators of pcdet_ops.pointnet2.pointnet2_stack that gather a frame's points at query points: here every query
+weighs ALL of its frame's encoder states (points, voxels, RoI grid points; another number of them per frame) by
+softmax(scale q k^T).
 
 Two layouts.  Stacked, as (N1 + N2 + .., H, D) with int32 counts per frame on the device (no read-back: the call can be
-recorded), or a padded batch (B, L, H, D).  key_mask says which encoder states take part; masked ones are never read."""
+recorded), or a padded batch (B, L, H, D).  key_mask says which encoder states take part; what the
+others hold, NaN included, reaches no result."""
 import math
 
 import torch
 
 from . import _lib
+
+
+def _counts(c):
+    if c.numel() == 0:
+        return c.new_zeros(1, dtype=torch.int32)              # no frames: one empty frame
+    if c.dtype == torch.int64:
+        c = c.clamp(0, 2 ** 31 - 1).to(torch.int32)
+    return c.contiguous()
 
 
 def cross_attention(q, k, v, q_batch_cnt=None, k_batch_cnt=None, key_mask=None, scale=None):
@@ -41,8 +50,7 @@ def cross_attention(q, k, v, q_batch_cnt=None, k_batch_cnt=None, key_mask=None, 
         for n, c in (("q_batch_cnt", q_batch_cnt), ("k_batch_cnt", k_batch_cnt)):
             if c is None or c.dim() != 1 or c.dtype not in (torch.int32, torch.int64) or c.shape != q_batch_cnt.shape:
                 raise ValueError("%s: %s must be an integer tensor (frames,) beside the other side's" % (who, n))
-        q_batch_cnt, k_batch_cnt = (c.to(torch.int32).contiguous() if c.numel() else c.new_zeros(1, dtype=torch.int32)
-                                    for c in (q_batch_cnt, k_batch_cnt))           # (no frames: one empty frame)
+        q_batch_cnt, k_batch_cnt = _counts(q_batch_cnt), _counts(k_batch_cnt)
     if key_mask is not None:
         if key_mask.dtype != torch.bool or key_mask.shape != k.shape[:-2]:
             raise ValueError("%s: key_mask must be bool of shape %s, got %s %s" % (who, tuple(k.shape[:-2]), key_mask.dtype, tuple(key_mask.shape)))

@@ -563,7 +563,14 @@ extern "C" int glx_orthogonalize(const glx_matrix* mats, int count, int dtype, i
               "glx_orthogonalize: these coefficients let singular values grow beyond the arithmetic's range");
   std::vector<NsPlan> plans;
   size_t need = 256;                                   // (place 0 means none)
-  for (int i = 0; i < count; ++i) plans.push_back(ns_plan(mats[i].rows, mats[i].cols, dtype, steps, need));
+  double steepest = 1.0;
+  for (double p : pmax) steepest = fmax(steepest, p);
+  for (int i = 0; i < count; ++i) {
+    plans.push_back(ns_plan(mats[i].rows, mats[i].cols, dtype, steps, need));
+    // (a segment's Gram matrix loses its error times the slope squared per step: coefficients steeper than the usual ones, whose
+    // 3.4445 keeps five bfloat16 steps below half a step of the result, take segments of one step)
+    if (steepest > 4.0) plans.back().seg = 1;
+  }
   GLX_REQUIRE(need < (1ull << 40), "glx_orthogonalize: the list needs a workspace of %zu bytes", need);
   if (!workspace || workspace_bytes < need) {
     glx_set_error("glx_orthogonalize: workspace %zu < %zu bytes", workspace_bytes, need);
@@ -604,7 +611,9 @@ extern "C" int glx_orthogonalize(const glx_matrix* mats, int count, int dtype, i
     const NsPlan& p = plans[i];
     // bfloat16: single products in the last two steps, where what they lose is no longer amplified (it comes to 1e-3 of the
     // result, half a step is 4e-3); segments of one step only
-    auto last = [&](int s1) { return dtype == GLX_BF16 && p.seg == 1 && s1 > steps - 2 && steps >= 4; };
+    auto last = [&](int s1) {
+      return dtype == GLX_BF16 && p.seg == 1 && s1 > steps - 2 && steps >= 4 && steepest <= 4.0;
+    };
     // lo lo too: fp32 matrices on 64-wide tiles, whose time is latency and LDS (small ones lose up to 1.6 times a plain fp32
     // product's error without)
     const int full = dtype == GLX_F32 && p.tile == 64 && p.xtile == 64 ? 4 : 3;

@@ -1,9 +1,10 @@
-"""Layer norm over the last dimension (csrc/glx_layernorm.hip, bound in csrc/host/glx_torch.cpp), beside the training BatchNorms of spconv.core and conv2d.
+"""Layer norm over the last dimension (csrc/glx_layernorm.hip, bound in csrc/host/glx_torch.cpp), beside the training
+BatchNorms of spconv.core and conv2d.
 
     y = (x - mean) / sqrt(var + eps) * weight + bias          (biased variance, statistics in fp32)
 
 fp32, bf16 and fp16 rows of any width; weights of the rows' type or fp32.  The backward pass gives the gradients of the rows,
-the weight and the bias in two launches with fixed summation orders: the same bits every time.  Once differentiable."""
+the weight and the bias in one or two launches with fixed summation orders: the same bits every time.  Once differentiable."""
 import torch
 from torch import nn
 

@@ -85,6 +85,12 @@ def test_other_coefficients(dev):
     m = _gradient(140, 300, 3, dev)
     for coeffs in ((1.875, -1.25, 0.375), (1.5, -0.5, 0.0), (1.0, 0.0, 0.0)):
         assert _off(orthogonalize(m, coefficients=coeffs), _exact(m, 5, coeffs)) < LIMIT[torch.float32]
+    # T_5(0.9 x), the steepest that maps [0, 1] into itself: five steps raise what is lost in X_0 by at most (max |f'|) ^ 5,
+    # |f'| = 4.5 |U_4(0.9 x)| <= 8.1 (at x = 1; 4.5 at 0, 4.5 * 1.25 between)
+    steep = (4.5, -14.58, 9.44784)
+    for dtype in (torch.float32, torch.bfloat16):
+        g = _gradient(140, 900, 4, dev, dtype)
+        assert _off(orthogonalize(g, coefficients=steep), _exact(g, 5, steep)) < 4 * 8.1 ** 5 * 2.0 ** -22 + HALF[dtype]
     o = orthogonalize(torch.randn(200, 260, device=dev), steps=30, coefficients=(1.875, -1.25, 0.375)).double()
     assert float((o @ o.t() - torch.eye(200, device=dev, dtype=torch.float64)).abs().max()) < 200 * 2.0 ** -21
 
