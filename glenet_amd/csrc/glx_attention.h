@@ -22,6 +22,7 @@ typedef short xs8 __attribute__((ext_vector_type(8)));
 struct XaArgs {
   const void *q, *k, *v, *o, *go;
   void *out, *dq, *dk, *dv;
+  __bf16 *rest;                     // (Nq, H, D) what the rounding of a 16-bit out left, or NULL
   float *lse, *delta;               // (Nq, H); lse in base 2, +inf where no key is left
   float *part;                      // splits' partial results
   const unsigned char* mask;        // (Nk) or NULL
@@ -98,6 +99,22 @@ __device__ __forceinline__ typename XaFrag<T>::vec xa_down(const char* tile, int
     return v;
   }
 }
+// + the sum of an operand's eight values
+__device__ __forceinline__ float xa_total(const XaFrag<__bf16>::vec& p, float l) {
+  typedef __bf16 b2 __attribute__((ext_vector_type(2)));
+  const b2 one = {(__bf16)1.f, (__bf16)1.f};
+#pragma unroll
+  for (int i = 0; i < 8; i += 2) l = __builtin_amdgcn_fdot2_f32_bf16(b2{p[i], p[i + 1]}, one, l, false);
+  return l;
+}
+__device__ __forceinline__ float xa_total(const XaFrag<_Float16>::vec& p, float l) {
+  typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+  const h2 one = {(_Float16)1.f, (_Float16)1.f};
+#pragma unroll
+  for (int i = 0; i < 8; i += 2) l = __builtin_amdgcn_fdot2(h2{p[i], p[i + 1]}, one, l, false);
+  return l;
+}
+__device__ __forceinline__ float xa_total(const XaFrag<float>::vec&, float l) { return l; }
 // accumulators 8 c .. 8 c + 7 as an operand
 template <typename T>
 __device__ __forceinline__ typename XaFrag<T>::vec xa_pack(const xf16& s, int c) {

@@ -6,7 +6,9 @@
 // A block is four waves: four tiles of 32 rows that share the staged keys, or, where a frame has few rows, ONE tile whose
 // waves take the staged keys in turn and are joined at the end.  Few tiles are split over the keys as well; the splits' results
 // (O unnormalised, m, l) are joined by a second launch.  Scores, m, l and O are fp32; for 16-bit inputs p is rounded to their
-// type in front of the second product (each to half a step, unbiased: below the rounding of O itself).
+// type in front of the second product (each to half a step, unbiased: below the rounding of O itself).  O is divided by the sum
+// of the ROUNDED p -- a row that one key dominates is then as exact as that key's value -- and the log-sum-exp, from which the
+// backward pass forms p again in fp32, is that of the unrounded ones.
 #include "glx_attention.h"
 
 template <typename T, int DP, int RW>
@@ -18,7 +20,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(xa_waves<T,
   constexpr int JB = KW > 1 ? 4 * 32 * (DP + 1) * 4 : 0;
   constexpr int BYTES = 4 * TB > JB ? 4 * TB : JB;
   __shared__ __attribute__((aligned(16))) char smem[BYTES];
-  __shared__ float sm[4][32], sl[4][32];
+  __shared__ float sm[4][32], sl[4][32], slr[4][32];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5, l32 = lane & 31;
   const int rw = wave / KW, kw = wave % KW;
   const int hk = blockIdx.y;
@@ -46,7 +48,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(xa_waves<T,
 #pragma unroll
   for (int i = 0; i < DT; ++i) O[i] = (xf16)(0.f);
   const float scale2 = fabsf(a.scale2);
-  float m = -INFINITY, l = 0.f;                               // m unscaled
+  float m = -INFINITY, l = 0.f, lr = 0.f;                     // m unscaled; sums of p, of the rounded p (16-bit)
   XaLoad<T, DP, BN> kl, vl;
   const bool kdma = a.dma & 2, vdma = a.dma & 4;
   auto koff = [&](int r) { return (long long)r * a.sk; };
@@ -112,6 +114,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(xa_waves<T,
         const float now = fmaxf(m, top), shrink = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((m - now) * scale2);
         m = now;
         l *= shrink;
+        lr *= shrink;
 #pragma unroll
         for (int i = 0; i < DT; ++i)
 #pragma unroll
@@ -132,6 +135,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(xa_waves<T,
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
           const typename XaFrag<T>::vec p = xa_pack<T>(s[u], c);
+          lr = xa_total(p, lr);
 #pragma unroll
           for (int i = 0; i < DT; ++i) xa_mma(O[i], xa_down<T, DP>(tv, (u * KW + kw) * 32 + c * 16, i * 32, lane), p);
         }
@@ -143,9 +147,11 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(xa_waves<T,
     buf ^= 1;
   }
   l += __shfl_xor(l, 32, 64);
+  if (sizeof(T) == 2) lr += __shfl_xor(lr, 32, 64);
+  else lr = l;
   m = m == -INFINITY ? m : m * scale2;
   if (KW > 1) {                                               // the waves of a row tile, joined in order
-    if (half == 0) { sm[wave][l32] = m; sl[wave][l32] = l; }
+    if (half == 0) { sm[wave][l32] = m; sl[wave][l32] = l; slr[wave][l32] = lr; }
     __syncthreads();
     float top = -INFINITY;
 #pragma unroll
@@ -153,15 +159,19 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(xa_waves<T,
     const float at = top == -INFINITY ? 0.f : top;
     float* x = (float*)smem + wave * 32 * (DP + 1);
     const float w = __builtin_amdgcn_exp2f(m - at);
-    float all = 0.f;
+    float all = 0.f, allr = 0.f;
 #pragma unroll
-    for (int i = 0; i < KW; ++i) all += sl[rw * KW + i][l32] * exp2f(sm[rw * KW + i][l32] - at);
+    for (int i = 0; i < KW; ++i) {
+      const float u = exp2f(sm[rw * KW + i][l32] - at);
+      all += sl[rw * KW + i][l32] * u;
+      allr += slr[rw * KW + i][l32] * u;
+    }
 #pragma unroll
     for (int i = 0; i < DT; ++i)
 #pragma unroll
       for (int e = 0; e < 16; ++e) x[l32 * (DP + 1) + i * 32 + (e >> 2) * 8 + half * 4 + (e & 3)] = O[i][e] * w;
     __syncthreads();
-    m = top; l = all;
+    m = top; l = all; lr = allr;
     if (kw == 0) {
 #pragma unroll
       for (int i = 0; i < DT; ++i)
@@ -178,18 +188,18 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(xa_waves<T,
   if (!live || kw != 0) return;
   const long long at = (f.q0 + qi) * a.heads + head;
   if (a.splits > 1) {
-    float* part = a.part + ((long long)split * a.nq * a.heads + at) * (a.dim + 2);
+    float* part = a.part + ((long long)split * a.nq * a.heads + at) * (a.dim + 3);
 #pragma unroll
     for (int i = 0; i < DT; ++i)
 #pragma unroll
       for (int e = 0; e < 16; ++e) {
         const int d = i * 32 + (e >> 2) * 8 + half * 4 + (e & 3);
-        if (d < a.dim) part[2 + d] = O[i][e];
+        if (d < a.dim) part[3 + d] = O[i][e];
       }
-    if (half == 0) { part[0] = m; part[1] = l; }
+    if (half == 0) { part[0] = m; part[1] = l; part[2] = lr; }
     return;
   }
-  const float inv = l == 0.f ? 0.f : 1.f / l;
+  const float inv = lr == 0.f ? 0.f : 1.f / lr;
   T* out = (T*)a.out + at * a.dim;
 #pragma unroll
   for (int i = 0; i < DT; ++i)
@@ -204,6 +214,17 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(xa_waves<T,
 #pragma unroll
         for (int e = 0; e < 4; ++e)
           if (d + e < a.dim) out[d + e] = v[e];
+      if (sizeof(T) == 2 && a.rest) {
+        __bf16* rest = a.rest + at * a.dim;
+        GlxVec<__bf16, 4>::vec w;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) w[e] = (__bf16)(O[i][g * 4 + e] * inv - (float)v[e]);
+        if (d + 4 <= a.dim) GlxVec<__bf16, 4>::store(rest + d, w);
+        else
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (d + e < a.dim) rest[d + e] = w[e];
+      }
     }
   if (a.lse && half == 0) a.lse[at] = l == 0.f ? INFINITY : m + log2f(l);
 }
@@ -214,23 +235,29 @@ __global__ __launch_bounds__(256) void k_xa_join(XaArgs a) {
   const long long at = (long long)blockIdx.x * 4 + (threadIdx.x >> 6), rows = a.nq * a.heads;
   const int lane = threadIdx.x & 63;
   if (at >= rows) return;
-  const long long step = rows * (a.dim + 2);
-  const float* part = a.part + at * (a.dim + 2);
+  const long long step = rows * (a.dim + 3);
+  const float* part = a.part + at * (a.dim + 3);
   float top = -INFINITY;
   for (int s = lane; s < a.splits; s += 64) top = fmaxf(top, part[s * step]);
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o, 64));
   const float base = top == -INFINITY ? 0.f : top;
-  float l = 0.f;
-  for (int s = lane; s < a.splits; s += 64) l += part[s * step + 1] * exp2f(part[s * step] - base);
+  float l = 0.f, lr = 0.f;
+  for (int s = lane; s < a.splits; s += 64) {
+    const float u = exp2f(part[s * step] - base);
+    l += part[s * step + 1] * u;
+    lr += part[s * step + 2] * u;
+  }
 #pragma unroll
-  for (int o = 32; o > 0; o >>= 1) l += __shfl_xor(l, o, 64);
-  const float inv = l == 0.f ? 0.f : 1.f / l;
+  for (int o = 32; o > 0; o >>= 1) { l += __shfl_xor(l, o, 64); lr += __shfl_xor(lr, o, 64); }
+  const float inv = lr == 0.f ? 0.f : 1.f / lr;
   for (int d = lane; d < a.dim; d += 64) {
     float v = 0.f;
 #pragma unroll 4
-    for (int s = 0; s < a.splits; ++s) v += part[s * step + 2 + d] * exp2f(part[s * step] - base);
-    ((T*)a.out)[at * a.dim + d] = (T)(v * inv);
+    for (int s = 0; s < a.splits; ++s) v += part[s * step + 3 + d] * exp2f(part[s * step] - base);
+    const T o = (T)(v * inv);
+    ((T*)a.out)[at * a.dim + d] = o;
+    if (sizeof(T) == 2 && a.rest) a.rest[at * a.dim + d] = (__bf16)(v * inv - (float)o);
   }
   if (a.lse && lane == 0) a.lse[at] = l == 0.f ? INFINITY : top + log2f(l);
 }
@@ -278,7 +305,7 @@ int xa_check(const char* who, const glx_attention* t) {
 }
 XaArgs xa_args(const glx_attention* t) {
   XaArgs a = {};
-  a.q = t->q; a.k = t->k; a.v = t->v; a.out = t->out; a.o = t->out; a.lse = t->lse; a.mask = t->key_mask;
+  a.q = t->q; a.k = t->k; a.v = t->v; a.out = t->out; a.o = t->out; a.lse = t->lse; a.rest = (__bf16*)t->out_rest; a.mask = t->key_mask;
   a.qcnt = t->q_cnt; a.kcnt = t->k_cnt;
   a.sq = t->q_stride; a.hq = t->q_head_stride; a.sk = t->k_stride; a.hk = t->k_head_stride; a.sv = t->v_stride; a.hv = t->v_head_stride;
   a.nq = t->q_rows; a.nk = t->k_rows;
@@ -295,7 +322,7 @@ XaArgs xa_args(const glx_attention* t) {
 extern "C" size_t glx_attention_workspace_bytes(const glx_attention* t) {
   if (xa_check("glx_attention_workspace_bytes", t) != GLX_OK) return 0;
   const XaForward p = xa_forward_plan(t);
-  return glx_align(p.splits > 1 ? (size_t)p.splits * t->q_rows * t->heads * (t->dim + 2) * sizeof(float) : 0) + 256;
+  return glx_align(p.splits > 1 ? (size_t)p.splits * t->q_rows * t->heads * (t->dim + 3) * sizeof(float) : 0) + 256;
 }
 
 template <typename T, int DP>

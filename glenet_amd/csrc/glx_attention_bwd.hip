@@ -12,6 +12,11 @@
 // keys P sits where fp16 has few bits left, and dS inherits the loss' scale -- so P is multiplied by 2^12 and dS by a power of
 // two that keeps a wave's largest value between 2^8 and 2^15 (taken from the first tile, lowered with the accumulators when a
 // later tile would pass it).
+//
+// dS sums to zero over a row, so what the keys of a row have in common leaves dQ, but the roundings of dS times it stay.  With few
+// channels the scores pull a row's keys together: at dim 8, 4 x 4012 x 2768, 2 heads, bf16, dQ was 2.7e-3 off (the rounding of
+// the result alone: 1.7e-3).  Heads of up to 32 channels, whose time is the exponentials, so add what the rounding left in a
+// second product (there 201 -> 208 us a training pass, and dQ below 2.4e-3); wider ones do not.
 #include "glx_attention.h"
 
 #include <type_traits>
@@ -72,7 +77,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(xa_waves<T,
   const XaPlace f = xa_place(a, blockIdx.x / a.splits, RW * 32, false);
   if (f.tile < 0) return;
   const int rows = f.nq * a.group, row = f.tile * RW * 32 + rw * 32 + l32;
-  const int tiles = a.dq ? (f.nk + BN - 1) / BN : 0;
+  const int tiles = (f.nk + BN - 1) / BN;
   const int t0 = (int)((long long)tiles * split / a.splits), t1 = (int)((long long)tiles * (split + 1) / a.splits);
   const bool live = row < rows;
   const int qi = live ? row / a.group : 0, head = hk * a.group + (live ? row - qi * a.group : 0);
@@ -80,11 +85,14 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(xa_waves<T,
   const T* kbase = (const T*)a.k + f.k0 * a.sk + hk * a.hk;
   const T* vbase = (const T*)a.v + f.k0 * a.sv + hk * a.hv;
   typename XaFrag<T>::vec Q[KS], G[KS];
+  // a frame of few keys: delta is formed below from the row's own P and dP, and is exact where the softmax has one key
+  const bool few = f.nk <= 32;
   float delta = 0.f;
   {
     const T* p = (const T*)a.q + (f.q0 + qi) * a.sq + head * a.hq;
     const T* g = (const T*)a.go + (f.q0 + qi) * a.sg + head * a.hg;
     const T* o = (const T*)a.o + at * a.dim;
+    const __bf16* rest = a.rest + at * a.dim;
 #pragma unroll
     for (int s = 0; s < KS; ++s) {
       Q[s] = G[s] = typename XaFrag<T>::vec{};
@@ -94,13 +102,18 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(xa_waves<T,
       const typename XaFrag<T>::vec x = xa_row<T>(o, s * 16 + half * 8, a.dim);
 #pragma unroll
       for (int i = 0; i < 8; ++i) delta += (float)G[s][i] * (float)x[i];
+      if (sizeof(T) == 2 && a.rest) {
+        const XaFrag<__bf16>::vec y = xa_row<__bf16>(rest, s * 16 + half * 8, a.dim);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) delta += (float)G[s][i] * (float)y[i];
+      }
     }
     delta += __shfl_xor(delta, 32, 64);
   }
   const float lse = live ? a.lse[at] : INFINITY;
   if (lse == INFINITY) delta = 0.f;                           // a row without keys: no gradient, whatever dO holds
-  if (live && kw == 0 && half == 0 && split == 0) a.delta[at] = delta;
-  if (!a.dq) return;
+  if (live && kw == 0 && half == 0 && split == 0 && !(few && lse != INFINITY)) a.delta[at] = delta;
+  if (!a.dq && !few) return;
   xf16 D[DT];
 #pragma unroll
   for (int i = 0; i < DT; ++i) D[i] = (xf16)(0.f);
@@ -129,6 +142,28 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(xa_waves<T,
   ok[0] = nok[0]; ok[1] = nok[1];
   __syncthreads();
   int buf = 0;
+  if (few && kw == 0 && t0 < t1 && (unsigned)ok[0]) {
+    const unsigned valid = (unsigned)ok[0], mine = valid >> (half * 4);
+    const bool one = (valid & (valid - 1)) == 0;
+    xf16 s = (xf16)(0.f), d = (xf16)(0.f);
+#pragma unroll
+    for (int k = 0; k < KS; ++k) {
+      xa_mma(s, xa_along<T, DP>(smem, l32, k, half), Q[k]);
+      xa_mma(d, xa_along<T, DP>(smem + TB, l32, k, half), G[k]);
+    }
+    float x = 0.f, y = 0.f;
+#pragma unroll
+    for (int i = 0; i < 16; ++i)
+      if ((mine >> ((i >> 2) * 8 + (i & 3))) & 1) {
+        const float p = one ? 1.f : __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], a.scale2, -lse));
+        x += p * d[i];
+        y += p;
+      }
+    x += __shfl_xor(x, 32, 64);
+    y += __shfl_xor(y, 32, 64);
+    delta = y > 0.f ? x / y : 0.f;
+    if (live && half == 0 && lse != INFINITY) a.delta[at] = delta;
+  }
   for (int t = t0; t < t1; ++t) {
     const bool more = t + 1 < t1;
     char* next = smem + (buf ^ 1) * 2 * TB;
@@ -157,6 +192,12 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(xa_waves<T,
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
           const typename XaFrag<T>::vec p = xa_pack<T>(s, c);
+          if constexpr (sizeof(T) == 2 && DP == 32) {         // what the rounding of dS left (above)
+            xf16 rest;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) rest[i] = s[c * 8 + i] - (float)p[i];
+            xa_mma(D[0], xa_down<T, DP>(tk, c0 + c * 16, 0, lane), xa_pack<T>(rest, 0));
+          }
 #pragma unroll
           for (int i = 0; i < DT; ++i) xa_mma(D[i], xa_down<T, DP>(tk, c0 + c * 16, i * 32, lane), p);
         }
@@ -191,7 +232,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(xa_waves<T,
         }
     }
   }
-  if (!live || kw != 0) return;
+  if (!live || kw != 0 || !a.dq) return;
   float* part = a.part + ((long long)split * a.nq * a.heads + at) * a.dim;
   T* out = (T*)a.dq + at * a.dim;
 #pragma unroll

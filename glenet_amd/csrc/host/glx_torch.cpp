@@ -144,9 +144,9 @@ Stack stack_of(const Tensor& t) {
 }
 
 glx_attention describe(const Stack& q, const Stack& k, const Stack& v, const Tensor& qc, const Tensor& kc, const Tensor& mask,
-                       double scale, const Tensor& out, const Tensor& lse) {
+                       double scale, const Tensor& out, const Tensor& rest, const Tensor& lse) {
   glx_attention a = {};
-  a.q = ptr(q.t); a.k = ptr(k.t); a.v = ptr(v.t); a.out = ptr(out); a.lse = (float*)ptr(lse);
+  a.q = ptr(q.t); a.k = ptr(k.t); a.v = ptr(v.t); a.out = ptr(out); a.out_rest = ptr(rest); a.lse = (float*)ptr(lse);
   a.key_mask = (const uint8_t*)ptr(mask);
   a.q_cnt = (const int32_t*)ptr(qc); a.k_cnt = (const int32_t*)ptr(kc);
   a.heads = (int)q.t.size(-2); a.kv_heads = (int)k.t.size(-2); a.dim = (int)q.t.size(-1);
@@ -163,12 +163,13 @@ glx_attention describe(const Stack& q, const Stack& k, const Stack& v, const Ten
 }
 
 Tensor xa_forward(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& qc, const Tensor& kc, const Tensor& mask,
-                  double scale, Tensor* lse) {
+                  double scale, Tensor* rest, Tensor* lse) {
   at::DeviceGuard guard(q.device());
   Tensor out = at::empty(q.sizes(), q.options());
   if (lse) *lse = at::empty(q.sizes().slice(0, q.dim() - 1), q.options().dtype(at::kFloat));
+  if (rest && q.scalar_type() != at::kFloat) *rest = at::empty(q.sizes(), q.options().dtype(at::kBFloat16));
   const Stack sq = stack_of(q), sk = stack_of(k), sv = stack_of(v);
-  const glx_attention a = describe(sq, sk, sv, qc, kc, mask, scale, out, lse ? *lse : Tensor());
+  const glx_attention a = describe(sq, sk, sv, qc, kc, mask, scale, out, rest ? *rest : Tensor(), lse ? *lse : Tensor());
   const size_t n = E.xa_bytes(&a);
   const Tensor ws = n > 256 ? bytes(n, q) : Tensor();
   check(E.xa_forward(&a, ptr(ws), n, stream(q)), "glx_attention_forward");
@@ -179,9 +180,9 @@ struct CrossAttention : public torch::autograd::Function<CrossAttention> {
   static Tensor forward(AutogradContext* ctx, const Tensor& q, const Tensor& k, const Tensor& v, const std::optional<Tensor>& q_cnt,
                         const std::optional<Tensor>& k_cnt, const std::optional<Tensor>& key_mask, double scale) {
     const Tensor qc = q_cnt.value_or(Tensor()), kc = k_cnt.value_or(Tensor()), mask = key_mask.value_or(Tensor());
-    Tensor lse;
-    Tensor out = xa_forward(q, k, v, qc, kc, mask, scale, &lse);
-    ctx->save_for_backward({q, k, v, qc, kc, mask, out, lse});
+    Tensor rest, lse;
+    Tensor out = xa_forward(q, k, v, qc, kc, mask, scale, &rest, &lse);
+    ctx->save_for_backward({q, k, v, qc, kc, mask, out, lse, rest});
     ctx->saved_data["s"] = scale;
     ctx->saved_data["g"] = (int64_t)(wanted(q) | wanted(k) << 1 | wanted(v) << 2);
     return out;
@@ -196,7 +197,7 @@ struct CrossAttention : public torch::autograd::Function<CrossAttention> {
     for (int i = 0; i < 3; ++i)
       if ((want >> i & 1) && ctx->needs_input_grad(i)) grads[i] = at::empty(saved[i].sizes(), saved[i].options());
     const Stack sq = stack_of(q), sk = stack_of(saved[1]), sv = stack_of(saved[2]), sg = stack_of(g[0]);
-    const glx_attention a = describe(sq, sk, sv, saved[3], saved[4], saved[5], ctx->saved_data["s"].toDouble(), saved[6], saved[7]);
+    const glx_attention a = describe(sq, sk, sv, saved[3], saved[4], saved[5], ctx->saved_data["s"].toDouble(), saved[6], saved[8], saved[7]);
     const size_t n = E.xa_backward_bytes(&a);
     const Tensor ws = bytes(n, q);
     check(E.xa_backward(&a, ptr(sg.t), sg.row, sg.head, ptr(grads[0]), ptr(grads[1]), ptr(grads[2]), ptr(ws), n, stream(q)),
@@ -209,7 +210,7 @@ Tensor cross_attention(const Tensor& q, const Tensor& k, const Tensor& v, const 
                        const std::optional<Tensor>& k_cnt, const std::optional<Tensor>& key_mask, double scale) {
   const Tensor qc = q_cnt.value_or(Tensor()), kc = k_cnt.value_or(Tensor()), mask = key_mask.value_or(Tensor());
   if (at::GradMode::is_enabled() && (wanted(q) || wanted(k) || wanted(v))) return CrossAttention::apply(q, k, v, q_cnt, k_cnt, key_mask, scale);
-  return xa_forward(q, k, v, qc, kc, mask, scale, nullptr);
+  return xa_forward(q, k, v, qc, kc, mask, scale, nullptr, nullptr);
 }
 
 }  // namespace

@@ -1531,11 +1531,13 @@ int glx_muon_apply(float* params, const float* update, const glx_opt_chunk* chun
  * dim), k / v (k_rows, kv_heads, dim) of `dtype` with unit stride inside a head and the given strides (elements) between rows
  * and heads; heads / kv_heads query heads share a key head.  Frames lie behind each other: q_cnt / k_cnt (frames) int32 DEVICE
  * counts (clamped into the tensors; rows behind the last frame give zeros), or both NULL and q_len / k_len rows per frame.
- * key_mask (k_rows) bytes, 0 = not attended and never read; NULL: none.  A row without keys gives 0.  lse (q_rows, heads) fp32:
- * the rows' base-2 log-sum-exp for the backward pass (+inf without keys), NULL: inference.  dim 1 .. 128. */
+ * key_mask (k_rows) bytes, 0 = not attended, whatever the state holds; NULL: none.  A row without keys gives 0.  For the
+ * backward pass, NULL: inference: lse (q_rows, heads) fp32, the rows' base-2 log-sum-exp (+inf without keys); out_rest (like out,
+ * bf16; 16-bit dtypes only) what the rounding of out left, without which gradients of rows that one key dominates are off by
+ * that rounding.  dim 1 .. 128. */
 typedef struct glx_attention {
   const void* q; const void* k; const void* v;
-  void* out; float* lse;
+  void* out; void* out_rest; float* lse;
   const uint8_t* key_mask;
   const int32_t* q_cnt; const int32_t* k_cnt;
   int64_t q_rows, k_rows, q_len, k_len;

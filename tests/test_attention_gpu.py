@@ -33,6 +33,9 @@ CASES = [
     ([4, 4], [3000, 900], 2, 1, 96, True, False),
     ([700, 650], [40, 33], 4, 2, 64, False, False),
     ([9, 3], [50, 70], 3, 1, 1, False, False),
+    ([50, 37], [140, 260], 6, 2, 32, True, False),             # three heads share one: tiles hold whole queries
+    ([3, 7], [200, 31], 70, 1, 16, False, False),              # more heads share one than a tile has rows
+    ([1], [129], 128, 2, 128, False, True),
 ]
 
 
@@ -385,3 +388,67 @@ def test_an_attention_block_trained_with_muon(dev):
     opt.step()
     for n, p in net.named_parameters():
         assert bool(torch.isfinite(p).all()) and not torch.equal(p, before[n])
+
+
+def test_negative_scale_and_64_bit_counts(dev):
+    case = ([25, 40], [70, 300], 4, 2, 24, True, False)
+    for dtype in (torch.float32, torch.bfloat16):
+        q, k, v, go, mask, cnts = _inputs(case, dtype, 6, dev)
+        outs = _run(q, k, v, go, mask, cnts, scale=-0.3)
+        ref = _reference(q, k, v, go, mask, case, dtype, scale=-0.3)
+        for t, n in zip(outs, ("o", "dq", "dk", "dv")):
+            _check(t, ref, n, dtype)
+        wide = tuple(c.long() for c in cnts)
+        wide[1][1] += 1 << 32                                 # beyond 32 bits: cut at the tensor's end, not wrapped
+        for a, b in zip(_run(q, k, v, go, mask, wide, scale=-0.3), outs):
+            assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("h,hk,d", [(4, 2, 16), (2, 2, 128), (14, 2, 72)])
+def test_rows_with_one_key_have_no_score_gradient(dev, h, hk, d, dtype):
+    """softmax of one score is 1 whatever the score: dq is 0, and dk (frames of one key), to the bit; o and dv are v and sum go."""
+    case = ([5, 300, 40], [1, 1, 20], h, hk, d, False, False)
+    q, k, v, go, _, cnts = _inputs(case, dtype, 9, dev)
+    mask = torch.ones(k.shape[0], dtype=torch.bool, device=dev)
+    mask[2:] = False
+    mask[11] = True                                           # the third frame: one of 20
+    o, dq, dk, dv = _run(q, k, v, go, mask, cnts)
+    assert not dq.any() and not dk.any()
+    at = torch.tensor([0] * 5 + [1] * 300 + [11] * 40, device=dev)
+    assert torch.equal(o, v[at].repeat_interleave(h // hk, 1))
+    for i, (a, b) in {0: (0, 5), 1: (5, 305), 11: (305, 345)}.items():
+        want = go[a:b].double().view(b - a, hk, h // hk, d)
+        # (P is 1 to the rounding of s and lse: |s| a few units)
+        lim = (HALF[dtype] + (40 + 300) * U) * want.abs().sum((0, 2)) + SUB[dtype]
+        assert bool(((dv[i].double() - want.sum((0, 2))).abs() <= lim).all())
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("lk", [20, 700])
+def test_gradients_of_rows_that_one_key_dominates(dev, lk, dtype):
+    """One key's weight is 1 - 1e-3: dS is a thousandth of P dP, so what o loses to its type must not reach delta = sum go o.  The
+    p's roundings move delta by h sum |dS| (o is divided by their own sum), o's by h^2 sum |go o| (its rest is kept)."""
+    g = torch.Generator().manual_seed(lk)
+    d, lq, h = 64, 50, 2
+    k, v, go = (torch.randn(n, h, d, generator=g).to(dtype).to(dev) for n in (lk, lk, lq))
+    near = torch.randint(0, lk, (lq,), generator=g).to(dev)
+    top = math.log(1000.0 * lk)
+    q = (k[near].double() * (top * math.sqrt(d) / (k[near].double() ** 2).sum(-1, keepdim=True))).to(dtype)
+    cnts = tuple(torch.tensor([n], dtype=torch.int32, device=dev) for n in (lq, lk))
+    _, dq, _, _ = _run(q, k, v, go, None, cnts)
+    u, scale = HALF[dtype], 1 / math.sqrt(d)
+    for j in range(h):
+        qq, kk, vv, gg = (t[:, j].double() for t in (q, k, v, go))
+        p = torch.softmax(qq @ kk.t() * scale, 1)
+        o = p @ vv
+        ds = p * (gg @ vv.t() - (gg * o).sum(1, keepdim=True))
+        want = scale * ds @ kk
+        low = 1.1 * u * ds.abs().sum(1, keepdim=True) + 1.1 * u * u * (gg.abs() * o.abs()).sum(1, keepdim=True)
+        # (fp32 sums and scores: the limits of the general test, without its rounding of o)
+        es = (2 * d + 40) * U * (qq.abs() @ kk.abs().t()).amax(1, keepdim=True) * scale * 3
+        fine = (2 * d + 40) * U * (gg.abs() @ vv.abs().t() + (gg.abs() * o.abs()).sum(1, keepdim=True)) + 2 * es * (gg @ vv.t()).abs().amax(1, keepdim=True)
+        lim = scale * ((1.1 * u * ds.abs() + p * (low + fine) + 2 * es * ds.abs()) @ kk.abs()) + u * want.abs() + SUB[dtype]
+        if dtype == torch.float16:
+            lim = lim + scale * 2.0 ** -24 * ds.abs().max() * kk.abs().sum(0)
+        assert bool(((dq[:, j].double() - want).abs() <= lim).all())
