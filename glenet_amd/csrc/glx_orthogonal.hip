@@ -1,4 +1,5 @@
-// Orthogonalised updates (glenet_amd/optim.py): Newton-Schulz steps on a list of matrices of any shapes, few launches for all.
+// Orthogonalised updates (glenet_amd/optim.py): Newton-Schulz steps on a list of matrices of any shapes, few launches for all.  Matrices of up
+// to 16 rows have a kernel of their own, further down; what follows is about the others.
 //
 //   X = G / (|G|_F + eps), transposed where G has more rows than columns (X: m x n, m <= n);  per step
 //   A = X X^T,  X <- a X + (b A + c A^2) X  =  P X,  P = a I + b A + c A^2
@@ -24,6 +25,8 @@
 #define NS_K 64                // the k range of a split comes in multiples of this
 #define NS_OPS 39              // products of one launch (kernel arguments: 96 bytes each)
 #define NS_MATS 40             // matrices of one prologue launch
+#define NS_SMALLS 64           // matrices of one launch of the small ones
+#define NS_AHEAD 4             // 16-column pieces that each of their 16 waves has on their way
 #define NS_STEPS 64            // at most
 #define NS_PARTS 1024          // partial sums of squares per matrix, at most
 
@@ -435,6 +438,111 @@ __global__ __launch_bounds__(256) void k_ns_join(NsOps s) {
   put((long long)(c0 + col) * ld + r0 + rr, nf4{tile[rr][col], tile[rr + 1][col], tile[rr + 2][col], tile[rr + 3][col]});
 }
 
+// ------------------------------------------------------------------------------------------------ matrices of up to 16 rows
+// One block per matrix, all of it in one launch and in 64 bits: A = X X^T on the fp64 matrix units (one value per lane is both
+// operands), the steps on the 16 x 16 polynomials, X <- Q X.  Few singular values leave nothing to average: on the split products
+// above such a matrix came out up to 3.9 times as far off as with plain fp32 arithmetic (here: 6e-8 of it, a tenth of that), and
+// its some 15 launches were all latency.  Bound by the fp64 matrix units (14 us of 56 at 16 x 4096) and one CU's loads.
+typedef double nd4 __attribute__((ext_vector_type(4)));
+struct NsSmall { const void* src; void* dst; long long ld_src, ld_dst; int rows, cols; };
+struct NsSmalls { NsSmall mat[NS_SMALLS]; double c[3], eps; int steps, dtype; };
+static_assert(sizeof(NsSmalls) <= 4032, "kernel arguments");
+
+__global__ __launch_bounds__(1024) void k_ns_small(NsSmalls s) {
+  __shared__ double part[16][16][17], A[16][17], P[16][17], H[16][17], Q[2][16][17];
+  const NsSmall& t = s.mat[blockIdx.x];
+  const bool tall = t.rows > t.cols;
+  const int m = tall ? t.cols : t.rows, n = tall ? t.rows : t.cols;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i = lane & 15, kq = lane >> 4;
+  const int r = threadIdx.x >> 4 & 15, c = threadIdx.x & 15;
+  const bool first = threadIdx.x < 256;                        // a thread per entry of the 16 x 16 matrices
+  auto run = [&](auto* src) {
+    typedef __remove_cvref(decltype(*src)) T;
+    const long long down = tall ? 1 : t.ld_src, along = tall ? t.ld_src : 1;
+    // of X, before the division by its norm (no branch around the load: many are on their way at once)
+    auto load = [&](int row, int col) { return (float)src[(row < m ? row : 0) * down + (col < n ? col : 0) * along]; };
+    auto there = [&](int row, int col, float v) { return row < m && col < n ? (double)v : 0.0; };
+    nd4 acc = {0.0, 0.0, 0.0, 0.0};
+    for (int k0 = wave * 16; k0 < n; k0 += 256 * NS_AHEAD) {
+      float v[NS_AHEAD][4];
+#pragma unroll
+      for (int a = 0; a < NS_AHEAD; ++a)
+#pragma unroll
+        for (int u = 0; u < 4; ++u) v[a][u] = load(i, k0 + a * 256 + kq * 4 + u);
+#pragma unroll
+      for (int a = 0; a < NS_AHEAD; ++a)
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          const double x = there(i, k0 + a * 256 + kq * 4 + u, v[a][u]);
+          acc = __builtin_amdgcn_mfma_f64_16x16x4f64(x, x, acc, 0, 0, 0);
+        }
+    }
+#pragma unroll
+    for (int u = 0; u < 4; ++u) part[wave][u * 4 + kq][i] = acc[u];
+    __syncthreads();
+    if (first) {
+      double v = 0.0;
+#pragma unroll
+      for (int w = 0; w < 16; ++w) v += part[w][r][c];
+      A[r][c] = v;
+    }
+    __syncthreads();
+    double square = 0.0;
+#pragma unroll
+    for (int u = 0; u < 16; ++u) square += A[u][u];            // |G|_F^2
+    const double inv = 1.0 / (sqrt(square) + s.eps);
+    __syncthreads();
+    if (first) {
+      A[r][c] = A[r][c] * inv * inv;
+      Q[0][r][c] = r == c ? 1.0 : 0.0;
+    }
+    __syncthreads();
+    auto product = [&](const double (*x)[17], const double (*y)[17]) {
+      double v = 0.0;
+#pragma unroll
+      for (int u = 0; u < 16; ++u) v += x[r][u] * y[u][c];
+      return v;
+    };
+    int q = 0;
+    for (int step = 0; step < s.steps; ++step, q ^= 1) {
+      if (first) P[r][c] = (r == c ? s.c[0] : 0.0) + s.c[1] * A[r][c] + s.c[2] * product(A, A);
+      __syncthreads();
+      if (first) {
+        Q[q ^ 1][r][c] = product(P, Q[q]);
+        H[r][c] = product(P, A);
+      }
+      __syncthreads();
+      if (first) A[r][c] = product(H, P);
+      __syncthreads();
+    }
+    double z[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) z[u] = Q[q][i][u * 4 + kq] * inv;
+    for (int j0 = wave * 16; j0 < n; j0 += 256 * NS_AHEAD) {
+      float v[NS_AHEAD][4];
+#pragma unroll
+      for (int a = 0; a < NS_AHEAD; ++a)
+#pragma unroll
+        for (int u = 0; u < 4; ++u) v[a][u] = load(u * 4 + kq, j0 + a * 256 + i);
+#pragma unroll
+      for (int a = 0; a < NS_AHEAD; ++a) {
+        const int col = j0 + a * 256 + i;
+        nd4 x = {0.0, 0.0, 0.0, 0.0};
+#pragma unroll
+        for (int u = 0; u < 4; ++u) x = __builtin_amdgcn_mfma_f64_16x16x4f64(z[u], there(u * 4 + kq, col, v[a][u]), x, 0, 0, 0);
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          const int row = u * 4 + kq;
+          if (row < m && col < n) ((T*)t.dst)[tall ? col * t.ld_dst + row : row * t.ld_dst + col] = (T)(float)x[u];
+        }
+      }
+    }
+  };
+  if (s.dtype == GLX_F32) run((float*)t.src);
+  else if (s.dtype == GLX_BF16) run((__bf16*)t.src);
+  else run((_Float16*)t.src);
+}
+
 // ------------------------------------------------------------------------------------------------ host: programs
 struct NsPlan {                // one matrix
   int rows, cols, m, n, mp, np, tile, xtile, tall, seg, splits, kper, nparts;       // tile: of symmetric products, xtile: of Q X
@@ -445,7 +553,7 @@ struct NsBounds { double g, p, h, q; };       // of one step of a segment: spect
 static float ns_scale(double bound) { return (float)exp2(floor(log2(32768.0 / bound))); }
 
 // the largest eigenvalues that the coefficients allow, step by step: lambda <- lambda p(lambda)^2 from [0, 1]
-static bool ns_bounds(int steps, const float* c, std::vector<double>& lam, std::vector<double>& pmax, std::vector<double>& hmax) {
+static bool ns_bounds(int steps, const double* c, std::vector<double>& lam, std::vector<double>& pmax, std::vector<double>& hmax) {
   if (!isfinite(c[0]) || !isfinite(c[1]) || !isfinite(c[2])) return false;
   double top = 1.01;           // (A's eigenvalues are at most 1 up to its own rounding)
   lam.push_back(top);
@@ -465,6 +573,9 @@ static bool ns_bounds(int steps, const float* c, std::vector<double>& lam, std::
 }
 
 static int ns_padded(int v, int tile) { return (v + tile - 1) / tile * tile; }
+
+// (16 x 64: 13 us in one launch, 81 on the tiles; x 801: 20 and 119; x 4096: 56 and 118; x 16384: 191 and 139)
+static bool ns_small(const glx_matrix& a) { return (a.rows < a.cols ? a.rows : a.cols) <= 16 && a.rows <= 8192 && a.cols <= 8192; }
 
 static NsPlan ns_plan(int rows, int cols, int dtype, int steps, size_t& at) {
   NsPlan p = {};
@@ -514,7 +625,8 @@ static int ns_check(const char* who, const glx_matrix* mats, int count, int dtyp
 extern "C" size_t glx_orthogonalize_workspace_bytes(const glx_matrix* mats, int count, int dtype, int steps) {
   if (ns_check("glx_orthogonalize_workspace_bytes", mats, count, dtype, steps) != GLX_OK) return 0;
   size_t at = 256;
-  for (int i = 0; i < count; ++i) ns_plan(mats[i].rows, mats[i].cols, dtype, steps, at);
+  for (int i = 0; i < count; ++i)
+    if (!ns_small(mats[i])) ns_plan(mats[i].rows, mats[i].cols, dtype, steps, at);
   return at + 256;
 }
 
@@ -550,14 +662,31 @@ static void ns_launch_ops(std::vector<NsOp>& ops, char* ws, int tile, int prods,
   }
 }
 
-extern "C" int glx_orthogonalize(const glx_matrix* mats, int count, int dtype, int steps, const float* coefficients, double eps,
+static void ns_launch_small(const std::vector<glx_matrix>& mats, int dtype, int steps, const double* c, double eps, hipStream_t st) {
+  for (size_t i = 0; i < mats.size(); i += NS_SMALLS) {
+    NsSmalls s;
+    memset(&s, 0, sizeof(s));
+    s.steps = steps; s.dtype = dtype; s.eps = eps;
+    for (int k = 0; k < 3; ++k) s.c[k] = c[k];
+    int n = 0;
+    for (size_t j = i; j < mats.size() && j < i + NS_SMALLS; ++j, ++n)
+      s.mat[n] = NsSmall{mats[j].src, mats[j].dst, mats[j].ld_src, mats[j].ld_dst, mats[j].rows, mats[j].cols};
+    hipLaunchKernelGGL(k_ns_small, dim3(n), dim3(1024), 0, st, s);
+  }
+}
+
+extern "C" int glx_orthogonalize(const glx_matrix* list, int listed, int dtype, int steps, const double* coefficients, double eps,
                                  void* workspace, size_t workspace_bytes, void* stream) try {
-  if (int rc = ns_check("glx_orthogonalize", mats, count, dtype, steps)) return rc;
+  if (int rc = ns_check("glx_orthogonalize", list, listed, dtype, steps)) return rc;
   GLX_REQUIRE(coefficients && eps >= 0.0, "glx_orthogonalize: bad coefficients or eps");
-  if (count == 0) return GLX_OK;
-  for (int i = 0; i < count; ++i)
-    GLX_REQUIRE(mats[i].src && mats[i].dst && mats[i].ld_src >= mats[i].cols && mats[i].ld_dst >= mats[i].cols,
+  if (listed == 0) return GLX_OK;
+  std::vector<glx_matrix> mats, small;
+  for (int i = 0; i < listed; ++i) {
+    GLX_REQUIRE(list[i].src && list[i].dst && list[i].ld_src >= list[i].cols && list[i].ld_dst >= list[i].cols,
                 "glx_orthogonalize: matrix %d: null pointer or rows that overlap", i);
+    (ns_small(list[i]) ? small : mats).push_back(list[i]);
+  }
+  const int count = (int)mats.size();
   std::vector<double> lam, pmax, hmax;
   GLX_REQUIRE(ns_bounds(steps, coefficients, lam, pmax, hmax),
               "glx_orthogonalize: these coefficients let singular values grow beyond the arithmetic's range");
@@ -578,8 +707,9 @@ extern "C" int glx_orthogonalize(const glx_matrix* mats, int count, int dtype, i
   }
   GLX_REQUIRE(((uintptr_t)workspace & 15) == 0, "glx_orthogonalize: the workspace must be 16-byte aligned");
   hipStream_t st = (hipStream_t)stream;
+  ns_launch_small(small, dtype, steps, coefficients, eps, st);
   char* ws = (char*)workspace;
-  const float a = coefficients[0], b = coefficients[1], c = coefficients[2];
+  const float a = (float)coefficients[0], b = (float)coefficients[1], c = (float)coefficients[2];
   auto qbound = [&](int s0, int s) { double v = 1; for (int i = s0; i <= s; ++i) v *= pmax[i]; return v; };
 
   for (int i = 0; i < count; i += NS_MATS) {           // |G|_F, then the planes

@@ -39,7 +39,7 @@ def _check_steps(who, steps, coefficients, eps):
         raise ValueError("%s: coefficients must be three finite numbers, got %r" % (who, coefficients))
     if not float(eps) >= 0.0:
         raise ValueError("%s: eps must not be negative, got %r" % (who, eps))
-    return int(steps), (ctypes.c_float * 3)(*coefficients), float(eps)
+    return int(steps), (ctypes.c_double * 3)(*coefficients), float(eps)
 
 
 def orthogonalize(mats, steps=5, coefficients=MUON_COEFFICIENTS, eps=1e-7):

@@ -1507,7 +1507,7 @@ typedef struct glx_matrix {
   int32_t rows, cols;
 } glx_matrix;
 size_t glx_orthogonalize_workspace_bytes(const glx_matrix* mats, int count, int dtype, int steps);    /* 0: bad arguments */
-int glx_orthogonalize(const glx_matrix* mats, int count, int dtype, int steps, const float* coefficients, double eps,
+int glx_orthogonalize(const glx_matrix* mats, int count, int dtype, int steps, const double* coefficients, double eps,
                       void* workspace, size_t workspace_bytes, void* stream);
 
 /* The flat update whose matrices take orthogonalised steps (glenet_amd.optim.FlatMuon).  A chunk is a run of at most 4096

@@ -53,7 +53,7 @@ def test_orthogonalize_c_entry_refuses():
 
     def call(rows=4, cols=6, ld=6, dtype=0, steps=5, coeffs=(3.4445, -4.775, 2.0315), eps=1e-7, ws=16, nbytes=0, src=64):
         t = (_Matrix * 1)(_Matrix(src, 64, ld, 6, rows, cols))
-        rc = lib.glx_orthogonalize(t, 1, dtype, steps, (ctypes.c_float * 3)(*coeffs), ctypes.c_double(eps), ctypes.c_void_p(ws),
+        rc = lib.glx_orthogonalize(t, 1, dtype, steps, (ctypes.c_double * 3)(*coeffs), ctypes.c_double(eps), ctypes.c_void_p(ws),
                                    ctypes.c_size_t(nbytes), ctypes.c_void_p(0))
         return rc, lib.glx_last_error().decode()
 
@@ -102,7 +102,7 @@ def test_attention_c_entry_refuses():
     lib = _lib.load()
 
     class _Attention(ctypes.Structure):        # glx_attention
-        _fields_ = ([(n, ctypes.c_void_p) for n in ("q", "k", "v", "out", "lse", "key_mask", "q_cnt", "k_cnt")]
+        _fields_ = ([(n, ctypes.c_void_p) for n in ("q", "k", "v", "out", "out_rest", "lse", "key_mask", "q_cnt", "k_cnt")]
                     + [(n, ctypes.c_int64) for n in ("q_rows", "k_rows", "q_len", "k_len", "q_stride", "q_head_stride", "k_stride",
                                                      "k_head_stride", "v_stride", "v_head_stride")]
                     + [(n, ctypes.c_int32) for n in ("frames", "heads", "kv_heads", "dim", "dtype")] + [("scale", ctypes.c_float)])

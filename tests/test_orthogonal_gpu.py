@@ -293,3 +293,33 @@ def test_the_training_step_takes_flat_muon(dev):
     opt.step(packed=True)
     torch.cuda.synchronize()
     assert int(opt.step_count) == 6 and not torch.equal(want, opt.exp_avg) and not torch.equal(p0, opt.flat_param)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("shape", [(1, 1), (2, 2), (3, 801), (801, 3), (4, 4), (16, 16), (16, 17), (15, 64), (16, 8192), (8192, 16), (16, 8193)])
+def test_few_rows(dev, shape, dtype):
+    """Up to 16 x 8192 all arithmetic is in 64 bits: the result's rounding, and its step through fp32, are all that is left."""
+    from glenet_amd.optim import orthogonalize
+    g = _gradient(*shape, 5, dev, dtype)
+    wide = torch.full((shape[0] + 2, shape[1] + 3), float("nan"), device=dev, dtype=dtype)
+    wide[1:-1, 1:-2] = g
+    o, want = orthogonalize(wide[1:-1, 1:-2]), _exact(g)
+    if max(shape) <= 8192:
+        assert bool(((o.double() - want).abs() <= (HALF[dtype] + 2.0 ** -23) * want.abs() + (6e-8 if dtype == torch.float16 else 1e-30)).all())
+        for steps in (1, 12):
+            assert _off(orthogonalize(g, steps=steps), _exact(g, steps)) < HALF[dtype] + 2.0 ** -23
+    else:
+        assert _off(o, want) < LIMIT[dtype] + HALF[dtype]
+    zero = torch.zeros(shape, device=dev, dtype=dtype)
+    assert not orthogonalize([zero, g])[0].any()
+    assert torch.equal(orthogonalize([zero, g, torch.cat([g, g])])[1], orthogonalize(g))
+
+
+def test_a_matrix_of_few_rows_may_be_overwritten(dev):
+    from glenet_amd.optim import _check_steps, _orthogonalize
+    steps, coeffs, eps = _check_steps("test", 5, COEFFS, 1e-7)
+    for shape in ((16, 1500), (700, 9), (40, 300)):
+        g = _gradient(*shape, 8, dev)
+        want, buf = _exact(g), g.clone()
+        _orthogonalize([buf], steps, coeffs, eps, [buf])
+        assert _off(buf, want) < LIMIT[torch.float32]
