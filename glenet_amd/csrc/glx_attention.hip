@@ -263,9 +263,11 @@ __global__ __launch_bounds__(256) void k_xa_join(XaArgs a) {
 }
 
 // ------------------------------------------------------------------------------------------------ host
-int xa_splits(long long blocks, long long keys_per_frame) {
+// one round of blocks on 256 compute units that hold `per_cu` each (two rounds of half the keys, 4 x 128 queries over 2048 states,
+// fp32, 4 heads of 64, training: 134 us instead of 122; one query over 4 x 32768, bf16: 120 instead of 115)
+int xa_splits(long long blocks, long long keys_per_frame, int per_cu) {
   if (blocks < 1) blocks = 1;
-  long long s = 512 / blocks, most = keys_per_frame / 256;        // 256 keys a split, at least
+  long long s = 256 * per_cu / blocks, most = keys_per_frame / 256;        // 256 keys a split, at least
   s = s < most ? s : most;
   return (int)(s < 1 ? 1 : (s > 256 ? 256 : s));
 }
@@ -278,7 +280,8 @@ void xa_rows_plan(const glx_attention* t, int* rw, long long* tiles, int* splits
   for (*rw = 4;; *rw = small) {
     *tiles = xa_tiles(rows, t->frames, (int)(t->q_len * group), counts, *rw * 32);
     const long long blocks = (counts ? rows / (*rw * 32) + 1 : *tiles) * t->kv_heads;
-    *splits = xa_splits(blocks, keys);
+    const long long lds = 4ll * (*rw == 1 ? 128 : 64) * ((t->dim + 31) / 32 * 32) * (long long)glx_elem_size(t->dtype);
+    *splits = xa_splits(blocks, keys, lds <= 80 * 1024 ? 2 : 1);
     if (*rw == small || (rows > 64 * fr && blocks * *splits >= 256)) return;
   }
 }

@@ -23,7 +23,7 @@
 
 #define XA_PSCALE 4096.f      // fp16: of P
 
-int xa_splits(long long blocks, long long keys_per_frame);
+int xa_splits(long long blocks, long long keys_per_frame, int per_cu);
 void xa_rows_plan(const glx_attention* t, int* rw, long long* tiles, int* splits);
 int xa_check(const char* who, const glx_attention* t);
 XaArgs xa_args(const glx_attention* t);
@@ -459,7 +459,7 @@ static XaBackward xa_backward_plan(const glx_attention* t) {
   const long long rows = t->q_rows * group / fr;
   xa_rows_plan(t, &p.rw, &p.qtiles, &p.qsplits);
   p.ktiles = xa_tiles(t->k_rows, t->frames, (int)t->k_len, counts, 128);
-  p.ksplits = xa_splits((counts ? t->k_rows / 128 + 1 : p.ktiles) * t->kv_heads, rows);
+  p.ksplits = xa_splits((counts ? t->k_rows / 128 + 1 : p.ktiles) * t->kv_heads, rows, 2);
   p.delta = 0;
   p.qpart = glx_align((size_t)t->q_rows * t->heads * sizeof(float));
   p.kpart = p.qpart + (p.qsplits > 1 ? glx_align((size_t)p.qsplits * t->q_rows * t->heads * t->dim * sizeof(float)) : 0);
