@@ -9,6 +9,9 @@
 // wave for narrow rows (sums by shuffles, several rows per wave), a block for wide ones.  In the backward pass a thread owns
 // the SAME columns of every row its group visits, so dw and db grow in registers and leave the block once; a second launch adds
 // the blocks' parts in a fixed order (no atomics: the same result every time).
+//
+// 131072 x 1024 bf16: forward 107 us (5.0 TB/s), backward 178 + 5 (4.4; a large copy: 5.1); 58733 x 64 fp32: 9 and 12 + 3 us
+// (3.4 TB/s and 3.0: 30 and 45 MB are over before all of the card's memory is busy); 128 x 256: 3.5 and 6.5, all latency.
 #include "glx_elem.h"
 
 #define LN_BLOCKS 1024        // forward / backward groups stride over the rows from this many blocks

@@ -17,6 +17,10 @@
 // from the coefficients (the eigenvalues start in [0, 1]) and from |X_0| = |G| / (|G| + eps), so nothing overflows and a
 // gradient far below eps keeps its precision.
 // Zero padding to whole tiles is exact: it stays zero in A and X.
+//
+// 4096 x 4096 bf16: 3.57 ms.  A split product of the size of Q X takes 426 us (968 TFLOP/s of fp16 products; a large library
+// product reaches 1119), a single one 209 us (658: its 64 KB stages wait for their way from L2 to LDS).  256 x 256 fp32: 15 products
+// of 8 us each, all latency.
 #include "glx_elem.h"
 
 #include <math.h>

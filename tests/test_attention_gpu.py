@@ -452,3 +452,17 @@ def test_gradients_of_rows_that_one_key_dominates(dev, lk, dtype):
         if dtype == torch.float16:
             lim = lim + scale * 2.0 ** -24 * ds.abs().max() * kk.abs().sum(0)
         assert bool(((dq[:, j].double() - want).abs() <= lim).all())
+
+
+@pytest.mark.parametrize("lk", [[20, 3], [200, 20]])
+def test_gradients_of_the_keys_alone(dev, lk):
+    """dk and dv without dq: delta comes from the same launch, which then writes nothing else."""
+    from glenet_amd.attention import cross_attention
+    case = ([70, 33], lk, 4, 2, 32, True, False)
+    for dtype in (torch.float32, torch.bfloat16):
+        q, k, v, go, mask, cnts = _inputs(case, dtype, 12, dev)
+        _, _, dk, dv = _run(q, k, v, go, mask, cnts)
+        kk, vv = k.clone().requires_grad_(True), v.clone().requires_grad_(True)
+        o = cross_attention(q, kk, vv, *cnts, key_mask=mask)
+        a, b = torch.autograd.grad(o, [kk, vv], go)
+        assert torch.equal(a, dk) and torch.equal(b, dv)
