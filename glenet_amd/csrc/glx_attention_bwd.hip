@@ -19,7 +19,8 @@
 // dS sums to zero over a row, so what the keys of a row have in common leaves dQ, but the roundings of dS times it stay.  With few
 // channels the scores pull a row's keys together: at dim 8, 4 x 4012 x 2768, 2 heads, bf16, dQ was 2.7e-3 off (the rounding of
 // the result alone: 1.7e-3).  Heads of up to 32 channels, whose time is the exponentials, so add what the rounding left in a
-// second product (there 201 -> 208 us a training pass, and dQ below 2.4e-3); wider ones do not.
+// second product (there 201 -> 208 us a training pass, and dQ below 2.4e-3); wider ones do not.  The same for P and dS in front
+// of dV and dK, where a few rows of a few channels left 1.6 times the rounding of the result.
 #include "glx_attention.h"
 
 #include <type_traits>
@@ -253,7 +254,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(xa_waves<T,
 
 // ------------------------------------------------------------------------------------------------ dK, dV
 template <typename T, int DP>
-__global__ __launch_bounds__(256) void k_xa_dkv(XaArgs a) {
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DP == 32 ? 2 : 1))) void k_xa_dkv(XaArgs a) {
   constexpr int BM = sizeof(T) == 2 ? 64 : 32, PARTS = BM / 32;
   constexpr int KS = DP / 16, DT = DP / 32;
   typedef XaTile<T, DP> Tile;
@@ -406,6 +407,13 @@ __global__ __launch_bounds__(256) void k_xa_dkv(XaArgs a) {
         if (j % DT == 0) { p = xa_pack<T>(s[u], j / DT); q = xa_pack<T>(d[u], j / DT); }
         xa_mma(dV[j % DT], ring[r][0], p);
         xa_mma(dK[j % DT], ring[r][1], q);
+        if constexpr (sizeof(T) == 2 && DP == 32) {            // what their rounding left (above)
+          xf16 x;
+#pragma unroll
+          for (int i = 0; i < 8; ++i) { x[i] = s[u][j / DT * 8 + i] - (float)p[i]; x[i + 8] = d[u][j / DT * 8 + i] - (float)q[i]; }
+          xa_mma(dV[0], ring[r][0], xa_pack<T>(x, 0));
+          xa_mma(dK[0], ring[r][1], xa_pack<T>(x, 1));
+        }
         if (PARTS > 1 && u == 0) {
 #pragma unroll
           for (int i = j * 16 / GS; i < (j + 1) * 16 / GS; ++i) weigh(PARTS - 1, i);

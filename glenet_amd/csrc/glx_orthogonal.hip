@@ -592,7 +592,8 @@ static NsPlan ns_plan(int rows, int cols, int dtype, int steps, size_t& at) {
   p.tile = pad == 128 && wide * (wide + 1) / 2 >= 200 ? 128 : 64;
   p.xtile = pad == 128 && wide * across >= 200 ? 128 : 64;
   p.seg = dtype == GLX_BF16 ? 5 : 3;
-  if (p.m <= 128 || (dtype == GLX_F32 ? p.n < 4ll * p.m : 4ll * p.n <= 5ll * p.m)) p.seg = 1;
+  // (fp32 rows up to 192: 129 x 1032 comes out 1.6 times as far off as plain fp32 products in segments of three, 0.7 times in ones)
+  if (p.m <= (dtype == GLX_F32 ? 192 : 128) || (dtype == GLX_F32 ? p.n < 4ll * p.m : 4ll * p.n <= 5ll * p.m)) p.seg = 1;
   if (p.seg > steps) p.seg = steps;
   const int t = p.mp / p.tile;
   const long long tiles = (long long)t * (t + 1) / 2, ksteps = p.np / NS_K;
@@ -744,9 +745,10 @@ extern "C" int glx_orthogonalize(const glx_matrix* list, int listed, int dtype, 
   for (int i = 0; i < count; ++i) {
     const NsPlan& p = plans[i];
     // bfloat16: single products in the last two steps, where what they lose is no longer amplified (it comes to 1e-3 of the
-    // result, half a step is 4e-3); segments of one step only
+    // result, half a step is 4e-3); segments of one step only, and matrices whose time is the products (smaller ones lose up
+    // to 2e-3 where all singular values are alike, 24 x 360, and gain nothing)
     auto last = [&](int s1) {
-      return dtype == GLX_BF16 && p.seg == 1 && s1 > steps - 2 && steps >= 4 && steepest <= 4.0;
+      return dtype == GLX_BF16 && p.seg == 1 && p.m > 1024 && s1 > steps - 2 && steps >= 4 && steepest <= 4.0;
     };
     // lo lo too: fp32 matrices on 64-wide tiles, whose time is latency and LDS (small ones lose up to 1.6 times a plain fp32
     // product's error without)
