@@ -1,5 +1,5 @@
-// Orthogonalised updates (glenet_amd/optim.py): Newton-Schulz steps on a list of matrices of any shapes, few launches for all.  Matrices of up
-// to 16 rows have a kernel of their own, further down; what follows is about the others.
+// Orthogonalised updates (glenet_amd/optim.py): Newton-Schulz steps on a list of matrices of any shapes, few launches for all.
+// Matrices of up to 16 rows have a kernel of their own, further down; what follows is about the others.
 //
 //   X = G / (|G|_F + eps), transposed where G has more rows than columns (X: m x n, m <= n);  per step
 //   A = X X^T,  X <- a X + (b A + c A^2) X  =  P X,  P = a I + b A + c A^2
@@ -10,7 +10,8 @@
 // s (3 m^2 n + m^3): the same for square matrices, s times less work on X for wide ones.  What limits s is rounding: a
 // perturbation of A in directions of small singular values grows by a^2 = 11.9 per step until the next look at X.  Measured
 // against 64 bits on gradients with decaying spectra, Frobenius: one step per segment 1e-5, 3 + 2 steps 1e-5, 5 steps 1e-4 to
-// 4e-4.  So fp32 and fp16 matrices take segments of three, bf16 ones (half a step is 4e-3) of five, nearly square ones of one.
+// 4e-4.  So fp32 and fp16 matrices take segments of three, bf16 ones (half a step is 4e-3) of five, nearly square ones and those
+// of up to 128 rows (fp32: 192) of one.
 //
 // Products: every operand is held as two fp16 planes of value * 2^k (hi + lo: 22 bits down to 2^-25 of the scale), and a
 // product is three MFMAs hi hi + hi lo + lo hi into fp32.  The scales 2^k come from bounds of the spectral norms that follow
@@ -213,7 +214,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1))) void k
     ti = b / tn; tj = b - ti * tn;
   }
   auto at = [&](unsigned place) { return s.ws + (size_t)place * 256; };
-  const float xin = t.xin ? ((const float*)at(t.xin))[t.xstep] : 1.f, alpha = t.alpha / (t.xpow == 2 ? xin * xin : xin), scale = t.xout ? ((const float*)at(t.xout))[t.xnext] : t.scale;
+  const float xin = t.xin ? ((const float*)at(t.xin))[t.xstep] : 1.f, alpha = t.alpha / (t.xpow == 2 ? xin * xin : xin);
+  const float scale = t.xout ? ((const float*)at(t.xout))[t.xnext] : t.scale;
   const int kper = t.kper * NS_K, k0 = split * kper, k1 = k0 + kper < t.K ? k0 + kper : t.K;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5, l32 = lane & 31;
   const int ld = ns_ld(t.K);
