@@ -31,7 +31,7 @@ def cross_attention(q, k, v, q_batch_cnt=None, k_batch_cnt=None, key_mask=None, 
     scale: default 1 / sqrt(D).
     -> q's shape and type.  A query whose frame has no state left gives 0 and no gradients, and so do rows behind the last
     frame (counts that reach beyond the tensors are cut there).  Scores, softmax and sums in fp32; gradients have the same bits
-    every time.  Once differentiable."""
+    every time.  Once differentiable, in reverse mode: an input with a forward-mode tangent is refused."""
     who = "cross_attention"
     if q.dtype not in _lib.DTYPE_CODES or k.dtype != q.dtype or v.dtype != q.dtype:
         raise ValueError("%s: q, k, v must share one type, float32, bfloat16 or float16; got %s, %s, %s" % (who, q.dtype, k.dtype, v.dtype))

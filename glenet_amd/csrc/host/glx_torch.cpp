@@ -50,6 +50,12 @@ Tensor bytes(size_t n, const Tensor& like) {
 std::optional<Tensor> maybe(const Tensor& t) { return t.defined() ? std::optional<Tensor>(t) : std::nullopt; }
 bool wanted(const Tensor& t) { return t.defined() && t.requires_grad(); }
 
+// forward mode: the kernels have no formula for tangents, and one that they left out would look like a tangent of zero
+void no_tangents(const char* who, std::initializer_list<const Tensor*> inputs) {
+  for (const Tensor* t : inputs)
+    TORCH_CHECK_NOT_IMPLEMENTED(!t->defined() || !t->_fw_grad(0).defined(), who, " has no forward-mode derivative (an input carries a tangent)");
+}
+
 // gradients that may be used but not differentiated again: under create_graph they hang on the inputs by a node that raises
 variable_list once(variable_list g, const variable_list& inputs, const char* who) {
   if (!at::GradMode::is_enabled()) return g;
@@ -123,6 +129,7 @@ struct LayerNorm : public torch::autograd::Function<LayerNorm> {
 
 Tensor layer_norm(const Tensor& x, const std::optional<Tensor>& weight, const std::optional<Tensor>& bias, double eps) {
   const Tensor w = weight ? weight->contiguous() : Tensor(), b = bias ? bias->contiguous() : Tensor();
+  no_tangents("layer_norm", {&x, &w, &b});
   if (at::GradMode::is_enabled() && (wanted(x) || wanted(w) || wanted(b))) return LayerNorm::apply(x, maybe(w), maybe(b), eps);
   return ln_forward(x, w, b, eps, nullptr, nullptr);
 }
@@ -209,6 +216,7 @@ struct CrossAttention : public torch::autograd::Function<CrossAttention> {
 Tensor cross_attention(const Tensor& q, const Tensor& k, const Tensor& v, const std::optional<Tensor>& q_cnt,
                        const std::optional<Tensor>& k_cnt, const std::optional<Tensor>& key_mask, double scale) {
   const Tensor qc = q_cnt.value_or(Tensor()), kc = k_cnt.value_or(Tensor()), mask = key_mask.value_or(Tensor());
+  no_tangents("cross_attention", {&q, &k, &v});
   if (at::GradMode::is_enabled() && (wanted(q) || wanted(k) || wanted(v))) return CrossAttention::apply(q, k, v, q_cnt, k_cnt, key_mask, scale);
   return xa_forward(q, k, v, qc, kc, mask, scale, nullptr, nullptr);
 }

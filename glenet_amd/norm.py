@@ -4,7 +4,8 @@ BatchNorms of spconv.core and conv2d.
     y = (x - mean) / sqrt(var + eps) * weight + bias          (biased variance, statistics in fp32)
 
 fp32, bf16 and fp16 rows of any width; weights of the rows' type or fp32.  The backward pass gives the gradients of the rows,
-the weight and the bias in one or two launches with fixed summation orders: the same bits every time.  Once differentiable."""
+the weight and the bias in one or two launches with fixed summation orders: the same bits every time.  Once differentiable, in
+reverse mode: an input with a forward-mode tangent is refused."""
 import torch
 from torch import nn
 
