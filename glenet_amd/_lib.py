@@ -100,8 +100,19 @@ def stream_ptr():
     return c_void_p(torch.cuda.current_stream().cuda_stream)
 
 
+_TRACERS = (torch._C._TorchDispatchModeKey.PROXY, torch._C._TorchDispatchModeKey.FAKE)
+
+
+def _refuse_tracing(name):
+    """A launch on raw pointers leaves nothing in a trace but the allocation of its results, and a tensor without storage has no
+    pointer: neither may pass for a result."""
+    if torch._C._len_torch_dispatch_stack() and any(torch._C._get_dispatch_mode(k) is not None for k in _TRACERS):
+        raise GlxError("%s cannot be traced: it launches kernels on its tensors' memory" % name)
+
+
 def call(name, *args):
     """Call an int-returning entry point with the current torch stream appended."""
+    _refuse_tracing(name)
     lib = load()
     fn = getattr(lib, name)
     rc = fn(*[_arg(a) for a in args], stream_ptr())
@@ -112,6 +123,7 @@ def call(name, *args):
 
 def call_on(device, name, *args):
     """call() on `device`'s current stream: tensors may live on another device than the current one."""
+    _refuse_tracing(name)
     if device.index is None or device.index == torch.cuda.current_device():
         return call(name, *args)
     with torch.cuda.device(device):

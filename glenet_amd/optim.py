@@ -49,7 +49,7 @@ def orthogonalize(mats, steps=5, coefficients=MUON_COEFFICIENTS, eps=1e-7):
 
     mats: a device tensor (..., rows, cols), or a list / tuple of 2-D tensors of ANY shapes but one type (float32, bfloat16 or
     float16) and one device: a list costs as many launches as one matrix (csrc/glx_orthogonal.hip).
-    -> new tensors of the same shapes and type (a list for a list), outside autograd."""
+    -> new tensors of the same shapes and type (a list for a list), outside autograd; tracing it is refused."""
     who = "orthogonalize"
     steps, coeffs, eps = _check_steps(who, steps, coefficients, eps)
     if isinstance(mats, torch.Tensor):

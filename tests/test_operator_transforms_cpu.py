@@ -118,3 +118,19 @@ def test_tensors_without_a_device_are_refused_by_the_binding():
         ops.layer_norm.default(x, None, None, 1e-5)
     with pytest.raises(NotImplementedError, match="CPU"):
         ops.cross_attention.default(x, x, x, None, None, None, 1.0)
+
+
+def test_what_launches_on_raw_pointers_is_not_traced():
+    """The orthogonaliser is outside autograd and no operator of torch: a trace of it would return memory that nobody wrote."""
+    from glenet_amd import _lib
+    from glenet_amd.optim import orthogonalize
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    from torch.fx.experimental.proxy_tensor import make_fx
+    with FakeTensorMode():
+        m = torch.empty(20, 30, device="cuda")
+        with pytest.raises(_lib.GlxError, match="cannot be traced"):
+            make_fx(lambda t: orthogonalize(t))(m)
+        with pytest.raises(_lib.GlxError, match="cannot be traced"):
+            orthogonalize([m])
+    with pytest.raises(_lib.GlxError, match="cannot be traced"):
+        make_fx(lambda t: (_lib.call("glx_abi_version"), t * 2)[1])(torch.ones(3))

@@ -74,3 +74,13 @@ def test_a_direct_call_of_a_training_pass_has_no_gradient_of_its_own(dev, name):
         y = ops.cross_attention_train.default(x, args[1], args[1], None, None, None, 1.0)[0]
     with pytest.raises(RuntimeError, match="not implemented"):
         y.sum().backward()
+
+
+def test_the_orthogonaliser_is_not_traced(dev):
+    from glenet_amd import _lib
+    from glenet_amd.optim import orthogonalize
+    from torch.fx.experimental.proxy_tensor import make_fx
+    m = torch.randn(20, 30, device=dev)
+    with pytest.raises(_lib.GlxError, match="cannot be traced"):
+        make_fx(lambda t: orthogonalize(t))(m)
+    assert torch.equal(orthogonalize(m), orthogonalize(m))       # (nothing of the trace is left)
