@@ -440,7 +440,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DP == 32 ? 
       for (int k = 0; k < 4; ++k) {
         const int d = i * 32 + g * 8 + half * 4 + k;
         if (d >= a.dim) continue;
-        const float x = dK[i][g * 4 + k] * ksize, y = dV[i][g * 4 + k] * vsize;
+        // (a masked state's weights are 0, but 0 times a gradient or a query that is no number is none either)
+        const float x = valid ? dK[i][g * 4 + k] * ksize : 0.f, y = valid ? dV[i][g * 4 + k] * vsize : 0.f;
         if (a.splits > 1) {
           pk[d] = x; pk[n + d] = y;
         } else {

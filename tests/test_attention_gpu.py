@@ -466,3 +466,39 @@ def test_gradients_of_the_keys_alone(dev, lk):
         o = cross_attention(q, kk, vv, *cnts, key_mask=mask)
         a, b = torch.autograd.grad(o, [kk, vv], go)
         assert torch.equal(a, dk) and torch.equal(b, dv)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("d", [32, 40, 128])
+def test_masked_states_have_no_gradient_whatever_the_queries_gradients_hold(dev, d, dtype):
+    """A loss takes the logarithm of rows without a state (0) and hands back infinities and NaN: nothing of that reaches the
+    gradients of masked states, of trailing ones or of other frames."""
+    from glenet_amd.attention import cross_attention
+    g = torch.Generator().manual_seed(d)
+    ql, kl, h, hk = [40, 70, 3, 2], [50, 150, 0, 40], 4, 2
+
+    def normal(*s):
+        return torch.randn(*s, generator=g).to(dtype).to(dev)
+
+    q, k, v, go = normal(sum(ql) + 1, h, d), normal(sum(kl) + 9, hk, d), normal(sum(kl) + 9, hk, d), normal(sum(ql) + 1, h, d)
+    mask = (torch.rand(sum(kl) + 9, generator=g) < 0.7).to(dev)
+    mask[:50] = False                                         # frame 0 has no state left, frame 2 has none at all
+    cnts = tuple(torch.tensor(x, dtype=torch.int32, device=dev) for x in (ql, kl))
+    want = _run(q, k, v, go, mask, cnts)
+    none = torch.cat([torch.arange(40), torch.arange(110, 113), torch.arange(sum(ql), sum(ql) + 1)]).to(dev)      # rows without a state
+    for bad in (float("nan"), float("inf"), -float("inf")):
+        broken, odd = go.clone(), q.clone()
+        broken[none] = bad
+        odd[none] = bad
+        for got in (_run(q, k, v, broken, mask, cnts), _run(odd, k, v, go, mask, cnts), _run(odd, k, v, broken, mask, cnts)):
+            for a, b in zip(got, want):
+                assert torch.equal(a, b)
+    broken = go.clone()
+    broken[60] = float("nan")                                 # a row of frame 1: its masked states and other frames stay clean
+    _, dq, dk, dv = _run(q, k, v, broken, mask, cnts)
+    off = ~mask
+    off[200:] = True
+    for a, b in ((dk, want[2]), (dv, want[3])):
+        assert torch.equal(a[off], b[off]) and bool(torch.isnan(a[50:200][mask[50:200]]).any())
+    rows = torch.arange(sum(ql) + 1, device=dev) != 60
+    assert torch.equal(dq[rows], want[1][rows])
