@@ -52,6 +52,10 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(xa_waves<T,
 #pragma unroll
   for (int i = 0; i < DT; ++i) O[i] = (xf16)(0.f);
   const float scale2 = fabsf(a.scale2);
+  // fp16 ends at 2^-25: beside a key of weight 1 the many small ones of a long row would vanish (131 072 of 2^-25.4 are 3e-3 of it).
+  // So p is formed 2^11 times as large, and m lags by 2^4 at most: up to 2^15, down to 2^-36 of a row's largest
+  constexpr bool FP16 = __is_same(T, _Float16);
+  constexpr float UP = FP16 ? 11.f : 0.f, LAG = FP16 ? 4.f : 8.f;
   float m = -INFINITY, l = 0.f, lr = 0.f;                     // m unscaled; sums of p, of the rounded p (16-bit)
   XaLoad<T, DP, BN> kl, vl;
   const bool kdma = a.dma & 2, vdma = a.dma & 4;
@@ -113,8 +117,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(xa_waves<T,
 #pragma unroll
         for (int i = 0; i < 16; ++i) top = fmaxf(top, s[u][i]);
       top = fmaxf(top, __shfl_xor(top, 32, 64));
-      // m follows the maximum only where p would pass 2^8: then O and l shrink, else the tile is added as it is
-      if (__any((top - m) * scale2 > 8.f || m == -INFINITY)) {
+      // m follows the maximum only where p would pass 2^LAG: then O and l shrink, else the tile is added as it is
+      if (__any((top - m) * scale2 > LAG || m == -INFINITY)) {
         const float now = fmaxf(m, top), shrink = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((m - now) * scale2);
         m = now;
         l *= shrink;
@@ -125,7 +129,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(xa_waves<T,
           for (int e = 0; e < 16; ++e) O[i][e] *= shrink;
       }
       // (16-bit: one fused operation; its rounding of m scale2 is a factor that p and l share.  fp32 keeps 2^0 = 1 exactly)
-      const float ref = m == -INFINITY ? 0.f : m, at = ref * scale2;
+      const float ref = m == -INFINITY ? 0.f : m, at = ref * scale2 - UP;
 #pragma unroll
       for (int u = 0; u < SUB; ++u) {
         float sum = 0.f;
@@ -153,7 +157,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(xa_waves<T,
   l += __shfl_xor(l, 32, 64);
   if (sizeof(T) == 2) lr += __shfl_xor(lr, 32, 64);
   else lr = l;
-  m = m == -INFINITY ? m : m * scale2;
+  m = m == -INFINITY ? m : m * scale2 - UP;                   // l and O are sums of 2^(s scale2 - m)
   if (KW > 1) {                                               // the waves of a row tile, joined in order
     if (half == 0) { sm[wave][l32] = m; sl[wave][l32] = l; slr[wave][l32] = lr; }
     __syncthreads();

@@ -502,3 +502,28 @@ def test_masked_states_have_no_gradient_whatever_the_queries_gradients_hold(dev,
         assert torch.equal(a[off], b[off]) and bool(torch.isnan(a[50:200][mask[50:200]]).any())
     rows = torch.arange(sum(ql) + 1, device=dev) != 60
     assert torch.equal(dq[rows], want[1][rows])
+
+
+@pytest.mark.parametrize("first", [True, False])
+@pytest.mark.parametrize("queries,keys", [(8192, 131072), (1, 131072), (40, 700)])
+def test_fp16_rows_that_one_key_dominates_keep_the_others_weight(dev, queries, keys, first):
+    """One key's weight is 2^25.4 times each of the others', which together add keys 2^-25.4 to the row: 3e-3 of it at 131 072 keys.
+    They carry the values 1, the one key 0, so that the row IS what they add.
+
+    A weight is rounded to fp16 at 2^11 times its size, the largest of a row's between 2^11 and 2^15: what rounds to a subnormal is
+    off by 2^-25 2^-11, the others by 2^-11 of themselves; the weights' exponents by 4 2^-24 25.4 and the sums by keys 2^-24 relative
+    at most; the result is rounded to 2^-11 or half a subnormal step."""
+    from glenet_amd.attention import cross_attention
+    h, d = 8 if queries > 1 else 2, 8
+    q, k, v = (torch.zeros(n, h, d, device=dev, dtype=torch.float16) for n in (queries, keys, keys))
+    at = 0 if first else keys - 1
+    q[:, :, 0], k[at, :, 0] = 4.195, 4.195
+    v.fill_(1.0)
+    v[at] = 0.0
+    other = math.exp(-float(q[0, 0, 0].double() * k[at, 0, 0].double()))
+    want = (keys - 1) * other / (1 + (keys - 1) * other)
+    limit = (keys - 1) * 2.0 ** -36 + want * (2 * 2.0 ** -11 + keys * U + 120 * U) + 2.0 ** -25
+    for o in (cross_attention(q[None], k[None], v[None], scale=1.0),
+              cross_attention(q.clone().requires_grad_()[None], k[None], v[None], scale=1.0)):
+        off = float((o.detach().double() - want).abs().max())
+        assert off < limit
