@@ -6,9 +6,12 @@
 // A block is four waves: four tiles of 32 rows that share the staged keys, or, where a frame has few rows, ONE tile whose
 // waves take the staged keys in turn and are joined at the end.  Few tiles are split over the keys as well; the splits' results
 // (O unnormalised, m, l) are joined by a second launch.  Scores, m, l and O are fp32; for 16-bit inputs p is rounded to their
-// type in front of the second product (each to half a step, unbiased: below the rounding of O itself).  O is divided by the sum
-// of the ROUNDED p -- a row that one key dominates is then as exact as that key's value -- and the log-sum-exp, from which the
-// backward pass forms p again in fp32, is that of the unrounded ones.
+// type in front of the second product (each to half a step, unbiased: together with the rounding of O 1.4 times the error that O's
+// alone leaves).  O is divided by the sum of the ROUNDED p -- a row that one key dominates is then as exact as that key's value --
+// and the log-sum-exp, from which the backward pass forms p again in fp32, is that of the unrounded ones.  Few rows, whose time is
+// the keys' way from memory, take what the rounding left in a second product (one query over 4 x 32768, bf16: 2.3e-3 off, then
+// 1.7e-3, 114.6 us both); with four row tiles it would cost 5 to 7 % (2 x 4096 x 16384, 128 channels: 2.71 -> 2.84 ms a training
+// pass; 6 x 217 x 1531, 40 channels: 27.5 -> 29.4 us).
 //
 // 2 frames of 4096 queries over 16384 keys, 8 heads of 128 on 2 key heads, bf16: 720 us (764 TFLOP/s; a large library product
 // reaches 1156), bound by the exponentials beside the products; one query over each of 4 x 32768 keys, 32 heads on 8: 108 us with
@@ -143,9 +146,22 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(xa_waves<T,
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
           const typename XaFrag<T>::vec p = xa_pack<T>(s[u], c);
-          lr = xa_total(p, lr);
+          if constexpr (KW > 1 && sizeof(T) == 2) {            // and what the rounding left
+            xf16 rest;
 #pragma unroll
-          for (int i = 0; i < DT; ++i) xa_mma(O[i], xa_down<T, DP>(tv, (u * KW + kw) * 32 + c * 16, i * 32, lane), p);
+            for (int i = 0; i < 8; ++i) rest[i] = s[u][c * 8 + i] - (float)p[i];
+            const typename XaFrag<T>::vec r = xa_pack<T>(rest, 0);
+#pragma unroll
+            for (int i = 0; i < DT; ++i) {
+              const typename XaFrag<T>::vec v = xa_down<T, DP>(tv, (u * KW + kw) * 32 + c * 16, i * 32, lane);
+              xa_mma(O[i], v, r);
+              xa_mma(O[i], v, p);
+            }
+          } else {
+            lr = xa_total(p, lr);
+#pragma unroll
+            for (int i = 0; i < DT; ++i) xa_mma(O[i], xa_down<T, DP>(tv, (u * KW + kw) * 32 + c * 16, i * 32, lane), p);
+          }
         }
       }
     }
@@ -155,7 +171,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(xa_waves<T,
     buf ^= 1;
   }
   l += __shfl_xor(l, 32, 64);
-  if (sizeof(T) == 2) lr += __shfl_xor(lr, 32, 64);
+  if (sizeof(T) == 2 && KW == 1) lr += __shfl_xor(lr, 32, 64);
   else lr = l;
   m = m == -INFINITY ? m : m * scale2 - UP;                   // l and O are sums of 2^(s scale2 - m)
   if (KW > 1) {                                               // the waves of a row tile, joined in order

@@ -527,3 +527,27 @@ def test_fp16_rows_that_one_key_dominates_keep_the_others_weight(dev, queries, k
               cross_attention(q.clone().requires_grad_()[None], k[None], v[None], scale=1.0)):
         off = float((o.detach().double() - want).abs().max())
         assert off < limit
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("frames,lq,lk,h,hk,d", [(4, 1, 5000, 8, 2, 128), (1, 1, 700, 4, 4, 64), (2, 3, 900, 6, 3, 40), (3, 20, 130, 2, 2, 96)])
+def test_few_rows_are_rounded_once(dev, frames, lq, lk, h, hk, d, dtype):
+    """Rows of up to one tile a frame: weights go into their product as two 16-bit numbers, off by (half a step)^2 of themselves
+    (fp16, whose exponents end: or by 2^-36 of the row's largest), and the result is rounded once.  Scores as in the limits above."""
+    from glenet_amd.attention import cross_attention
+    g = torch.Generator().manual_seed(lk)
+    q, k, v = (torch.randn(frames, n, j, d, generator=g).to(dtype).to(dev) for n, j in ((lq, h), (lk, hk), (lk, hk)))
+    kk, vv = (t.double().repeat_interleave(h // hk, 2).permute(0, 2, 1, 3) for t in (k, v))
+    qq = q.double().permute(0, 2, 1, 3)
+    s = torch.stack([a @ b.transpose(-1, -2) for a, b in zip(qq, kk)]) / math.sqrt(d)
+    p = torch.softmax(s, -1)
+    es = (d + 8) * U * qq.norm(dim=-1)[..., None] * kk.norm(dim=-1).amax(-1)[..., None, None] / math.sqrt(d) * 1.5 + 4 * U * s.abs().amax()
+    mass = torch.stack([a @ b.abs() for a, b in zip(p, vv)])
+    want = torch.stack([a @ b for a, b in zip(p, vv)])
+    small = 2 * (2 * es + (16 + lk) * U) + HALF[dtype] ** 2
+    tiny = 2.0 ** -36 * vv.abs().sum(2, keepdim=True) if dtype == torch.float16 else 0.0
+    limit = HALF[dtype] * want.abs() + small * mass + tiny + SUB[dtype]
+    for o in (cross_attention(q, k, v), cross_attention(q.clone().requires_grad_(), k, v)):
+        off = (o.detach().double().permute(0, 2, 1, 3) - want).abs()
+        worst = float((off / limit).max())
+        assert worst <= 1
