@@ -34,6 +34,7 @@
 #define NS_AHEAD 4             // 16-column pieces that each of their 16 waves has on their way
 #define NS_STEPS 64            // at most
 #define NS_PARTS 1024          // partial sums of squares per matrix, at most
+#define NS_BYTES (1ull << 30)  // workspace of the matrices that run together: a list beyond it runs in groups, one behind the other
 
 typedef _Float16 nh8 __attribute__((ext_vector_type(8)));
 typedef _Float16 nh4 __attribute__((ext_vector_type(4)));
@@ -552,9 +553,8 @@ __global__ __launch_bounds__(1024) void k_ns_small(NsSmalls s) {
 // ------------------------------------------------------------------------------------------------ host: programs
 struct NsPlan {                // one matrix
   int rows, cols, m, n, mp, np, tile, xtile, tall, seg, splits, kper, nparts;       // tile: of symmetric products, xtile: of Q X
-  size_t x, xt, x2, xt2, g, h, p[2], q[2], part, parts, xscale;        // byte offsets in the workspace
+  size_t x, xt[2], g, h, p[2], q[2], part, parts, xscale;              // byte offsets in the workspace
 };
-struct NsBounds { double g, p, h, q; };       // of one step of a segment: spectral norms of A, P, H = P A and Q behind the step
 
 static float ns_scale(double bound) { return (float)exp2(floor(log2(32768.0 / bound))); }
 
@@ -583,7 +583,8 @@ static int ns_padded(int v, int tile) { return (v + tile - 1) / tile * tile; }
 // (16 x 64: 13 us in one launch, 81 on the tiles; x 801: 20 and 119; x 4096: 56 and 118; x 16384: 191 and 139)
 static bool ns_small(const glx_matrix& a) { return (a.rows < a.cols ? a.rows : a.cols) <= 16 && a.rows <= 8192 && a.cols <= 8192; }
 
-static NsPlan ns_plan(int rows, int cols, int dtype, int steps, size_t& at) {
+// the plan of one matrix and its places in the workspace from `at` on.  Steep: segments of one step
+static NsPlan ns_plan(int rows, int cols, int dtype, int steps, bool steep, size_t& at) {
   NsPlan p = {};
   p.rows = rows; p.cols = cols; p.tall = rows > cols;
   p.m = p.tall ? cols : rows; p.n = p.tall ? rows : cols;
@@ -595,7 +596,7 @@ static NsPlan ns_plan(int rows, int cols, int dtype, int steps, size_t& at) {
   p.xtile = pad == 128 && wide * across >= 200 ? 128 : 64;
   p.seg = dtype == GLX_BF16 ? 5 : 3;
   // (fp32 rows up to 192: 129 x 1032 comes out 1.6 times as far off as plain fp32 products in segments of three, 0.7 times in ones)
-  if (p.m <= (dtype == GLX_F32 ? 192 : 128) || (dtype == GLX_F32 ? p.n < 4ll * p.m : 4ll * p.n <= 5ll * p.m)) p.seg = 1;
+  if (p.m <= (dtype == GLX_F32 ? 192 : 128) || (dtype == GLX_F32 ? p.n < 4ll * p.m : 4ll * p.n <= 5ll * p.m) || steep) p.seg = 1;
   if (p.seg > steps) p.seg = steps;
   const int t = p.mp / p.tile;
   const long long tiles = (long long)t * (t + 1) / 2, ksteps = p.np / NS_K;
@@ -610,8 +611,11 @@ static NsPlan ns_plan(int rows, int cols, int dtype, int steps, size_t& at) {
   if (p.nparts > NS_PARTS) p.nparts = NS_PARTS;
   const size_t ldn = ns_ld(p.np), ldm = ns_ld(p.mp), X = p.mp * ldn * 4, XT = p.np * ldm * 4, S = p.mp * ldm * 4;
   auto take = [&](size_t bytes) { const size_t o = at; at += glx_align(bytes); return o; };
-  p.x = take(X); p.xt = take(XT); p.x2 = take(X); p.xt2 = take(XT);
-  p.g = take(S); p.h = take(S); p.p[0] = take(S); p.p[1] = take(S); p.q[0] = take(S); p.q[1] = take(S);
+  // X <- Q X reads the transposed planes alone, so X's own are overwritten; H, the second P and the Qs are those of longer segments
+  p.x = take(X); p.xt[0] = take(XT); p.xt[1] = p.seg < steps ? take(XT) : p.xt[0];
+  p.g = take(S); p.p[0] = take(S);
+  if (p.seg > 1) { p.h = take(S); p.p[1] = take(S); p.q[1] = take(S); }
+  if (p.seg > 2) p.q[0] = take(S);
   p.part = take(p.splits > 1 ? (size_t)p.mp * p.mp * 4 * p.splits : 256);
   p.parts = take(NS_PARTS * sizeof(double));
   p.xscale = take(NS_STEPS * sizeof(float));
@@ -629,12 +633,29 @@ static int ns_check(const char* who, const glx_matrix* mats, int count, int dtyp
   return GLX_OK;
 }
 
+// of one matrix, whatever the coefficients
+static size_t ns_bytes(const glx_matrix& a, int dtype, int steps) {
+  size_t usual = 0, steep = 0;
+  ns_plan(a.rows, a.cols, dtype, steps, false, usual);
+  ns_plan(a.rows, a.cols, dtype, steps, true, steep);
+  return usual > steep ? usual : steep;
+}
+// the end of the group that begins at matrix i, and its bytes: one matrix at least, more while they fit NS_BYTES
+static int ns_group(const glx_matrix* mats, int i, int count, int dtype, int steps, size_t* bytes) {
+  *bytes = 256;                                        // (place 0 means none)
+  for (const int first = i; i < count; ++i) {
+    const size_t b = ns_small(mats[i]) ? 0 : ns_bytes(mats[i], dtype, steps);
+    if (i > first && b > 0 && *bytes + b > NS_BYTES) break;
+    *bytes += b;
+  }
+  return i;
+}
+
 extern "C" size_t glx_orthogonalize_workspace_bytes(const glx_matrix* mats, int count, int dtype, int steps) {
   if (ns_check("glx_orthogonalize_workspace_bytes", mats, count, dtype, steps) != GLX_OK) return 0;
-  size_t at = 256;
-  for (int i = 0; i < count; ++i)
-    if (!ns_small(mats[i])) ns_plan(mats[i].rows, mats[i].cols, dtype, steps, at);
-  return at + 256;
+  size_t most = 256, bytes;
+  for (int i = 0; i < count; most = bytes > most ? bytes : most) i = ns_group(mats, i, count, dtype, steps, &bytes);
+  return most + 256;
 }
 
 struct NsStage {               // what one launch round does, over all matrices
@@ -682,41 +703,19 @@ static void ns_launch_small(const std::vector<glx_matrix>& mats, int dtype, int 
   }
 }
 
-extern "C" int glx_orthogonalize(const glx_matrix* list, int listed, int dtype, int steps, const double* coefficients, double eps,
-                                 void* workspace, size_t workspace_bytes, void* stream) try {
-  if (int rc = ns_check("glx_orthogonalize", list, listed, dtype, steps)) return rc;
-  GLX_REQUIRE(coefficients && eps >= 0.0, "glx_orthogonalize: bad coefficients or eps");
-  if (listed == 0) return GLX_OK;
-  std::vector<glx_matrix> mats, small;
-  for (int i = 0; i < listed; ++i) {
-    GLX_REQUIRE(list[i].src && list[i].dst && list[i].ld_src >= list[i].cols && list[i].ld_dst >= list[i].cols,
-                "glx_orthogonalize: matrix %d: null pointer or rows that overlap", i);
-    (ns_small(list[i]) ? small : mats).push_back(list[i]);
-  }
-  const int count = (int)mats.size();
-  std::vector<double> lam, pmax, hmax;
-  GLX_REQUIRE(ns_bounds(steps, coefficients, lam, pmax, hmax),
-              "glx_orthogonalize: these coefficients let singular values grow beyond the arithmetic's range");
-  std::vector<NsPlan> plans;
-  size_t need = 256;                                   // (place 0 means none)
-  double steepest = 1.0;
-  for (double p : pmax) steepest = fmax(steepest, p);
-  for (int i = 0; i < count; ++i) {
-    plans.push_back(ns_plan(mats[i].rows, mats[i].cols, dtype, steps, need));
-    // (a segment's Gram matrix loses its error times the slope squared per step: coefficients steeper than the usual ones, whose
-    // 3.4445 keeps five bfloat16 steps below half a step of the result, take segments of one step)
-    if (steepest > 4.0) plans.back().seg = 1;
-  }
-  GLX_REQUIRE(need < (1ull << 40), "glx_orthogonalize: the list needs a workspace of %zu bytes", need);
-  if (!workspace || workspace_bytes < need) {
-    glx_set_error("glx_orthogonalize: workspace %zu < %zu bytes", workspace_bytes, need);
-    return GLX_EWORKSPACE;
-  }
-  GLX_REQUIRE(((uintptr_t)workspace & 15) == 0, "glx_orthogonalize: the workspace must be 16-byte aligned");
-  hipStream_t st = (hipStream_t)stream;
-  ns_launch_small(small, dtype, steps, coefficients, eps, st);
-  char* ws = (char*)workspace;
+struct NsBounds { std::vector<double> lam, p, h; double steepest; };       // of A, P and P A, step by step (ns_bounds)
+
+// the launches of `count` matrices that share one workspace; their plans lie in it from place 0 on
+static void ns_run(const glx_matrix* mats, int count, int dtype, int steps, const double* coefficients, double eps, const NsBounds& bound,
+                   char* ws, hipStream_t st) {
   const float a = (float)coefficients[0], b = (float)coefficients[1], c = (float)coefficients[2];
+  const std::vector<double>&lam = bound.lam, &pmax = bound.p, &hmax = bound.h;
+  const double steepest = bound.steepest;
+  std::vector<NsPlan> plans;
+  size_t at = 256;
+  // (a segment's Gram matrix loses its error times the slope squared per step: coefficients steeper than the usual ones, whose
+  // 3.4445 keeps five bfloat16 steps below half a step of the result, take segments of one step)
+  for (int i = 0; i < count; ++i) plans.push_back(ns_plan(mats[i].rows, mats[i].cols, dtype, steps, steepest > 4.0, at));
   auto qbound = [&](int s0, int s) { double v = 1; for (int i = s0; i <= s; ++i) v *= pmax[i]; return v; };
 
   for (int i = 0; i < count; i += NS_MATS) {           // |G|_F, then the planes
@@ -734,7 +733,7 @@ extern "C" int glx_orthogonalize(const glx_matrix* list, int listed, int dtype, 
       s.first[s.count] = nb; s.tfirst[s.count] = tb;
       NsMat& t = s.mat[s.count++];
       t.src = mats[j].src; t.ld = mats[j].ld_src;
-      t.x = (_Float16*)(ws + p.x); t.xt = (_Float16*)(ws + p.xt); t.parts = (double*)(ws + p.parts); t.xscale = (float*)(ws + p.xscale);
+      t.x = (_Float16*)(ws + p.x); t.xt = (_Float16*)(ws + p.xt[0]); t.parts = (double*)(ws + p.parts); t.xscale = (float*)(ws + p.xscale);
       t.rows = p.rows; t.cols = p.cols; t.mp = p.mp; t.np = p.np; t.tall = p.tall; t.nparts = p.nparts;
       nb += p.nparts; tb += p.mp / 64 * (p.np / 64);
     }
@@ -768,14 +767,14 @@ extern "C" int glx_orthogonalize(const glx_matrix* list, int listed, int dtype, 
       o.mp = p.mp; o.np = p.mp; o.K = p.mp; o.kper = (unsigned short)(p.mp / NS_K); o.splits = 1; o.kind = NS_PLANES; o.sym = 1;
       return o;
     };
-    size_t x = p.x, xt = p.xt, x2 = p.x2, xt2 = p.xt2;
+    size_t xt = p.xt[0], xt2 = p.xt[1];
     for (int s0 = 0; s0 < steps; s0 += p.seg) {
       const int s1 = s0 + p.seg < steps ? s0 + p.seg : steps;
       const unsigned xs = planes(p.xscale);
       float gs = ns_scale(lam[s0]);
       {                                                // A = X X^T
         NsOp o = {};
-        o.a = o.b = planes(x);
+        o.a = o.b = planes(p.x);
         o.alpha = 1.f; o.scale = gs; o.xin = xs; o.xpow = 2; o.xstep = (unsigned char)s0;
         o.mp = o.np = p.mp; o.K = p.np; o.kper = (unsigned short)(p.kper / NS_K); o.splits = (unsigned short)p.splits; o.sym = 1;
         const int prods = last(s1) || (s0 == 0 && dtype != GLX_F32) ? 1 : full;
@@ -825,11 +824,10 @@ extern "C" int glx_orthogonalize(const glx_matrix* list, int listed, int dtype, 
           o.kind = NS_FINAL; o.dst = mats[i].dst; o.ldd = mats[i].ld_dst;
           o.m = p.m; o.n = p.n; o.tall = (unsigned char)p.tall; o.dtype = (unsigned char)dtype;
         } else {
-          o.kind = NS_XPLANES; o.out = planes(x2); o.out2 = planes(xt2); o.xout = xs; o.xnext = (unsigned char)s1;
+          o.kind = NS_XPLANES; o.out = planes(p.x); o.out2 = planes(xt2); o.xout = xs; o.xnext = (unsigned char)s1;
         }
         stage().add(p.xtile, last(s1) ? 1 : s0 == 0 && dtype != GLX_F32 ? 2 : full, o);
-        size_t y = x; x = x2; x2 = y;
-        y = xt; xt = xt2; xt2 = y;
+        const size_t y = xt; xt = xt2; xt2 = y;
       }
     }
   }
@@ -838,6 +836,39 @@ extern "C" int glx_orthogonalize(const glx_matrix* list, int listed, int dtype, 
       for (int n = 0; n < 4; ++n) ns_launch_ops(g.gemm[t][n], ws, t ? 128 : 64, n + 1, st);
     }
     ns_launch_ops(g.join, ws, 64, 0, st);
+  }
+}
+
+extern "C" int glx_orthogonalize(const glx_matrix* list, int listed, int dtype, int steps, const double* coefficients, double eps,
+                                 void* workspace, size_t workspace_bytes, void* stream) try {
+  if (int rc = ns_check("glx_orthogonalize", list, listed, dtype, steps)) return rc;
+  GLX_REQUIRE(coefficients && eps >= 0.0, "glx_orthogonalize: bad coefficients or eps");
+  if (listed == 0) return GLX_OK;
+  std::vector<glx_matrix> mats, small;
+  size_t need = 256, bytes;
+  for (int i = 0; i < listed; need = bytes > need ? bytes : need) i = ns_group(list, i, listed, dtype, steps, &bytes);
+  for (int i = 0; i < listed; ++i) {
+    GLX_REQUIRE(list[i].src && list[i].dst && list[i].ld_src >= list[i].cols && list[i].ld_dst >= list[i].cols,
+                "glx_orthogonalize: matrix %d: null pointer or rows that overlap", i);
+    (ns_small(list[i]) ? small : mats).push_back(list[i]);
+  }
+  NsBounds bound;
+  GLX_REQUIRE(ns_bounds(steps, coefficients, bound.lam, bound.p, bound.h),
+              "glx_orthogonalize: these coefficients let singular values grow beyond the arithmetic's range");
+  bound.steepest = 1.0;
+  for (double p : bound.p) bound.steepest = fmax(bound.steepest, p);
+  GLX_REQUIRE(need < (1ull << 40), "glx_orthogonalize: a matrix needs a workspace of %zu bytes", need);
+  if (!workspace || workspace_bytes < need) {
+    glx_set_error("glx_orthogonalize: workspace %zu < %zu bytes", workspace_bytes, need);
+    return GLX_EWORKSPACE;
+  }
+  GLX_REQUIRE(((uintptr_t)workspace & 15) == 0, "glx_orthogonalize: the workspace must be 16-byte aligned");
+  hipStream_t st = (hipStream_t)stream;
+  ns_launch_small(small, dtype, steps, coefficients, eps, st);
+  const int count = (int)mats.size();
+  for (int i = 0, to; i < count; i = to) {
+    to = ns_group(mats.data(), i, count, dtype, steps, &bytes);
+    ns_run(mats.data() + i, to - i, dtype, steps, coefficients, eps, bound, (char*)workspace, st);
   }
   GLX_LAUNCH_CHECK();
   return GLX_OK;

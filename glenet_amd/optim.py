@@ -48,7 +48,8 @@ def orthogonalize(mats, steps=5, coefficients=MUON_COEFFICIENTS, eps=1e-7):
     The default coefficients bring singular values from ~1e-3 .. 1 into 0.7 .. 1.2 in five steps.
 
     mats: a device tensor (..., rows, cols), or a list / tuple of 2-D tensors of ANY shapes but one type (float32, bfloat16 or
-    float16) and one device: a list costs as many launches as one matrix (csrc/glx_orthogonal.hip).
+    float16) and one device: a list costs as many launches as one matrix (csrc/glx_orthogonal.hip), one that needs more than 1 GiB
+    of workspace (20 bytes per element and more) as many as its parts of 1 GiB.
     -> new tensors of the same shapes and type (a list for a list), outside autograd; tracing it is refused."""
     who = "orthogonalize"
     steps, coeffs, eps = _check_steps(who, steps, coefficients, eps)

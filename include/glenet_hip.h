@@ -1499,8 +1499,10 @@ int glx_layer_norm_backward(const void* gy, int64_t ldg, const void* x, int64_t 
 /* ---- orthogonalised updates: Newton-Schulz steps on a list of matrices (glenet_amd/optim.py) ----
  * Per matrix: X = src / (|src|_F + eps), transposed where rows > cols; `steps` times  A = X X^T,
  * X = a X + (b A + c A A) X  with coefficients = {a, b, c}; dst = X (transposed back).  src and dst are row-major of `dtype`
- * with ld_src / ld_dst elements between rows; dst may be src.  coefficients and the list are host memory, read during the
- * call.  Coefficients under which singular values leave the arithmetic's range are refused. */
+ * with ld_src / ld_dst elements between rows; dst may be its own src, no other one's.  coefficients and the list are host memory, read during the
+ * call.  Coefficients under which singular values leave the arithmetic's range are refused.  The workspace: 20 bytes per element
+ * of a matrix, padded to tiles, and up to 36 for m x m ones beside wide matrices; a list that needs more than 1 GiB runs in groups
+ * of matrices that share it. */
 typedef struct glx_matrix {
   const void* src; void* dst;
   int64_t ld_src, ld_dst;

@@ -127,3 +127,47 @@ def test_attention_c_entry_refuses():
     assert call(True) == -3                                          # every other check passed
     assert call(q_rows=2, q_len=1) == -3                             # few rows: split over the keys, a workspace
     assert lib.glx_attention_forward(None, None, ctypes.c_size_t(0), None) == -1
+
+
+def test_workspace_of_the_orthogonaliser():
+    """Of one matrix m x n, rows padded to 64 (above 1024: 128) elements and 64 more: X once, its transpose twice, A and P (longer
+    segments: also H, a second P and two Qs) as two 16-bit planes, sums and split products beside them; of a list at most 1 GiB and
+    one matrix."""
+    import ctypes
+
+    from glenet_amd import _lib
+    from glenet_amd.optim import _Matrix
+    lib = _lib.load()
+
+    def need(shapes, dtype=1, steps=5):
+        t = (_Matrix * len(shapes))(*[_Matrix(64, 64, c, c, r, c) for r, c in shapes])
+        return lib.glx_orthogonalize_workspace_bytes(t, len(shapes), dtype, steps)
+
+    small = 1 << 16
+    assert need([(4096, 4096)]) <= 4 * 5 * 4096 * 4160 + small
+    assert need([(4096, 4096)], steps=1) <= 4 * 4 * 4096 * 4160 + small
+    assert need([(8192, 8192)], dtype=0) <= 4 * 5 * 8192 * 8256 + small
+    for dtype in range(3):
+        wide = 4 * (2 * 1280 * 5184 + 5120 * 1344 + 6 * 1280 * 1344)
+        assert need([(1200, 5000)], dtype) <= wide + 4 * 5120 * 1344 + small
+    one = need([(4096, 4096)])
+    assert one <= need([(4096, 4096)] * 3) <= 3 * one
+    assert need([(4096, 4096)] * 300) <= (1 << 30) + small and need([(100, 4096)] * 3000) <= (1 << 30) + small
+    assert need([(20000, 20000)] * 4) == need([(20000, 20000)])             # one of them is beyond it already: one by one
+    assert need([(4096, 4096)] + [(16, 100)] * 50) == one and need([(3, 5)] * 9) <= small
+
+
+def test_orthogonalize_c_entry_asks_for_the_workspace_it_names():
+    import ctypes
+
+    from glenet_amd import _lib
+    from glenet_amd.optim import _Matrix
+    lib = _lib.load()
+    for shapes in ([(4096, 4096)] * 9, [(900, 140)], [(140, 900), (3, 4), (2500, 2500)], [(16, 16)] + [(20000, 20000)]):
+        t = (_Matrix * len(shapes))(*[_Matrix(64, 64, c, c, r, c) for r, c in shapes])
+        named = lib.glx_orthogonalize_workspace_bytes(t, len(shapes), 1, 5)
+        for coeffs in ((3.4445, -4.775, 2.0315), (4.5, -14.58, 9.44784)):
+            rc = lib.glx_orthogonalize(t, len(shapes), 1, 5, (ctypes.c_double * 3)(*coeffs), ctypes.c_double(1e-7), ctypes.c_void_p(256),
+                                       ctypes.c_size_t(0), ctypes.c_void_p(0))
+            asked = int(lib.glx_last_error().decode().split("<")[1].split()[0])
+            assert rc == -3 and asked <= named < asked + 1024

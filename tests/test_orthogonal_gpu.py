@@ -323,3 +323,20 @@ def test_a_matrix_of_few_rows_may_be_overwritten(dev):
         want, buf = _exact(g), g.clone()
         _orthogonalize([buf], steps, coeffs, eps, [buf])
         assert _off(buf, want) < LIMIT[torch.float32]
+
+
+def test_a_list_beyond_one_workspace_runs_in_groups(dev):
+    """17 matrices of 2100 x 2100 need more than 1 GiB side by side; between them small and wide ones, in place and not."""
+    from glenet_amd import _lib
+    from glenet_amd.optim import _Matrix, _check_steps, _orthogonalize, orthogonalize
+    shapes = ([(2100, 2100)] * 5 + [(12, 300), (150, 900)]) * 3 + [(2100, 2100)] * 2
+    mats = [_gradient(r, c, i, dev) for i, (r, c) in enumerate(shapes)]
+    table = (_Matrix * len(shapes))(*[_Matrix(64, 64, c, c, r, c) for r, c in shapes])
+    one = _lib.query("glx_orthogonalize_workspace_bytes", (_Matrix * 1)(_Matrix(64, 64, 2100, 2100, 2100, 2100)), 1, 0, 5)
+    assert _lib.query("glx_orthogonalize_workspace_bytes", table, len(shapes), 0, 5) <= 1 << 30 < 17 * one
+    alone = [orthogonalize(m) for m in mats]
+    for got in (orthogonalize(mats), orthogonalize(mats)):
+        assert all(torch.equal(a, b) for a, b in zip(got, alone))
+    steps, coeffs, eps = _check_steps("test", 5, COEFFS, 1e-7)
+    _orthogonalize(mats, steps, coeffs, eps, mats)
+    assert all(torch.equal(a, b) for a, b in zip(mats, alone))
