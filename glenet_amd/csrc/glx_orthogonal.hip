@@ -16,7 +16,7 @@
 // Products: every operand is held as two fp16 planes of value * 2^k (hi + lo: 22 bits down to 2^-25 of the scale), and a
 // product is three MFMAs hi hi + hi lo + lo hi into fp32.  The scales 2^k come from bounds of the spectral norms that follow
 // from the coefficients (the eigenvalues start in [0, 1]) and from |X_0| = |G| / (|G| + eps), so nothing overflows and a
-// gradient far below eps keeps its precision.
+// gradient far below eps keeps its precision (down to norms of 1e-36).
 // Zero padding to whole tiles is exact: it stays zero in A and X.
 //
 // 4096 x 4096 bf16: 3.57 ms.  A split product of the size of Q X takes 426 us (968 TFLOP/s of fp16 products; a large library
@@ -140,14 +140,15 @@ __global__ __launch_bounds__(256) void k_ns_planes(NsMats s) {
   const int b = blockIdx.x - s.tfirst[k], tiles_n = t.np / 64;
   const double norm = sqrt(red[0]), rho = norm / (norm + s.eps);
   // the planes hold G 2^k with |G| 2^k in [2^14, 2^15): 16-bit values exactly, in the hi plane alone
-  const int k0 = norm > 0.0 ? 14 - ilogb(norm) : 60, kx = k0 > 120 ? 120 : (k0 < -120 ? -120 : k0);
+  const int k0 = norm > 0.0 ? 14 - ilogb(norm) : 60, kx = k0 > 127 ? 127 : (k0 < -120 ? -120 : k0);
   const float up = ldexpf(1.f, kx);
   if (b == 0 && (int)threadIdx.x < s.steps) {
-    // X = planes / xscale; later X in front of step st: min(xb, qb rho) 2^e in [2^14, 2^15)
+    // X = planes / xscale; later X in front of step st: min(xb, qb rho) 2^e in [2^14, 2^15).  (|G| = 1e-36 beside eps = 1e-7 has
+    // e = 110; xscale^2 is infinite from 2^64 on, which makes A, below 2^-100 there, 0)
     const int st = threadIdx.x;
     const float bound = fminf(s.xb[st], (float)(s.qb[st] * rho));
     const int e = bound > 0.f ? 14 - ilogbf(bound) : 60;
-    t.xscale[st] = st == 0 ? (float)((double)up * (norm + s.eps)) : ldexpf(1.f, e > 60 ? 60 : e);
+    t.xscale[st] = st == 0 ? (float)((double)up * (norm + s.eps)) : ldexpf(1.f, e > 120 ? 120 : e);
   }
   const int i0 = b / tiles_n * 64, j0 = b % tiles_n * 64;      // of X
   const int c = threadIdx.x & 63;

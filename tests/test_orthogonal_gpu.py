@@ -340,3 +340,15 @@ def test_a_list_beyond_one_workspace_runs_in_groups(dev):
     steps, coeffs, eps = _check_steps("test", 5, COEFFS, 1e-7)
     _orthogonalize(mats, steps, coeffs, eps, mats)
     assert all(torch.equal(a, b) for a, b in zip(mats, alone))
+
+
+@pytest.mark.parametrize("size", [1e-27, 1e-30, 1e-33, 1e-35])
+def test_gradients_that_vanish_beside_eps(dev, size):
+    """A = X X^T is below 2^-100 there and a step multiplies X by 3.4445: five products of operands of 22 bits, each off by two
+    operands' 2^-22 and the sum's 2^-24, and the division.  Without eps the result does not depend on the size."""
+    from glenet_amd.optim import orthogonalize
+    for shape in ((60, 90), (150, 400), (900, 150), (200, 200)):
+        m = _gradient(*shape, 1, dev) * size
+        off = _off(orthogonalize(m), _exact(m))
+        assert off < 5 * (2 * 2.0 ** -22 + 2.0 ** -24) + 2.0 ** -22, shape
+        assert _off(orthogonalize(m, eps=0.0), _exact(m, eps=0.0)) < LIMIT[torch.float32], shape
