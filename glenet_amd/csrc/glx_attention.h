@@ -205,6 +205,13 @@ struct XaLoad {
     for (int i = 0; i < N; ++i)
       if (!valid(row_of(i))) *reinterpret_cast<vec*>(tile + (threadIdx.x + i * 256) * 16) = vec{};
   }
+  // behind `settle`, of rows that came straight from memory: clears the channels from D on, which repeat the row's first ones.  A
+  // product's zeros on the other side make nothing of them unless they are infinite
+  __device__ __forceinline__ void trim(char* tile, int D) const {
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      if (chunk_of(i) * E >= D) *reinterpret_cast<vec*>(tile + (threadIdx.x + i * 256) * 16) = vec{};
+  }
 };
 
 // ------------------------------------------------------------------------------------------------ frames

@@ -75,8 +75,11 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(xa_waves<T,
     kl.issue(to, kbase + (long long)k0 * a.sk, koff, on, n, a.dim, kdma);
     vl.issue(to + TB, vbase + (long long)k0 * a.sv, voff, on, n, a.dim, vdma);
   };
-  // (masked scores are replaced, so only the values' rows have to be clean)
-  auto settle = [&](char* to) { vl.settle(to + TB, on, nok[0] == ~0ull && nok[BN / 64 - 1] == ~0ull); };
+  // (masked scores are replaced, so only the values' rows have to be clean; a key of -infinity is one of weight 0)
+  auto settle = [&](char* to) {
+    vl.settle(to + TB, on, nok[0] == ~0ull && nok[BN / 64 - 1] == ~0ull);
+    if (kdma && a.dim < DP) kl.trim(to, a.dim);
+  };
   if (t0 < t1) {
     load(t0, smem);
     settle(smem);

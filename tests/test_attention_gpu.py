@@ -551,3 +551,20 @@ def test_few_rows_are_rounded_once(dev, frames, lq, lk, h, hk, d, dtype):
         off = (o.detach().double().permute(0, 2, 1, 3) - want).abs()
         worst = float((off / limit).max())
         assert worst <= 1
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("d", [16, 20, 32, 40, 72, 96, 128])
+def test_a_score_of_minus_infinity_is_a_weight_of_zero(dev, d, dtype):
+    """A state whose product with every query is -infinity weighs nothing, without a mask and at any number of channels."""
+    from glenet_amd.attention import cross_attention
+    g = torch.Generator().manual_seed(d)
+    for lq, lk in ((5, 300), (700, 90)):
+        q, k, v = (torch.randn(1, n, 2, d, generator=g).to(dtype).to(dev) for n in (lq, lk, lk))
+        q[..., 0] = q[..., 0].abs() + 0.5
+        mask = torch.ones(1, lk, dtype=torch.bool, device=dev)
+        mask[0, lk // 3] = mask[0, 0] = False
+        want = cross_attention(q, k, v, key_mask=mask)
+        k[:, lk // 3, :, 0] = k[:, 0, :, 0] = -float("inf")
+        got = cross_attention(q, k, v)
+        assert bool(torch.isfinite(got).all()) and torch.equal(got, want)
