@@ -844,6 +844,11 @@ extern "C" int glx_orthogonalize(const glx_matrix* list, int listed, int dtype, 
                                  void* workspace, size_t workspace_bytes, void* stream) try {
   if (int rc = ns_check("glx_orthogonalize", list, listed, dtype, steps)) return rc;
   GLX_REQUIRE(coefficients && eps >= 0.0, "glx_orthogonalize: bad coefficients or eps");
+  NsBounds bound;
+  GLX_REQUIRE(ns_bounds(steps, coefficients, bound.lam, bound.p, bound.h),
+              "glx_orthogonalize: these coefficients let singular values grow beyond the arithmetic's range");
+  bound.steepest = 1.0;
+  for (double p : bound.p) bound.steepest = fmax(bound.steepest, p);
   if (listed == 0) return GLX_OK;
   std::vector<glx_matrix> mats, small;
   size_t need = 256, bytes;
@@ -853,11 +858,6 @@ extern "C" int glx_orthogonalize(const glx_matrix* list, int listed, int dtype, 
                 "glx_orthogonalize: matrix %d: null pointer or rows that overlap", i);
     (ns_small(list[i]) ? small : mats).push_back(list[i]);
   }
-  NsBounds bound;
-  GLX_REQUIRE(ns_bounds(steps, coefficients, bound.lam, bound.p, bound.h),
-              "glx_orthogonalize: these coefficients let singular values grow beyond the arithmetic's range");
-  bound.steepest = 1.0;
-  for (double p : bound.p) bound.steepest = fmax(bound.steepest, p);
   GLX_REQUIRE(need < (1ull << 40), "glx_orthogonalize: a matrix needs a workspace of %zu bytes", need);
   if (!workspace || workspace_bytes < need) {
     glx_set_error("glx_orthogonalize: workspace %zu < %zu bytes", workspace_bytes, need);

@@ -355,8 +355,8 @@ class FlatMuon(FlatAdamW):
     The factor gives a matrix' step the size that AdamW's has, so one learning rate, decay and beta1 (device scalars, set_lr)
     serve both.  A parameter's matrix is its MEMORY as (rows, cols): shape[0] rows for 2-D to 4-D weights (Linear, Conv1d,
     Conv2d, channels-last ones too: the columns' order does not matter), the last dimension as columns for the 5-D filters of
-    the sparse convolutions (kd, kh, kw, Cin, Cout).  shapes: {parameter: (rows, cols) or None} overrides that; None, vectors
-    and matrices of one row or column take AdamW.  The whole update is recorded into a HIP graph like FlatAdamW's, gradient
+    the sparse convolutions (kd, kh, kw, Cin, Cout).  shapes: {parameter: (rows, cols) or None} overrides that; None, vectors,
+    matrices of one row or column and those beyond orthogonalize's sizes take AdamW.  The whole update is recorded into a HIP graph like FlatAdamW's, gradient
     exchange, state dictionary and buckets included; it is what StaticTrainStep(optimizer=FlatMuon(model.parameters())) steps."""
 
     def __init__(self, params, lr=1e-2, betas=(0.95, 0.99), eps=1e-8, weight_decay=1e-2, max_norm=None, lookahead=True, steps=5,
@@ -395,6 +395,8 @@ class FlatMuon(FlatAdamW):
         tail[:, 3] = torch.tensor([c[2] for c in chunks], dtype=torch.float32).view(torch.int32)
         self._chunks = raw.to(dev)
         self._ns_ws = None
+        # (an empty list: what the coefficients are refused for is said here, not in a step that has moved the moments already)
+        _lib.call_on(dev, "glx_orthogonalize", self._table, 0, 0, self._ns[0], self._ns[1], ctypes.c_double(self._ns[2]), None, _lib.size_arg(0))
         if self._mats:
             self._ns_ws = torch.empty(_lib.query("glx_orthogonalize_workspace_bytes", self._table, self._mats, 0, self._ns[0]),
                                       dtype=torch.uint8, device=dev)

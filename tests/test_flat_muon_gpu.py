@@ -93,3 +93,11 @@ def test_two_ranks_make_the_update_of_one_on_both_gradients(dev, buckets):
     assert sorted(d["rank"] for d in got) == [0, 1]
     for d in got:
         assert d["equal"] and d["scale"] == 0.5 and d["steps"] == 3, d
+
+
+def test_coefficients_are_refused_before_anything_moves(dev):
+    from glenet_amd import _lib
+    from glenet_amd.optim import FlatMuon
+    for coeffs in ((50.0, 0.0, 0.0), (3.4445, -4.775, 9.0)):
+        with pytest.raises(_lib.GlxError, match="range"):
+            FlatMuon(_params(dev), coefficients=coeffs)

@@ -171,3 +171,12 @@ def test_orthogonalize_c_entry_asks_for_the_workspace_it_names():
                                        ctypes.c_size_t(0), ctypes.c_void_p(0))
             asked = int(lib.glx_last_error().decode().split("<")[1].split()[0])
             assert rc == -3 and asked <= named < asked + 1024
+
+
+def test_orthogonalize_c_entry_refuses_coefficients_of_an_empty_list():
+    import ctypes
+
+    from glenet_amd import _lib
+    lib = _lib.load()
+    for coeffs, want in (((3.4445, -4.775, 2.0315), 0), ((50.0, 0.0, 0.0), -1), ((3.4445, -4.775, 9.0), -1)):
+        assert lib.glx_orthogonalize(None, 0, 0, 5, (ctypes.c_double * 3)(*coeffs), ctypes.c_double(1e-7), None, ctypes.c_size_t(0), None) == want
