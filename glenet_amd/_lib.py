@@ -106,7 +106,8 @@ _TRACERS = (torch._C._TorchDispatchModeKey.PROXY, torch._C._TorchDispatchModeKey
 def _refuse_tracing(name):
     """A launch on raw pointers leaves nothing in a trace but the allocation of its results, and a tensor without storage has no
     pointer: neither may pass for a result."""
-    if torch._C._len_torch_dispatch_stack() and any(torch._C._get_dispatch_mode(k) is not None for k in _TRACERS):
+    if (torch._C._get_tracing_state() is not None
+            or torch._C._len_torch_dispatch_stack() and any(torch._C._get_dispatch_mode(k) is not None for k in _TRACERS)):
         raise GlxError("%s cannot be traced: it launches kernels on its tensors' memory" % name)
 
 

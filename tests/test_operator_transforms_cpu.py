@@ -134,3 +134,10 @@ def test_what_launches_on_raw_pointers_is_not_traced():
             orthogonalize([m])
     with pytest.raises(_lib.GlxError, match="cannot be traced"):
         make_fx(lambda t: (_lib.call("glx_abi_version"), t * 2)[1])(torch.ones(3))
+
+
+def test_nor_is_it_by_the_script_tracer():
+    from glenet_amd import _lib
+    with pytest.raises(_lib.GlxError, match="cannot be traced"):
+        torch.jit.trace(lambda t: (_lib.call("glx_abi_version"), t * 2)[1], torch.ones(3))
+    assert torch._C._get_tracing_state() is None

@@ -84,3 +84,27 @@ def test_the_orthogonaliser_is_not_traced(dev):
     with pytest.raises(_lib.GlxError, match="cannot be traced"):
         make_fx(lambda t: orthogonalize(t))(m)
     assert torch.equal(orthogonalize(m), orthogonalize(m))       # (nothing of the trace is left)
+
+
+@pytest.mark.parametrize("name", ["layer_norm", "cross_attention"])
+def test_compiled_and_exported_functions(dev, name):
+    """torch.compile with the operators' own gradients, torch.export and the script tracer: the function's results, to the bit."""
+    f, args = _args(name, torch.float32, dev, 5)
+    leaves = [a.requires_grad_() if a.is_floating_point() else a for a in args]
+    wanted = [a for a in leaves if a.requires_grad]
+
+    def both(g):
+        y = g(*leaves)
+        return [y] + list(torch.autograd.grad(y.sum(), wanted))
+
+    for a, b in zip(both(f), both(torch.compile(f, backend="aot_eager"))):
+        assert torch.equal(a, b)
+
+    class Module(torch.nn.Module):
+        def forward(self, *a):
+            return f(*a)
+
+    with torch.no_grad():
+        want = f(*leaves)
+        assert torch.equal(torch.export.export(Module(), tuple(args)).module()(*args), want)
+        assert torch.equal(torch.jit.trace(f, tuple(args), check_trace=False)(*args), want)
