@@ -13,9 +13,10 @@
 // 1.7e-3, 114.6 us both); with four row tiles it would cost 5 to 7 % (2 x 4096 x 16384, 128 channels: 2.71 -> 2.84 ms a training
 // pass; 6 x 217 x 1531, 40 channels: 27.5 -> 29.4 us).
 //
-// 2 frames of 4096 queries over 16384 keys, 8 heads of 128 on 2 key heads, bf16: 720 us (764 TFLOP/s; a large library product
-// reaches 1156), bound by the exponentials beside the products; one query over each of 4 x 32768 keys, 32 heads on 8: 108 us with
-// the join, 5.0 TB/s of keys and values.
+// 2 frames of 4096 queries over 16384 keys, 8 heads of 128 on 2 key heads, bf16: 734 us (749 TFLOP/s; a large library product
+// reaches 1156).  Of a SIMD's cycles products take 35 % and vector instructions 54 % (ten per product: an exponential, its argument,
+// the maximum, the sum, the rounding), so that they mostly take turns.  One query over each of 4 x 32768 keys, 32 heads on 8: 108 us
+// (5.0 TB/s of keys and values) and 5 us for the join.
 #include "glx_attention.h"
 
 template <typename T, int DP, int RW>

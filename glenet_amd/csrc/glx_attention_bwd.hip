@@ -8,8 +8,9 @@
 // are its sum).  Seven tile products instead of the five of a single pass that would need atomics or a second dQ buffer; the
 // results are the same bits every time.  Few tiles are split over the other side and added by a last launch.
 //
-// 2 frames of 4096 queries over 16384 keys, 8 heads of 128 on 2 key heads, bf16: dQ 837 us (985 TFLOP/s; a large library product
-// reaches 1156), dK / dV 1362 us (808; one wave per SIMD holds K, V, dK and dV, its LDS reads take as long as its products).
+// 2 frames of 4096 queries over 16384 keys, 8 heads of 128 on 2 key heads, bf16: dQ 862 us (957 TFLOP/s; a large library product
+// reaches 1156; products 48 % of a SIMD's cycles, vector instructions 52 %), dK / dV 1395 us (788; products 37 %, vector instructions
+// 35 %: one wave per SIMD holds K, V, dK and dV, its LDS reads take as long as its products).
 //
 // P and dS are rounded to the inputs' type in front of their products.  fp16 would lose both to its range -- over a thousand
 // keys P sits where fp16 has few bits left, and dS inherits the loss' scale -- so P is multiplied by 2^12 and dS by a power of

@@ -9,9 +9,12 @@
 // symmetric products formed once per pair of tiles a segment costs 3 m^2 n + (4 s - 3) m^3 multiply-adds instead of
 // s (3 m^2 n + m^3): the same for square matrices, s times less work on X for wide ones.  What limits s is rounding: a
 // perturbation of A in directions of small singular values grows by a^2 = 11.9 per step until the next look at X.  Measured
-// against 64 bits on gradients with decaying spectra, Frobenius: one step per segment 1e-5, 3 + 2 steps 1e-5, 5 steps 1e-4 to
-// 4e-4.  So fp32 and fp16 matrices take segments of three, bf16 ones (half a step is 4e-3) of five, nearly square ones and those
-// of up to 128 rows (fp32: 192) of one.
+// against 64 bits over six gradients with decaying spectra, in the Frobenius norm and as a multiple of what plain fp32 products leave
+// (1e-6 to 3e-6): fp32 in segments of one step 0.4 to 0.8, of three 0.4 to 1.3 (single ones of 300 x 1500 up to 1.9), and below the
+// limits that follow 1.1 to 2.0 (200 x 300 1.7, 129 x 1032 2.0).  So fp32 takes segments of three above 192 rows and from 4 : 1 on
+// (1000 x 4400: 440 us, in segments of one 634; 200 x 300 would not gain), fp16, whose rounding covers both, three above 128 rows and
+// from 1.25 : 1 on (1000 x 3600: 347 and 471 us; 512 x 600 188 and 179, the other way), bf16 five there (290 and 471 us; 2000 x 2400
+// 1078 and 936; its error up to 1.24 times its rounding's), and the rest one.
 //
 // Products: every operand is held as two fp16 planes of value * 2^k (hi + lo: 22 bits down to 2^-25 of the scale), and a
 // product is three MFMAs hi hi + hi lo + lo hi into fp32.  The scales 2^k come from bounds of the spectral norms that follow
@@ -19,8 +22,8 @@
 // gradient far below eps keeps its precision (down to norms of 1e-36).
 // Zero padding to whole tiles is exact: it stays zero in A and X.
 //
-// 4096 x 4096 bf16: 3.57 ms.  A split product of the size of Q X takes 426 us (968 TFLOP/s of fp16 products; a large library
-// product reaches 1119), a single one 209 us (658: its 64 KB stages wait for their way from L2 to LDS).  256 x 256 fp32: 15 products
+// 4096 x 4096 bf16: 3.54 to 3.7 ms by the box.  A split product of the size of Q X takes 446 us (925 TFLOP/s of fp16 products; a large
+// library product reaches 1119), a single one 212 us (649: its 64 KB stages wait for their way from L2 to LDS).  256 x 256 fp32: 15 products
 // of 8 us each, all latency.
 #include "glx_elem.h"
 
@@ -448,9 +451,9 @@ __global__ __launch_bounds__(256) void k_ns_join(NsOps s) {
 
 // ------------------------------------------------------------------------------------------------ matrices of up to 16 rows
 // One block per matrix, all of it in one launch and in 64 bits: A = X X^T on the fp64 matrix units (one value per lane is both
-// operands), the steps on the 16 x 16 polynomials, X <- Q X.  Few singular values leave nothing to average: on the split products
-// above such a matrix came out up to 3.9 times as far off as with plain fp32 arithmetic (here: 6e-8 of it, a tenth of that), and
-// its some 15 launches were all latency.  Bound by the fp64 matrix units (14 us of 56 at 16 x 4096) and one CU's loads.
+// operands), the steps on the 16 x 16 polynomials, X <- Q X.  Few singular values leave nothing to average: here a
+// matrix is 2e-8 to 4e-8 off, a twentieth of what plain fp32 arithmetic leaves, and on the split products above its some 15
+// launches were all latency.  Bound by the fp64 matrix units (14 us of 56 at 16 x 4096) and one CU's loads.
 typedef double nd4 __attribute__((ext_vector_type(4)));
 struct NsSmall { const void* src; void* dst; long long ld_src, ld_dst; int rows, cols; };
 struct NsSmalls { NsSmall mat[NS_SMALLS]; double c[3], eps; int steps, dtype; };
@@ -596,7 +599,8 @@ static NsPlan ns_plan(int rows, int cols, int dtype, int steps, bool steep, size
   p.tile = pad == 128 && wide * (wide + 1) / 2 >= 200 ? 128 : 64;
   p.xtile = pad == 128 && wide * across >= 200 ? 128 : 64;
   p.seg = dtype == GLX_BF16 ? 5 : 3;
-  // (fp32 rows up to 192: 129 x 1032 comes out 1.6 times as far off as plain fp32 products in segments of three, 0.7 times in ones)
+  // (fp32 rows up to 192: 129 x 1032 comes out 2.0 times as far off as plain fp32 products in segments of three, 0.6 times in ones;
+  // 160 x 800 takes 155 and 158 us)
   if (p.m <= (dtype == GLX_F32 ? 192 : 128) || (dtype == GLX_F32 ? p.n < 4ll * p.m : 4ll * p.n <= 5ll * p.m) || steep) p.seg = 1;
   if (p.seg > steps) p.seg = steps;
   const int t = p.mp / p.tile;
@@ -747,13 +751,14 @@ static void ns_run(const glx_matrix* mats, int count, int dtype, int steps, cons
   for (int i = 0; i < count; ++i) {
     const NsPlan& p = plans[i];
     // bfloat16: single products in the last two steps, where what they lose is no longer amplified (it comes to 1e-3 of the
-    // result, half a step is 4e-3); segments of one step only, and matrices whose time is the products (smaller ones lose up
-    // to 2e-3 where all singular values are alike, 24 x 360, and gain nothing)
+    // result: 4096 x 4096 is 1.86e-3 off, 1.98e-3 where all singular values are alike, with split ones 1.66e-3, its rounding; 3.65
+    // and 4.7 ms); segments of one step only, and matrices whose time is the products (smaller ones lose as much -- 24 x 360 2.0e-3
+    // in all -- and gain nothing)
     auto last = [&](int s1) {
       return dtype == GLX_BF16 && p.seg == 1 && p.m > 1024 && s1 > steps - 2 && steps >= 4 && steepest <= 4.0;
     };
-    // lo lo too: fp32 matrices on 64-wide tiles, whose time is latency and LDS (small ones lose up to 1.6 times a plain fp32
-    // product's error without)
+    // lo lo too: fp32 matrices on 64-wide tiles, whose time is latency and LDS (24 x 360: 0.7 to 0.8 of a plain fp32 product's
+    // error, without 0.9)
     const int full = dtype == GLX_F32 && p.tile == 64 && p.xtile == 64 ? 4 : 3;
     size_t k = 0;
     auto stage = [&]() -> NsStage& {

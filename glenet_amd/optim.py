@@ -50,7 +50,11 @@ def orthogonalize(mats, steps=5, coefficients=MUON_COEFFICIENTS, eps=1e-7):
     mats: a device tensor (..., rows, cols), or a list / tuple of 2-D tensors of ANY shapes but one type (float32, bfloat16 or
     float16) and one device: a list costs as many launches as one matrix (csrc/glx_orthogonal.hip), one that needs more than 1 GiB
     of workspace (20 bytes per element and more) as many as its parts of 1 GiB.
-    -> new tensors of the same shapes and type (a list for a list), outside autograd; tracing it is refused."""
+    -> new tensors of the same shapes and type (a list for a list), outside autograd; tracing it is refused.
+
+    float32 comes out as far from the exact steps as plain fp32 products would leave it (0.2 to 1.3 times), float16 as far as its
+    rounding, bfloat16 up to 1.25 times that: wide matrices take their steps on one Gram matrix, nearly square ones above 1024 rows
+    the last two steps in single 16-bit products."""
     who = "orthogonalize"
     steps, coeffs, eps = _check_steps(who, steps, coefficients, eps)
     if isinstance(mats, torch.Tensor):
